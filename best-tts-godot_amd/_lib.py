@@ -120,6 +120,13 @@ PROTOTYPES = {
     "kk_fir": [_T, _T, _T, _i],
     "kk_pcm16": [_T, _T, _f],
     "kk_fir_pcm16": [_T, _T, _T, _i, _f],
+    "kk_qk_norm_rotary": [_T] * 8 + [_f, _i, _f],
+    "kk_cache_append": [_T] * 9,
+    "kk_cache_attention": [_T] * 9 + [_f, ctypes.c_int64],
+    "kk_cross_attention": [_T] * 6 + [_f],
+    "kk_process_logits": [_T] * 9,
+    "kk_stream_wait": [_vp],
+    "kk_stream_signal": [_vp],
     "kk_graph_begin": [],
     "kk_graph_begin_arena": [_sz],
     "kk_graph_abort": [],

@@ -1,0 +1,272 @@
+// Attention of a token decoder: over a paged cache of 8-bit codes, and over
+// an encoder's states.
+#include "kk_decode.h"
+
+namespace kk {
+
+constexpr int kMaxHead = 256;
+
+// Queries and outputs: [B, T, heads, D], group query heads a key head.
+struct QueryArgs {
+  const void* q;
+  void* y;
+  int64_t qs[3], ys[3];
+  int64_t B;
+  int T, heads, group, D;
+  float scale;  // times log2 e: the softmax is formed from powers of two
+};
+
+// Keys and values of one piece each: [B, S, key heads, D].
+struct DenseArgs {
+  const void *k, *v;
+  int64_t ks[4], vs[4];
+  int64_t S;
+  const void* lengths;
+  int lengths_dt;
+  int64_t lengths_st;
+  const uint8_t* mask;
+  int64_t ms[3];
+};
+
+struct PagedArgs {
+  const int8_t *k, *v;
+  const float *k_scale, *v_scale;
+  const int32_t* table;
+  int64_t table_stride, pages, columns;
+  const void *lengths, *counts;
+  int lengths_dt, counts_dt;
+  int64_t lengths_st, counts_st, window;
+  int heads, block;
+};
+
+// What the query t of sequence b sees, and the score of one token.
+template <typename T>
+struct DenseRows {
+  DenseArgs a;
+  __device__ Seen seen(int64_t b, int64_t) const {
+    int64_t n = a.S;
+    if (a.lengths) {
+      const int64_t l = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
+      n = l < 0 ? 0 : (l < n ? l : n);
+    }
+    return Seen{0, n};
+  }
+  __device__ bool sees(int64_t b, int64_t t, int64_t j) const {
+    return !a.mask || a.mask[b * a.ms[0] + t * a.ms[1] + j * a.ms[2]] != 0;
+  }
+  __device__ float key(int64_t b, int h, int64_t j, int d) const {
+    return to_f32(static_cast<const T*>(a.k)[b * a.ks[0] + j * a.ks[1] + h * a.ks[2] + d * a.ks[3]]);
+  }
+  __device__ float value(int64_t b, int h, int64_t j, int d) const {
+    return to_f32(static_cast<const T*>(a.v)[b * a.vs[0] + j * a.vs[1] + h * a.vs[2] + d * a.vs[3]]);
+  }
+};
+
+struct PagedRows {
+  PagedArgs a;
+  int T, D;
+  __device__ Seen seen(int64_t b, int64_t t) const {
+    int64_t n = T;
+    if (a.counts) {
+      const int64_t c = load_index(a.counts, a.counts_dt, b * a.counts_st);
+      n = c < 0 ? 0 : (c < n ? c : n);
+    }
+    const int64_t len = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
+    const int64_t place = (len < 0 ? 0 : len) - n + t;
+    return seen_tokens(t < n ? place : -1, a.window, a.columns * a.block);
+  }
+  __device__ int64_t page(int64_t b, int64_t j) const {
+    const int64_t p = a.table[b * a.table_stride + j / a.block];
+    return p < a.pages ? p : -1;
+  }
+  __device__ bool sees(int64_t b, int64_t, int64_t j) const { return page(b, j) >= 0; }
+  __device__ float key(int64_t b, int h, int64_t j, int d) const {
+    const int64_t p = page(b, j) * a.heads + h;
+    return static_cast<float>(a.k[(p * a.block + j % a.block) * D + d]) * a.k_scale[p];
+  }
+  __device__ float value(int64_t b, int h, int64_t j, int d) const {
+    const int64_t p = page(b, j) * a.heads + h;
+    return static_cast<float>(a.v[(p * D + d) * a.block + j % a.block]) * a.v_scale[p];
+  }
+};
+
+constexpr int kRowWaves = 4;
+
+// One wave a query: a lane scores one of 64 tokens, then owns every 64th
+// value of the output.  Right for every size, stride and type.
+template <typename T, class Rows>
+__global__ void __launch_bounds__(kRowWaves * 64) attention_row_kernel(QueryArgs a, Rows rows, int64_t queries) {
+  __shared__ float qv[kRowWaves][kMaxHead];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;
+  if (at >= queries) return;  // (no barrier below: a wave keeps to its own row of qv)
+  const int head = static_cast<int>(at % a.heads), h = head / a.group;
+  const int64_t t = at / a.heads % a.T, b = at / a.heads / a.T;
+  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
+  for (int d = lane; d < a.D; d += 64) qv[wave][d] = to_f32(q[d]);
+  __builtin_amdgcn_wave_barrier();
+  const Seen w = rows.seen(b, t);
+  float m = -INFINITY, l = 0.0f, acc[kMaxHead / 64] = {};
+  for (int64_t j0 = w.lo; j0 < w.hi; j0 += 64) {
+    const int64_t j = j0 + lane;
+    const bool sees = j < w.hi && rows.sees(b, t, j);
+    float s = 0.0f;
+    if (sees)
+      for (int d = 0; d < a.D; ++d) s = __builtin_fmaf(qv[wave][d], rows.key(b, h, j, d), s);
+    s = sees ? s * a.scale : -INFINITY;
+    const float next = fmaxf(fmaxf(m, wave_max(s)), -3.4028235e38f);
+    const float keep = exp2f(m - next), p = exp2f(s - next);
+    m = next;
+    l = l * keep + wave_sum(p);
+#pragma unroll
+    for (int i = 0; i < kMaxHead / 64; ++i) acc[i] *= keep;
+    uint64_t live = __ballot(sees);
+    while (live) {
+      const int e = __builtin_ctzll(live);
+      live &= live - 1;
+      const float pe = __shfl(p, e, 64);
+#pragma unroll
+      for (int i = 0; i < kMaxHead / 64; ++i)
+        if (lane + 64 * i < a.D) acc[i] = __builtin_fmaf(pe, rows.value(b, h, j0 + e, lane + 64 * i), acc[i]);
+    }
+  }
+  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 64; ++i)
+    if (lane + 64 * i < a.D) from_f32(y[lane + 64 * i], l != 0.0f ? acc[i] / l : 0.0f);
+}
+
+template <typename T, class Rows>
+static int launch_rows(const QueryArgs& a, const Rows& rows) {
+  const int64_t queries = a.B * a.T * a.heads, blocks = ceil_div(queries, kRowWaves);
+  if (blocks > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "attention: too many queries");
+  KK_LAUNCH((attention_row_kernel<T, Rows>), dim3(static_cast<unsigned>(blocks)), dim3(kRowWaves * 64), 0,
+            ctx().stream, a, rows, queries);
+  return check_launch("attention_row_kernel");
+}
+
+static int check_queries(const kk_tensor* out, const kk_tensor* q, int64_t key_heads, int64_t D, float scale,
+                         QueryArgs* a, const char* who) {
+  KK_TRY(check_heads(q, "q", who));
+  KK_TRY(check_heads(out, "out", who));
+  KK_TRY(check_writable(out, "out", who));
+  if (out->dtype != q->dtype) return set_error(KK_E_ARG, "%s: out must have q's dtype", who);
+  for (int i = 0; i < 4; ++i)
+    if (out->shape[i] != q->shape[i]) return set_error(KK_E_ARG, "%s: out must have q's shape", who);
+  if (q->shape[3] != D)
+    return set_error(KK_E_ARG, "%s: queries of %lld values over keys of %lld", who,
+                     static_cast<long long>(q->shape[3]), static_cast<long long>(D));
+  if (key_heads < 1 || q->shape[2] % key_heads)
+    return set_error(KK_E_ARG, "%s: %lld query heads are not a multiple of %lld key heads", who,
+                     static_cast<long long>(q->shape[2]), static_cast<long long>(key_heads));
+  if (q->shape[1] > 0x7fffffff || q->shape[2] > 65535)
+    return set_error(KK_E_UNSUPPORTED, "%s: too many queries", who);
+  if (!(scale == scale) || scale == INFINITY || scale == -INFINITY)
+    return set_error(KK_E_ARG, "%s: scale must be finite", who);
+  a->q = q->data;
+  a->y = out->data;
+  for (int i = 0; i < 3; ++i) {
+    a->qs[i] = q->strides[i];
+    a->ys[i] = out->strides[i];
+  }
+  a->B = q->shape[0];
+  a->T = static_cast<int>(q->shape[1]);
+  a->heads = static_cast<int>(q->shape[2]);
+  a->group = static_cast<int>(q->shape[2] / key_heads);
+  a->D = static_cast<int>(D);
+  a->scale = scale * 0x1.715476p+0f;
+  return KK_OK;
+}
+
+}  // namespace kk
+
+using namespace kk;
+
+extern "C" {
+
+int kk_cache_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k_codes,
+                       const kk_tensor* k_scales, const kk_tensor* v_codes, const kk_tensor* v_scales,
+                       const kk_tensor* table, const kk_tensor* lengths, const kk_tensor* counts, float scale,
+                       int64_t window) {
+  const char* who = "cache_attention";
+  CacheShape c;
+  KK_TRY(check_cache(k_codes, k_scales, v_codes, v_scales, table, &c, who));
+  QueryArgs a{};
+  KK_TRY(check_queries(out, q, c.heads, c.D, scale, &a, who));
+  if (table->shape[0] != a.B) return set_error(KK_E_ARG, "%s: table must have a row a sequence", who);
+  KK_TRY(check_per_row(lengths, "lengths", a.B, true, who));
+  if (counts) KK_TRY(check_per_row(counts, "counts", a.B, true, who));
+  if (window < 0) return set_error(KK_E_ARG, "%s: window must not be negative", who);
+  PagedArgs p{};
+  p.k = static_cast<const int8_t*>(k_codes->data);
+  p.v = static_cast<const int8_t*>(v_codes->data);
+  p.k_scale = static_cast<const float*>(k_scales->data);
+  p.v_scale = static_cast<const float*>(v_scales->data);
+  p.table = static_cast<const int32_t*>(table->data);
+  p.table_stride = c.table_stride;
+  p.pages = c.pages;
+  p.columns = c.columns;
+  p.lengths = lengths->data;
+  p.lengths_dt = lengths->dtype;
+  p.lengths_st = row_stride(lengths);
+  if (counts) {
+    p.counts = counts->data;
+    p.counts_dt = counts->dtype;
+    p.counts_st = row_stride(counts);
+  }
+  p.window = window;
+  p.heads = static_cast<int>(c.heads);
+  p.block = static_cast<int>(c.block);
+  KK_TRY(require_ready());
+  if (a.B * a.T * a.heads == 0) return KK_OK;
+  const PagedRows rows{p, a.T, a.D};
+  return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
+}
+
+int kk_cross_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k, const kk_tensor* v,
+                       const kk_tensor* lengths, const kk_tensor* mask, float scale) {
+  const char* who = "cross_attention";
+  KK_TRY(check_heads(k, "k", who));
+  KK_TRY(check_heads(v, "v", who));
+  QueryArgs a{};
+  KK_TRY(check_queries(out, q, k->shape[2], k->shape[3], scale, &a, who));
+  if (a.D < 1 || a.D > kMaxHead)
+    return set_error(KK_E_UNSUPPORTED, "%s: heads of %d values (1 to %d)", who, a.D, kMaxHead);
+  if (k->dtype != q->dtype || v->dtype != q->dtype)
+    return set_error(KK_E_ARG, "%s: q, k and v must have one dtype", who);
+  for (int i = 0; i < 4; ++i)
+    if (k->shape[i] != v->shape[i]) return set_error(KK_E_ARG, "%s: k and v must have one shape", who);
+  if (k->shape[0] != a.B) return set_error(KK_E_ARG, "%s: k must have q's sequences", who);
+  DenseArgs d{};
+  d.k = k->data;
+  d.v = v->data;
+  d.S = k->shape[1];
+  for (int i = 0; i < 4; ++i) {
+    d.ks[i] = k->strides[i];
+    d.vs[i] = v->strides[i];
+  }
+  if (lengths) {
+    KK_TRY(check_per_row(lengths, "lengths", a.B, true, who));
+    d.lengths = lengths->data;
+    d.lengths_dt = lengths->dtype;
+    d.lengths_st = row_stride(lengths);
+  }
+  if (mask) {
+    KK_TRY(check_tensor(mask, "mask"));
+    const int r = mask->rank;
+    if ((mask->dtype != KK_BOOL && mask->dtype != KK_U8) || r < 2 || r > 3 ||
+        (mask->shape[0] != a.B && mask->shape[0] != 1) ||
+        (r == 3 && mask->shape[1] != a.T && mask->shape[1] != 1) || mask->shape[r - 1] != d.S)
+      return set_error(KK_E_ARG, "%s: mask must be bool [sequences, states] or [sequences, tokens, states]", who);
+    d.mask = static_cast<const uint8_t*>(mask->data);
+    d.ms[0] = mask->shape[0] > 1 ? mask->strides[0] : 0;
+    d.ms[1] = r == 3 && mask->shape[1] > 1 ? mask->strides[1] : 0;
+    d.ms[2] = mask->strides[r - 1];
+  }
+  KK_TRY(require_ready());
+  if (a.B * a.T * a.heads == 0) return KK_OK;
+  return q->dtype == KK_F16 ? launch_rows<__half>(a, DenseRows<__half>{d})
+                            : launch_rows<float>(a, DenseRows<float>{d});
+}
+
+}  // extern "C"

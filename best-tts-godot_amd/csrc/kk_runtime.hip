@@ -747,6 +747,29 @@ int kk_event_elapsed(int a, int b, float* ms) {
   return KK_OK;
 }
 
+// `after` waits for what `before` holds: an event that lives for the call (a
+// recorded event that is destroyed is released when it has completed).
+static int order_streams(hipStream_t before, hipStream_t after) {
+  hipEvent_t ev;
+  KK_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+  hipError_t e = hipEventRecord(ev, before);
+  if (e == hipSuccess) e = hipStreamWaitEvent(after, ev, 0);
+  (void)hipEventDestroy(ev);
+  return check_hip(e, "ordering two streams");
+}
+
+int kk_stream_wait(void* stream) {
+  KK_TRY(require_ready());
+  KK_TRY(not_capturing("kk_stream_wait"));
+  return order_streams(static_cast<hipStream_t>(stream), ctx().stream);
+}
+
+int kk_stream_signal(void* stream) {
+  KK_TRY(require_ready());
+  KK_TRY(not_capturing("kk_stream_signal"));
+  return order_streams(ctx().stream, static_cast<hipStream_t>(stream));
+}
+
 int kk_graph_begin(void) {
   KK_TRY(require_ready());
   KK_TRY(not_capturing("kk_graph_begin"));

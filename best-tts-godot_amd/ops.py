@@ -569,3 +569,77 @@ def fir_pcm16(x, taps, center=-1, gain=1.0):
     _lib.call("kk_fir_pcm16", out.desc(), x.desc(), taps.contiguous().desc(), int(center),
               float(gain))
     return out
+
+
+# ------------------------------------------------------------ token decoder
+# (a copy that _inner or _flat makes must be held until the call: its buffer goes back to the pool with it)
+def _inner(t):
+    """t with its last axis in one piece."""
+    return t if t is None or t.shape[-1] == 1 or t.strides[-1] == 1 else t.contiguous()
+
+
+def _flat(t):
+    return None if t is None else t.contiguous()
+
+
+def qk_norm_rotary(q, k, positions=None, turns=None, q_weight=None, k_weight=None, eps=1e-6,
+                   interleaved=False, amplitude=1.0):
+    """(q, k) with each head's norm (where a weight [D] is given) and the
+    position rotation (where `turns` is: rotary_turns) in one pass; q
+    [B, T, Hq, D] and k [B, T, Hk, D] or None, positions int32 / int64 [T] or
+    [B, T]."""
+    q, k, turns = _inner(q), _inner(k), _flat(turns)
+    q_weight, k_weight = _flat(q_weight), _flat(k_weight)
+    out_q = DeviceTensor.empty(q.shape, q.dtype)
+    out_k = None if k is None else DeviceTensor.empty(k.shape, k.dtype)
+    _lib.call("kk_qk_norm_rotary", out_q.desc(), _d(out_k), q.desc(), _d(k), _d(q_weight), _d(k_weight),
+              _d(positions), _d(turns), float(eps), int(bool(interleaved)), float(amplitude))
+    return out_q, out_k
+
+
+def rotary(x, positions, turns, interleaved=False, amplitude=1.0):
+    """The position rotation alone of x [B, T, H, D]."""
+    return qk_norm_rotary(x, None, positions, turns, interleaved=interleaved, amplitude=amplitude)[0]
+
+
+def cache_append(cache, k, v, table, starts, counts=None):
+    """Keys and values [B, T, Hk, D] into a KVCache: tokens 0 .. counts[b] - 1
+    of sequence b at its places starts[b] on, in the pages of table [B, pages]."""
+    k, v, table = _inner(k), _inner(v), _inner(table)
+    _lib.call("kk_cache_append", cache.k.desc(), cache.k_scale.desc(), cache.v.desc(), cache.v_scale.desc(),
+              k.desc(), v.desc(), table.desc(), starts.desc(), _d(counts))
+
+
+def cache_attention(q, cache, table, lengths, counts=None, scale=None, window=0):
+    """Causal attention of q [B, T, Hq, D], the newest counts[b] (T) of the
+    lengths[b] tokens of each sequence, over a KVCache; scale 1 / sqrt(D)
+    where None, window 0 for all tokens."""
+    q, table = _inner(q), _inner(table)
+    out = DeviceTensor.empty(q.shape, q.dtype)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _lib.call("kk_cache_attention", out.desc(), q.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
+              cache.v_scale.desc(), table.desc(), lengths.desc(), _d(counts), scale, int(window))
+    return out
+
+
+def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
+    """Attention of q [B, T, Hq, D] over an encoder's states k, v
+    [B, S, Hk, D]: those below lengths[b] whose mask (bool [B, S] or
+    [B, T, S]) is set; scale 1 / sqrt(D) where None."""
+    q, k, v = _inner(q), _inner(k), _inner(v)
+    out = DeviceTensor.empty(q.shape, q.dtype)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _lib.call("kk_cross_attention", out.desc(), q.desc(), k.desc(), v.desc(), _d(lengths), _d(mask), scale)
+    return out
+
+
+def process_logits(logits, history=None, history_lengths=None, repetition=None, presence=None, frequency=None,
+                   bias=None, allowed=None):
+    """Logits [B, V] with the penalties of tokens in history [B, L], the bias
+    [V] or [B, V] and the grammar's mask (bits of int32 words; allowed_bits),
+    as float32."""
+    logits, history, bias, allowed = _inner(logits), _inner(history), _inner(bias), _inner(allowed)
+    out = DeviceTensor.empty(logits.shape, np.float32)
+    _lib.call("kk_process_logits", out.desc(), logits.desc(), _d(history), _d(history_lengths), _d(repetition),
+              _d(presence), _d(frequency), _d(bias), _d(allowed))
+    return out

@@ -96,6 +96,30 @@ class Storage:
                 pass
 
 
+class Borrowed:
+    """Device memory of another library's array, which is kept alive."""
+
+    __slots__ = ("ptr", "nbytes", "owner")
+
+    def __init__(self, ptr, nbytes, owner):
+        self.ptr = ptr
+        self.nbytes = nbytes
+        self.owner = owner
+
+
+def wait_stream(stream=0):
+    """Work given to libkk from here on starts after what `stream` (a HIP
+    stream's handle, 0 the default stream; torch: `s.cuda_stream`) holds now."""
+    init()
+    _lib.call("kk_stream_wait", int(stream))
+
+
+def signal_stream(stream=0):
+    """Work given to `stream` from here on starts after what libkk holds now."""
+    init()
+    _lib.call("kk_stream_signal", int(stream))
+
+
 _PROTOS = {}  # (shape, strides, dtype) -> KKTensor with data unset
 
 
@@ -158,6 +182,44 @@ class DeviceTensor:
             _lib.call("kk_upload", ctypes.c_void_p(t.ptr),
                       arr.ctypes.data_as(ctypes.c_void_p), arr.nbytes)
         return t
+
+    @classmethod
+    def from_array(cls, arr, stream=None):
+        """A tensor over the memory of a device array of another library (one
+        with `__cuda_array_interface__`, as torch's and cupy's have): no copy,
+        any strides, `arr` kept alive.  libkk has a stream of its own: with
+        `stream` (see wait_stream), or where the array names its stream,
+        libkk's later work waits for what that stream holds; otherwise the
+        values must be there already.  Memory that its owner may hand out
+        again must be kept until libkk has used it (sync or signal_stream)."""
+        desc = arr.__cuda_array_interface__
+        dtype = np.dtype(desc["typestr"])
+        if dtype not in NP_TO_CODE:
+            raise TypeError(f"unsupported dtype {dtype}")
+        if desc.get("mask") is not None:
+            raise TypeError("masked arrays are not supported")
+        shape = tuple(map(int, desc["shape"]))
+        strides = desc.get("strides")
+        if strides is not None:
+            if any(st % dtype.itemsize for st in strides):
+                raise ValueError(f"strides {strides} are not whole elements of {dtype}")
+            strides = [st // dtype.itemsize for st in strides]
+        if stream is None and desc.get("stream") is not None:
+            # the interface's names of the default and the per-thread stream are HIP's handles but for 1
+            stream = 0 if desc["stream"] == 1 else desc["stream"]
+        if stream is not None:
+            wait_stream(stream)
+        t = cls(Borrowed(int(desc["data"][0] or 0), math.prod(shape) * dtype.itemsize, arr), shape, dtype, strides)
+        return t
+
+    @property
+    def __cuda_array_interface__(self):
+        """This tensor's memory for another library (torch.as_tensor(t,
+        device="cuda") makes a view that keeps it alive).  Not synchronised:
+        call sync(), or signal_stream() with the stream that reads it."""
+        item = self.dtype.itemsize
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr if self.size else 0, False),
+                "strides": None if self.is_contiguous() else tuple(st * item for st in self.strides), "version": 2}
 
     # ------------------------------------------------------------ queries
     @property

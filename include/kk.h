@@ -484,6 +484,84 @@ int kk_pcm16(const kk_tensor* out_bytes, const kk_tensor* x, float gain);
 int kk_fir_pcm16(const kk_tensor* out_bytes, const kk_tensor* x, const kk_tensor* taps,
                  int center, float gain);
 
+/* ------------------------------------------------------- token decoder
+ * The steps of an autoregressive decoder that writes tokens from an encoder's
+ * states.  No counterpart in the reference, whose graph writes all frames at
+ * once.  f32 or f16 operands, sums, norms and softmax statistics in fp32, one
+ * rounding at the end.  Arguments that HIP cannot check (places in tables,
+ * lengths, positions) may hold anything: what lies outside is left out.  None
+ * of these allocates, and all may be recorded into a graph. */
+
+/* Norms of the queries' and keys' heads with the position rotation in the
+ * same pass.  q [B, T, Hq, D] and k [B, T, Hk, D] (NULL: q alone), f32 or f16
+ * of any strides but over a head's values, 1 <= D <= 256; out_q and out_k of
+ * their shapes and dtype, each its input where it is to be overwritten.
+ *   y = x / sqrt(mean(x^2) + eps) * weight    (weight [D]; NULL: y = x)
+ * then pair i of a head's first 2R values, R = numel(turns), turns by the angle
+ * 2 pi (p * turns[i] mod 2^64) / 2^64 at position p, times `amplitude`:
+ *   (a, b) -> amplitude (a cos - b sin, b cos + a sin)
+ * where the pair is (i, i + R), or (2i, 2i + 1) if `interleaved`; the values
+ * past 2R pass.  turns: int64 [R], what a position turns, in 2^64ths of a turn
+ * (any scaling of the frequencies is in them; the product wraps, so that far
+ * positions lose nothing); NULL: norms alone.  positions: int32 or int64, [T] or
+ * [B, T] (extents of 1 broadcast). */
+int kk_qk_norm_rotary(const kk_tensor* out_q, const kk_tensor* out_k, const kk_tensor* q,
+                      const kk_tensor* k, const kk_tensor* q_weight, const kk_tensor* k_weight,
+                      const kk_tensor* positions, const kk_tensor* turns, float eps,
+                      int interleaved, float amplitude);
+
+/* A cache of keys and values in 8 bits: pages of `block` tokens (16, 32, 64, 128 or
+ * 256) with a scale for each page and head, a value being code * scale.
+ *   k_codes int8 [pages, Hk, block, D]   v_codes int8 [pages, Hk, D, block]
+ *   k_scales, v_scales f32 [pages, Hk]   D 16 to 256 in steps of 16
+ * (the values' tokens lie next to each other: the order in which attention
+ * sums over them).  table int32 [B, columns]: token j of sequence b lies in
+ * page table[b, j / block], row j % block.
+ *
+ * kk_cache_append puts tokens 0 .. counts[b] - 1 of k and v [B, T, Hk, D] at places
+ * starts[b] on (starts, counts int32 or int64 [B] or [1]; counts NULL: T each).  A
+ * page's scale becomes s' = max(s, largest |x| / 127) where the page holds tokens
+ * before starts[b], whose codes become rint(code * (s / s')), and largest |x| / 127
+ * where it holds none; a new code is rint(x / s'), of the exact quotient, ties to
+ * even.  Infinities saturate and count for no scale, NaN is 0.  A negative start,
+ * tokens past the table's columns and pages outside 0 .. pages - 1 are left
+ * out.  No page may be written for two sequences in one call. */
+int kk_cache_append(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                    const kk_tensor* v_scales, const kk_tensor* k, const kk_tensor* v,
+                    const kk_tensor* table, const kk_tensor* starts, const kk_tensor* counts);
+/* Attention over such a cache: q and out [B, T, Hq, D], Hq a multiple of Hk
+ * (query head h reads key head h / (Hq / Hk)).  lengths[b] tokens are cached,
+ * the counts[b] (NULL: T) newest of them q's own: query t is at place
+ * p = lengths[b] - counts[b] + t and sees the places max(0, p - window + 1) .. p
+ * (window 0: all up to p) whose pages are within 0 .. pages - 1.
+ *   out = sum_j softmax_j(scale q . k_j) v_j
+ * Queries that see nothing (also t >= counts[b]) give zeros. */
+int kk_cache_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k_codes,
+                       const kk_tensor* k_scales, const kk_tensor* v_codes,
+                       const kk_tensor* v_scales, const kk_tensor* table, const kk_tensor* lengths,
+                       const kk_tensor* counts, float scale, int64_t window);
+/* Attention over an encoder's states: q and out [B, T, Hq, D], k and v
+ * [B, S, Hk, D], all of one dtype, any strides but over a head's values,
+ * 1 <= D <= 256.  Query t sees the states j < lengths[b] (NULL: S) with
+ * mask[b, t, j] nonzero (bool [B, S] or [B, T, S], extents of 1 broadcast over B
+ * and T; NULL: all); whatever lies at the others, NaN and infinities
+ * included, does not count.  Queries that see nothing give zeros. */
+int kk_cross_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k,
+                       const kk_tensor* v, const kk_tensor* lengths, const kk_tensor* mask,
+                       float scale);
+/* Penalties, biases and a grammar's mask on logits [B, V] (f32 or f16), into
+ * out f32 [B, V].  With c the times a token stands in history[b, :history_lengths[b]]
+ * (int32 or int64 [B, L]; lengths NULL: L; entries outside 0 .. V - 1 count for none):
+ *   c > 0:  x = x > 0 ? x / repetition : x * repetition;  x -= frequency c + presence
+ *   x += bias;   x = -inf where the token's bit of `allowed` is 0
+ * repetition, presence, frequency f32 [B] or [1] (NULL: 1, 0, 0; they need the history);
+ * bias f32 [V] or [B, V]; allowed int32 [W] or [B, W], W = ceil(V / 32), token v
+ * the bit v % 32 of word v / 32.  Either may be NULL. */
+int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_tensor* history,
+                      const kk_tensor* history_lengths, const kk_tensor* repetition,
+                      const kk_tensor* presence, const kk_tensor* frequency, const kk_tensor* bias,
+                      const kk_tensor* allowed);
+
 /* -------------------------------------------------------------- timing
  * HIP events on the library stream, for measuring kernels where they run.
  * Slots 0..KK_MAX_EVENTS-1.  No counterpart in the reference, which has no
@@ -491,6 +569,16 @@ int kk_fir_pcm16(const kk_tensor* out_bytes, const kk_tensor* x, const kk_tensor
 #define KK_MAX_EVENTS 16
 int kk_event_record(int slot);
 int kk_event_elapsed(int start_slot, int stop_slot, float* ms);
+
+/* ------------------------------------------------ streams of other libraries
+ * libkk's stream does not wait for the default stream.  Tensors of another
+ * library are handed over in both directions with these: what libkk is given
+ * after kk_stream_wait starts after all that `stream` (a hipStream_t, NULL
+ * the default stream) holds at the call, and what `stream` is given after
+ * kk_stream_signal starts after all that libkk holds.  Neither blocks the
+ * host.  Not while a graph is being recorded. */
+int kk_stream_wait(void* stream);
+int kk_stream_signal(void* stream);
 
 /* ---------------------------------------------------------- HIP graphs
  * Records the ops called between kk_graph_begin and kk_graph_end on the
