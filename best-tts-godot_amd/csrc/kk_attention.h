@@ -1,0 +1,292 @@
+// What the attention kernels share: their operands, what a query sees, the cut
+// of long sequences over blocks and the join of the parts.
+#pragma once
+
+#include "kk_decode.h"
+
+namespace kk {
+
+constexpr int kMaxHead = 256;
+
+// Queries and outputs: [B, T, heads, D], group query heads a key head.
+struct QueryArgs {
+  const void* q;
+  void* y;
+  int64_t qs[3], ys[3];
+  int64_t B;
+  int T, heads, group, D;
+  float scale;  // times log2 e: the softmax is formed from powers of two
+};
+
+// Keys and values of one piece each: [B, S, key heads, D].
+struct DenseArgs {
+  const void *k, *v;
+  int64_t ks[4], vs[4];
+  int64_t S;
+  const void* lengths;
+  int lengths_dt;
+  int64_t lengths_st;
+  const uint8_t* mask;
+  int64_t ms[3];
+};
+
+struct PagedArgs {
+  const int8_t *k, *v;
+  const float *k_scale, *v_scale;
+  const int32_t* table;
+  int64_t table_stride, pages, columns;
+  const void *lengths, *counts;
+  int lengths_dt, counts_dt;
+  int64_t lengths_st, counts_st, window;
+  int heads, block;
+};
+
+// What the query t of sequence b sees, and the score of one token.
+template <typename T>
+struct DenseRows {
+  DenseArgs a;
+  __device__ Seen seen(int64_t b, int64_t) const {
+    int64_t n = a.S;
+    if (a.lengths) {
+      const int64_t l = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
+      n = l < 0 ? 0 : (l < n ? l : n);
+    }
+    return Seen{0, n};
+  }
+  __device__ Seen span(int64_t b) const { return seen(b, 0); }  // of all its queries
+  __device__ bool sees(int64_t b, int64_t t, int64_t j) const {
+    return !a.mask || a.mask[b * a.ms[0] + t * a.ms[1] + j * a.ms[2]] != 0;
+  }
+  __device__ float key(int64_t b, int h, int64_t j, int d) const {
+    return to_f32(static_cast<const T*>(a.k)[b * a.ks[0] + j * a.ks[1] + h * a.ks[2] + d * a.ks[3]]);
+  }
+  __device__ float value(int64_t b, int h, int64_t j, int d) const {
+    return to_f32(static_cast<const T*>(a.v)[b * a.vs[0] + j * a.vs[1] + h * a.vs[2] + d * a.vs[3]]);
+  }
+};
+
+struct PagedRows {
+  PagedArgs a;
+  int T, D;
+  __device__ int64_t count(int64_t b) const {  // of b's queries that are there
+    if (!a.counts) return T;
+    const int64_t c = load_index(a.counts, a.counts_dt, b * a.counts_st);
+    return c < 0 ? 0 : (c < T ? c : T);
+  }
+  __device__ Seen span(int64_t b) const {  // of all its queries
+    const int64_t n = count(b);
+    return Seen{seen(b, 0).lo, n ? seen(b, n - 1).hi : 0};
+  }
+  __device__ Seen seen(int64_t b, int64_t t) const {
+    const int64_t n = count(b);
+    const int64_t len = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
+    const int64_t place = (len < 0 ? 0 : len) - n + t;
+    return seen_tokens(t < n ? place : -1, a.window, a.columns * a.block);
+  }
+  __device__ int64_t page(int64_t b, int64_t j) const {
+    const int64_t p = a.table[b * a.table_stride + j / a.block];
+    return p < a.pages ? p : -1;
+  }
+  __device__ bool sees(int64_t b, int64_t, int64_t j) const { return page(b, j) >= 0; }
+  __device__ float key(int64_t b, int h, int64_t j, int d) const {
+    const int64_t p = page(b, j) * a.heads + h;
+    return static_cast<float>(a.k[(p * a.block + j % a.block) * D + d]) * a.k_scale[p];
+  }
+  __device__ float value(int64_t b, int h, int64_t j, int d) const {
+    const int64_t p = page(b, j) * a.heads + h;
+    return static_cast<float>(a.v[(p * D + d) * a.block + j % a.block]) * a.v_scale[p];
+  }
+};
+
+// ---------------------------------------------- few queries, many tokens
+// A step reads a whole cache for a few queries: sequences are cut into chunks
+// so that every CU has some.  How long they are is known on the device only,
+// so the blocks find their chunk there: with n_b steps of kStep tokens in
+// sequence b, a chunk is c = max(least, ceil(sum n_b / units)) steps, one and
+// the same for all, so that ragged batches load the CUs evenly.  At most
+// units + B chunks come of that, times the key heads: the grid.
+constexpr int kStep = 64;
+constexpr int kMaxChunks = 64;  // of a sequence: what the block that joins them reads
+
+struct Cut {
+  int64_t B;
+  int heads;           // key heads
+  int64_t units;       // chunks to aim for, for each head
+  int64_t least;       // steps of a chunk at least
+  int64_t rows;        // queries of a key head: T * group
+  float* part;         // a slot of rows * (D + 2) floats a block
+  int* arrived;        // a counter for each sequence and head, zero between launches
+};
+
+struct Unit {
+  int64_t b, lo, hi;   // tokens of the chunk; lo a multiple of kStep
+  int h, chunk, chunks;
+  int64_t slot;        // of the sequence's first chunk and this head; the next chunk's is `heads` later
+};
+
+__device__ __forceinline__ int64_t chunk_steps(int64_t steps, int64_t c) {
+  const int64_t most = ceil_div(steps, kMaxChunks);
+  return c < most ? most : c;
+}
+
+// This block's chunk (the same in every wave); false where it has none.
+template <class Rows>
+__device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit* u) {
+  const int lane = threadIdx.x % 64;
+  const int64_t id = blockIdx.x / cut.heads;
+  u->h = static_cast<int>(blockIdx.x % cut.heads);
+  auto steps_of = [&](int64_t b) -> int64_t {
+    if (b >= cut.B) return 0;
+    const Seen s = rows.span(b);
+    return ceil_div(s.hi - (s.lo / kStep) * kStep, kStep);
+  };
+  const int64_t mine = steps_of(lane);
+  int64_t total = mine;
+  for (int64_t b = 64 + lane; b < cut.B; b += 64) total += steps_of(b);
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+  int64_t c = ceil_div(total, cut.units);
+  c = c < cut.least ? cut.least : c;
+  int64_t before = 0;
+  for (int64_t b0 = 0; b0 < cut.B; b0 += 64) {
+    const int64_t b = b0 + lane, n = b0 ? steps_of(b) : mine;
+    const int64_t each = chunk_steps(n, c);
+    const int64_t chunks = b >= cut.B ? 0 : n <= each ? 1 : ceil_div(n, each);
+    int64_t upto = chunks;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t o = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += o;
+    }
+    const uint64_t past = __ballot(before + upto > id);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int64_t first = before + __shfl(upto - chunks, at, 64);
+      u->b = b0 + at;
+      u->chunks = static_cast<int>(__shfl(chunks, at, 64));
+      u->chunk = static_cast<int>(id - first);
+      u->slot = first * cut.heads + u->h;
+      const Seen s = rows.span(u->b);
+      const int64_t lo = (s.lo / kStep) * kStep, size = __shfl(each, at, 64) * kStep;
+      u->lo = lo + u->chunk * size;
+      u->hi = u->lo + size < s.hi ? u->lo + size : s.hi;
+      return true;
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return false;
+}
+
+// Chunks and grid for `most` tokens a sequence at the most; *blocks the grid.
+// Where scratch or counters do not hold a slot for each, sequences stay whole.
+inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int64_t least, int64_t aim, Cut* cut,
+                    int64_t* blocks, const char* who) {
+  const int64_t slots = static_cast<int64_t>(kScratchBytes / 4) / (rows * (D + 2)) / heads;
+  cut->B = B;
+  cut->heads = heads;
+  cut->rows = rows;
+  cut->least = least;
+  cut->units = ceil_div(aim, heads);
+  cut->part = static_cast<float*>(ctx().scratch);
+  cut->arrived = ctx().row_counters;
+  int64_t n = B * (most / kStep / least + 2);  // (two: a window's first step may hold tokens it does not see)
+  if (n > B + cut->units) n = B + cut->units;
+  if (n > slots) {
+    cut->units = slots - B;
+    n = slots;
+  }
+  if (cut->units < 1 || B * heads > kRowCounters) {
+    cut->units = 1;
+    cut->least = int64_t{1} << 40;
+    n = B;
+  }
+  if (n * heads > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "%s: too many sequences and heads", who);
+  *blocks = n * heads;
+  return KK_OK;
+}
+
+// The block's sums of `rows` queries, each pitch floats apart in LDS (acc, not
+// yet divided; m[r] and l[r] its maximum and sum of powers of two), to the
+// output, or to the block's slot and, by the block that comes last of a
+// sequence's, joined from there: always in the chunks' order.  The order of
+// slot and counter is that of the row reductions: stores that write through
+// to where all XCDs read, a wait for them, then the count; no whole cache is
+// written back.  Called by all threads, after a barrier; lds is free for
+// kMaxChunks * rows floats from `weights` on.
+template <typename T, int THREADS>
+__device__ __forceinline__ void put_rows(const QueryArgs& a, const Cut& cut, const Unit& u, const float* acc, int pitch,
+                                         const float* m, const float* l, float* weights) {
+  const int rows = static_cast<int>(cut.rows), D = a.D;
+  auto out = [&](int r, int d, float v) {
+    const int t = r / a.group, head = u.h * a.group + r % a.group;
+    from_f32(static_cast<T*>(a.y)[u.b * a.ys[0] + t * a.ys[1] + head * a.ys[2] + d], v);
+  };
+  if (u.chunks == 1) {
+    for (int i = threadIdx.x; i < rows * D; i += THREADS) {
+      const int r = i / D, d = i - r * D;
+      out(r, d, l[r] != 0.0f ? acc[r * pitch + d] / l[r] : 0.0f);
+    }
+    return;
+  }
+  const int64_t size = int64_t{rows} * (D + 2);
+  auto put = [&](float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  auto get = [&](const float* p) {
+    return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  float* mine = cut.part + (u.slot + int64_t{u.chunk} * cut.heads) * size;
+  for (int i = threadIdx.x; i < rows * D; i += THREADS) {
+    const int r = i / D, d = i - r * D;
+    put(mine + i, acc[r * pitch + d]);
+  }
+  for (int r = threadIdx.x; r < rows; r += THREADS) {
+    put(mine + rows * D + r, m[r]);
+    put(mine + rows * D + rows + r, l[r]);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __shared__ int last;
+  __syncthreads();
+  int* count = cut.arrived + u.b * cut.heads + u.h;
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.chunks - 1;
+  __syncthreads();
+  if (!last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const float* first = cut.part + u.slot * size;
+  const int64_t next = size * cut.heads;
+  // weights[i][r] = 2^(m_i - max) / sum_i l_i 2^(m_i - max)
+  for (int r = threadIdx.x; r < rows; r += THREADS) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < u.chunks; ++i) {
+      const float mi = get(first + i * next + rows * D + r);
+      weights[i * rows + r] = mi;
+      top = fmaxf(top, mi);
+    }
+    for (int i = 0; i < u.chunks; ++i) {
+      const float w = exp2f(weights[i * rows + r] - top);
+      weights[i * rows + r] = w;
+      sum += w * get(first + i * next + rows * D + rows + r);
+    }
+    const float by = sum != 0.0f ? 1.0f / sum : 0.0f;
+    for (int i = 0; i < u.chunks; ++i) weights[i * rows + r] *= by;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * D; i += THREADS) {
+    const int r = i / D, d = i - r * D;
+    float sum = 0.0f;
+    for (int j0 = 0; j0 < u.chunks; j0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j0 + j < u.chunks ? get(first + (j0 + j) * next + i) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < u.chunks) sum = __builtin_fmaf(weights[(j0 + j) * rows + r], x[j], sum);
+    }
+    out(r, d, sum);
+  }
+  if (threadIdx.x == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Entry points of the kernels; false where a call is not theirs.
+bool few_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status);
+bool few_dense_try(const QueryArgs& a, const DenseArgs& d, int dtype, int* status);
+
+}  // namespace kk

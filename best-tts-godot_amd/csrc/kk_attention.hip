@@ -1,94 +1,8 @@
 // Attention of a token decoder: over a paged cache of 8-bit codes, and over
 // an encoder's states.
-#include "kk_decode.h"
+#include "kk_attention.h"
 
 namespace kk {
-
-constexpr int kMaxHead = 256;
-
-// Queries and outputs: [B, T, heads, D], group query heads a key head.
-struct QueryArgs {
-  const void* q;
-  void* y;
-  int64_t qs[3], ys[3];
-  int64_t B;
-  int T, heads, group, D;
-  float scale;  // times log2 e: the softmax is formed from powers of two
-};
-
-// Keys and values of one piece each: [B, S, key heads, D].
-struct DenseArgs {
-  const void *k, *v;
-  int64_t ks[4], vs[4];
-  int64_t S;
-  const void* lengths;
-  int lengths_dt;
-  int64_t lengths_st;
-  const uint8_t* mask;
-  int64_t ms[3];
-};
-
-struct PagedArgs {
-  const int8_t *k, *v;
-  const float *k_scale, *v_scale;
-  const int32_t* table;
-  int64_t table_stride, pages, columns;
-  const void *lengths, *counts;
-  int lengths_dt, counts_dt;
-  int64_t lengths_st, counts_st, window;
-  int heads, block;
-};
-
-// What the query t of sequence b sees, and the score of one token.
-template <typename T>
-struct DenseRows {
-  DenseArgs a;
-  __device__ Seen seen(int64_t b, int64_t) const {
-    int64_t n = a.S;
-    if (a.lengths) {
-      const int64_t l = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
-      n = l < 0 ? 0 : (l < n ? l : n);
-    }
-    return Seen{0, n};
-  }
-  __device__ bool sees(int64_t b, int64_t t, int64_t j) const {
-    return !a.mask || a.mask[b * a.ms[0] + t * a.ms[1] + j * a.ms[2]] != 0;
-  }
-  __device__ float key(int64_t b, int h, int64_t j, int d) const {
-    return to_f32(static_cast<const T*>(a.k)[b * a.ks[0] + j * a.ks[1] + h * a.ks[2] + d * a.ks[3]]);
-  }
-  __device__ float value(int64_t b, int h, int64_t j, int d) const {
-    return to_f32(static_cast<const T*>(a.v)[b * a.vs[0] + j * a.vs[1] + h * a.vs[2] + d * a.vs[3]]);
-  }
-};
-
-struct PagedRows {
-  PagedArgs a;
-  int T, D;
-  __device__ Seen seen(int64_t b, int64_t t) const {
-    int64_t n = T;
-    if (a.counts) {
-      const int64_t c = load_index(a.counts, a.counts_dt, b * a.counts_st);
-      n = c < 0 ? 0 : (c < n ? c : n);
-    }
-    const int64_t len = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
-    const int64_t place = (len < 0 ? 0 : len) - n + t;
-    return seen_tokens(t < n ? place : -1, a.window, a.columns * a.block);
-  }
-  __device__ int64_t page(int64_t b, int64_t j) const {
-    const int64_t p = a.table[b * a.table_stride + j / a.block];
-    return p < a.pages ? p : -1;
-  }
-  __device__ bool sees(int64_t b, int64_t, int64_t j) const { return page(b, j) >= 0; }
-  __device__ float key(int64_t b, int h, int64_t j, int d) const {
-    const int64_t p = page(b, j) * a.heads + h;
-    return static_cast<float>(a.k[(p * a.block + j % a.block) * D + d]) * a.k_scale[p];
-  }
-  __device__ float value(int64_t b, int h, int64_t j, int d) const {
-    const int64_t p = page(b, j) * a.heads + h;
-    return static_cast<float>(a.v[(p * D + d) * a.block + j % a.block]) * a.v_scale[p];
-  }
-};
 
 constexpr int kRowWaves = 4;
 
@@ -219,6 +133,8 @@ int kk_cache_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor
   p.block = static_cast<int>(c.block);
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
+  int status = KK_OK;
+  if (few_paged_try(a, p, q->dtype, &status)) return status;
   const PagedRows rows{p, a.T, a.D};
   return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
 }
@@ -265,6 +181,8 @@ int kk_cross_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor
   }
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
+  int status = KK_OK;
+  if (few_dense_try(a, d, q->dtype, &status)) return status;
   return q->dtype == KK_F16 ? launch_rows<__half>(a, DenseRows<__half>{d})
                             : launch_rows<float>(a, DenseRows<float>{d});
 }
