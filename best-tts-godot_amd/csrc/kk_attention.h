@@ -129,6 +129,12 @@ __device__ __forceinline__ int64_t chunk_steps(int64_t steps, int64_t c) {
   return c < most ? most : c;
 }
 
+__device__ __forceinline__ int64_t uniform(int64_t v) {  // the same in all lanes: in scalar registers
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return static_cast<int64_t>(uint64_t{hi} << 32 | lo);
+}
+
 // This block's chunk (the same in every wave); false where it has none.
 template <class Rows>
 __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit* u) {
@@ -161,13 +167,13 @@ __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit
       const int at = __builtin_ctzll(past);
       const int64_t first = before + __shfl(upto - chunks, at, 64);
       u->b = b0 + at;
-      u->chunks = static_cast<int>(__shfl(chunks, at, 64));
-      u->chunk = static_cast<int>(id - first);
-      u->slot = first * cut.heads + u->h;
+      u->chunks = static_cast<int>(uniform(__shfl(chunks, at, 64)));
+      u->chunk = static_cast<int>(uniform(id - first));
+      u->slot = uniform(first) * cut.heads + u->h;
       const Seen s = rows.span(u->b);
       const int64_t lo = (s.lo / kStep) * kStep, size = __shfl(each, at, 64) * kStep;
-      u->lo = lo + u->chunk * size;
-      u->hi = u->lo + size < s.hi ? u->lo + size : s.hi;
+      u->lo = uniform(lo + u->chunk * size);
+      u->hi = uniform(u->lo + size < s.hi ? u->lo + size : s.hi);
       return true;
     }
     before += __shfl(upto, 63, 64);

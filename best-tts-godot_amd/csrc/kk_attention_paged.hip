@@ -5,6 +5,7 @@
 namespace kk {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 // Eight codes as halves, exactly: a byte with its sign turned over is the low
@@ -34,10 +35,13 @@ constexpr int kFewWaves = kFewThreads / 64;
 
 // out = sum_j 2^(c q.k_j - m) v_j / sum_j 2^(c q.k_j - m), a wave its own
 // steps of 64 tokens, on the matrix cores (v_mfma_f32_16x16x32_f16): bound by
-// the codes' way from memory, so nothing is staged in LDS: each code is read
-// once, straight into the registers of the lane that multiplies it, a step's
-// values and the next step's keys (where there are registers for them) before
-// the step's products.
+// the codes' way from memory.  A wave loads the next step's codes, 16 bytes a
+// lane in the order of memory, while it works on a step, and hands them to the
+// lanes that multiply them through a part of LDS that is its own (no barrier).
+// 32 sequences of 16384 to 32768 tokens, 8 key heads of 128 values in pages of
+// 64, 32 query heads: 314 us, 5.1 TB/s of 6.2 that a kernel reaches which only
+// reads such pages (544 us where each lane loads the rows that it multiplies,
+// every 16 bytes of them in another line).
 //
 // Scores are formed transposed, S^T = K Q^T, 16 tokens by 16 queries: a lane
 // (n = l % 16, g = l / 16) holds a query's column, and with token 16 g + 4 a + i
@@ -48,21 +52,24 @@ constexpr int kFewWaves = kFewThreads / 64;
 //
 // Codes are exact in fp16.  fp16 queries are taken as they are, fp32 ones as
 // the sum of two halves after a power of two that brings the row's largest to
-// 2^14 (22 bits; smaller values keep 2^-38 of the largest).  Weights p times
-// the page's scale, over a power of two r >= all scales so far, are rounded to
-// fp16 (half a step of the output's type) or split the same way; 2^15 p <= 2^15
-// keeps 24 bits above fp16's smallest value.
-template <typename T, int KH, int NT>
-__global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
+// 2^14 (22 bits; smaller values keep 2^-38 of the largest).  Weights, times
+// their page's scale over a power of two r >= all scales so far, are split into
+// two halves as well, also for fp16 queries (rounded to one, the output was 1.4
+// times as far off for the same time); 2^15 p <= 2^15 keeps 24 bits above fp16's
+// smallest value.
+template <typename T, int DT, int NT, bool EXACT>
+__global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
     few_paged_kernel(QueryArgs a, PagedRows rows, Cut cut) {
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query or weight
-  constexpr int DT = 4 * KH;
-  extern __shared__ float lds[];
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
+  constexpr int PW = 2;                      // halves of a weight
+  constexpr int KH = (DT + 3) / 4;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   Unit u;
   if (!find_unit(rows, cut, &u)) return;
   const PagedArgs& p = rows.a;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
-  const int D = a.D, R = static_cast<int>(cut.rows);
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int n = lane % 16, g = lane / 16;
+  const int C = EXACT ? DT : a.D / 16, D = 16 * C, R = static_cast<int>(cut.rows);
 
   // the lane's queries: n + 16 nt, values 64 h + 16 g + 8 e + 0 .. 7 in slot 2 h + e
   h8 qf[NT][2 * KH][P];
@@ -111,28 +118,74 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
     }
   }
 
+  // Chunks of 16 bytes of a step: DT x 64 of keys, row by row of D / 16, and as
+  // many of values, row by row of 4; the lane loads those at 64 i + lane.  In LDS
+  // a row's chunks are exchanged by a key of the row, so that eight lanes that
+  // read or write together meet eight different places.
   const int shift = __builtin_ctz(p.block);
-  const int32_t* table = p.table + u.b * p.table_stride;
-  // page of the 16 tokens from t on, -1 where there is none
-  auto page_at = [&](int64_t t) -> int {
-    const int64_t column = t >> shift;
-    if (t >= u.hi || column >= p.columns) return -1;
-    const int id = table[column];
-    return id < p.pages ? id : -1;
+  const bool paired = C % 8 == 4, eight = C % 8 == 0;
+  auto key_of = [&](int row) {
+    return eight ? (row & 3) | (row >> 2 & 4) : paired ? (row >> 1 & 1) | (row >> 3 & 2) : 0;
   };
+  const int size = 2 * 64 * D;
+  const int tail = 2 * (kFewWaves + 1) * R * 4 + 15 & ~15;  // the waves' m and l come first
+  char* mine = reinterpret_cast<char*>(lds) + tail + wave * size;
+  int to_k[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) {
+    const int q = 64 * i + lane, row = q / C, chunk = q - row * C;
+    to_k[i] = row * D + 16 * (chunk ^ key_of(row));
+  }
+  // the lane's group of 16 tokens and row among 16 of the values: in the order of memory
+  const int vg = p.block == 16 ? lane / 16 : p.block == 32 ? lane / 32 * 2 + lane % 2 : lane % 4;
+  const int vr = p.block == 16 ? lane % 16 : p.block == 32 ? lane % 32 / 2 : lane / 4;
+  const int to_v = 64 * D + 64 * vr + 16 * (vg ^ (vr >> 1 & 3));
+  const char* from_k = mine + (16 * (n / 4) + n % 4) * D;
+  const int nkey = key_of(16 * (n / 4) + n % 4);
+  const char* from_v = mine + 64 * D + 64 * n + 16 * (g ^ (n >> 1 & 3));
+
+  const int32_t* table = p.table + u.b * p.table_stride;
   const int64_t t_first = u.lo + wave * kStep;
   constexpr int kStride = kFewWaves * kStep;
-  const int kg = n / 4;
-  auto load_keys = [&](int64_t t0, int page, uint4 (&k)[4][KH]) {
-    const int row = static_cast<int>((t0 + 16 * kg) & (p.block - 1)) + lane % 4;
-    const int8_t* from = p.k + ((int64_t{page} * p.heads + u.h) * p.block + row) * D + 16 * g;
+  // The table's entry for tokens t0 + 16 (lane % 4) on, as it stands (past the
+  // table its last), and the page, -1 where there is none: apart, so that an
+  // entry is waited for where its page is needed, a step later.
+  auto entry_at = [&](int64_t t0) -> int {
+    const int64_t column = (t0 + 16 * (lane % 4)) >> shift;
+    return table[column < p.columns ? column : p.columns - 1];
+  };
+  auto page_of = [&](int64_t t0, int entry) -> int {
+    const int64_t t = t0 + 16 * (lane % 4);
+    return t < u.hi && t >> shift < p.columns && entry < p.pages ? entry : -1;
+  };
+  // Where there is no page, page 0 is read, and its tokens get no weight.
+  u4 ck[DT], cv[DT];
+  const int64_t page_bytes = int64_t{p.block} * D;
+  auto load_k = [&](int64_t t0, int pages) {
+    if (p.block >= 64) {
+      const int page = __builtin_amdgcn_readfirstlane(pages < 0 ? 0 : pages);
+      const int8_t* k = p.k + (int64_t{page} * p.heads + u.h) * page_bytes + static_cast<int>(t0 & (p.block - 1)) * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < DT; ++i)
+        if (i < C) ck[i] = *reinterpret_cast<const u4*>(k + 1024 * i + 16 * lane);
+    } else {
 #pragma unroll
-      for (int h = 0; h < KH; ++h) {
-        k[i][h] = make_uint4(0, 0, 0, 0);
-        if (page >= 0 && 64 * h + 16 * g < D) k[i][h] = *reinterpret_cast<const uint4*>(from + 4 * i * D + 64 * h);
+      for (int i = 0; i < DT; ++i) {
+        if (i >= C) continue;
+        const int q = 64 * i + lane, of = q / D, page = __shfl(pages, of, 64);
+        const int8_t* k = p.k + (int64_t{page < 0 ? 0 : page} * p.heads + u.h) * page_bytes +
+                          static_cast<int>((t0 + 16 * of) & (p.block - 1)) * D + 16 * (q - of * D);
+        ck[i] = *reinterpret_cast<const u4*>(k);
       }
+    }
+  };
+  auto load_v = [&](int64_t t0, int pages) {
+    const int page = __shfl(pages, vg, 64);
+    const int8_t* v = p.v + (int64_t{page < 0 ? 0 : page} * p.heads + u.h) * page_bytes + vr * p.block +
+                      static_cast<int>((t0 + 16 * vg) & (p.block - 1));
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+      if (i < C) cv[i] = *reinterpret_cast<const u4*>(v + 16 * i * p.block);
   };
 
   f4 acc[NT][DT];
@@ -146,30 +199,42 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
     for (int i = 0; i < DT; ++i) acc[nt][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  constexpr bool kAhead = KH < 4;
-  int pk = page_at(t_first + 16 * kg), pv = page_at(t_first + 16 * g);
-  uint4 k[4][KH];
-  if (kAhead && t_first < u.hi) load_keys(t_first, pk, k);
-  int pk1 = page_at(t_first + kStride + 16 * kg), pv1 = page_at(t_first + kStride + 16 * g);
+  // In flight during a step: the codes and scales of the next, the pages of the
+  // one after.  (All are waited for at once; a load given out at a step's
+  // start and needed in it would add its whole way from memory to each step.)
+  float ks1 = 0.0f, vs1 = 0.0f;
+  auto load_scales = [&](int pages) {
+    const int page = __shfl(pages, g, 64);
+    const int64_t at = int64_t{page < 0 ? 0 : page} * p.heads + u.h;
+    ks1 = p.k_scale[at];
+    vs1 = p.v_scale[at];
+  };
+  int entry1 = entry_at(t_first + kStride), pages = page_of(t_first, entry_at(t_first));
+  if (t_first < u.hi) {
+    load_scales(pages);
+    load_k(t_first, pages);
+    load_v(t_first, pages);
+  }
   for (int64_t t0 = t_first; t0 < u.hi; t0 += kStride) {
-    uint4 k1[4][KH], v[DT];
-    if (!kAhead) load_keys(t0, pk, k);
-    const int vrow = static_cast<int>((t0 + 16 * g) & (p.block - 1));
-    const int64_t at = int64_t{pv} * p.heads + u.h;
-    const int8_t* from = p.v + (at * D + n) * p.block + vrow;
-    float ks = 0.0f, vs = 0.0f;
-    if (pv >= 0) {
-      ks = p.k_scale[at];
-      vs = p.v_scale[at];
-    }
+    const bool there = __shfl(pages, g, 64) >= 0;
+    const float ks = ks1, vs = there ? vs1 : 0.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (pv >= 0 && 16 * i < D) v[i] = *reinterpret_cast<const uint4*>(from + 16 * i * p.block);
+    for (int i = 0; i < DT; ++i)
+      if (i < C) {
+        *reinterpret_cast<u4*>(mine + to_k[i]) = ck[i];
+        *reinterpret_cast<u4*>(mine + to_v + 1024 * i) = cv[i];
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int pages1 = page_of(t0 + kStride, entry1);
+    entry1 = entry_at(t0 + 2 * kStride);
+    if (t0 + kStride < u.hi) {
+      load_scales(pages1);
+      load_k(t0 + kStride, pages1);
+      load_v(t0 + kStride, pages1);
     }
-    const bool more = t0 + kStride < u.hi;
-    if (kAhead && more) load_keys(t0 + kStride, pk1, k1);
-    const int pk2 = page_at(t0 + 2 * kStride + 16 * kg), pv2 = page_at(t0 + 2 * kStride + 16 * g);
 
     f4 s[NT][4];
 #pragma unroll
@@ -180,7 +245,10 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
     for (int h = 0; h < KH; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const h8 k0 = codes_h8(k[i][h].x, k[i][h].y), k1 = codes_h8(k[i][h].z, k[i][h].w);
+        if (4 * h >= C) continue;
+        const int chunk = 4 * h + g;  // (lanes past the row's end read another row's, against zeros of q)
+        const u4 w = *reinterpret_cast<const u4*>(from_k + 4 * i * D + 16 * ((chunk < C ? chunk : 0) ^ nkey));
+        const h8 k0 = codes_h8(w.x, w.y), k1 = codes_h8(w.z, w.w);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -207,22 +275,25 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
     }
     const float vw = vs * __uint_as_float(static_cast<uint32_t>(127 + 15 + 127 - er) << 23);
 
-    h8 pf[NT][2][P];
+    h8 pf[NT][2][PW];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float by = cq[nt] * ks;
       int64_t lo = qlo[nt] - (t0 + 16 * g), hi = qhi[nt] - (t0 + 16 * g);
-      if (pv < 0) hi = 0;
+      if (!there) hi = 0;
       const int a0 = lo < 0 ? 0 : (lo > 16 ? 16 : static_cast<int>(lo));
       const int a1 = hi < 0 ? 0 : (hi > 16 ? 16 : static_cast<int>(hi));
       const bool whole = __all(a0 == 0 && a1 == 16 && finite);
       float x[16], top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 16; ++j)
         x[j] = s[nt][j / 4][j % 4] * by;
-        if (!whole) x[j] = j >= a0 && j < a1 ? x[j] : -INFINITY;
-        top = fmaxf(top, x[j]);
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = j >= a0 && j < a1 ? x[j] : -INFINITY;
       }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       top = fmaxf(top, m[nt]);
@@ -238,45 +309,43 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float e = __builtin_amdgcn_exp2f(x[j] - m[nt]);
-        l[nt] += e;
-        float w = e * vw;
-        if (!whole) w = j >= a0 && j < a1 ? w : 0.0f;  // (a scale that is not finite)
+        x[j] = __builtin_amdgcn_exp2f(x[j] - m[nt]);
+        l[nt] += x[j];
+        x[j] *= vw;
+      }
+      if (!whole) {  // (past a scale that is not finite)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = j >= a0 && j < a1 ? x[j] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float w = x[j];
         const _Float16 hi16 = static_cast<_Float16>(w);
         pf[nt][j / 8][0][j % 8] = hi16;
-        if constexpr (P == 2) pf[nt][j / 8][1][j % 8] = static_cast<_Float16>(w - static_cast<float>(hi16));
+        pf[nt][j / 8][1][j % 8] = static_cast<_Float16>(w - static_cast<float>(hi16));
       }
     }
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       if (16 * i >= D) continue;
-      const h8 v0 = codes_h8(v[i].x, v[i].y), v1 = codes_h8(v[i].z, v[i].w);
+      const u4 w = *reinterpret_cast<const u4*>(from_v + 1024 * i);
+      const h8 v0 = codes_h8(w.x, w.y), v1 = codes_h8(w.z, w.w);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = P - 1; e >= 0; --e) {
+        for (int e = PW - 1; e >= 0; --e) {
           acc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[nt][0][e], acc[nt][i], 0, 0, 0);
           acc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[nt][1][e], acc[nt][i], 0, 0, 0);
         }
     }
-    if (kAhead && more) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int h = 0; h < KH; ++h) k[i][h] = k1[i][h];
-    }
-    pk = pk1;
-    pv = pv1;
-    pk1 = pk2;
-    pv1 = pv2;
+    pages = pages1;
   }
 
   // join the waves: m and l of a wave's queries, then the sums, in LDS
   const int pitch = D + 4;
   float* wm = lds;                        // [waves][R], then [R] the block's
   float* wl = wm + (kFewWaves + 1) * R;
-  float* sums = wl + (kFewWaves + 1) * R;  // [waves][R][pitch]
-  sums += (4 - (2 * (kFewWaves + 1) * R) % 4) % 4;
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<char*>(lds) + tail);  // [waves][R][pitch]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     l[nt] += __shfl_xor(l[nt], 16, 64);
@@ -315,7 +384,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && KH < 4 ? 2 : 1)
   put_rows<T, kFewThreads>(a, cut, u, sums, pitch, wm + kFewWaves * R, wl + kFewWaves * R, sums + R * pitch);
 }
 
-template <typename T, int KH, int NT>
+template <typename T, int DT, int NT, bool EXACT>
 static int launch_few(const QueryArgs& a, const PagedRows& rows, int64_t queries) {
   const int64_t capacity = rows.a.columns * rows.a.block;
   const int64_t seen = rows.a.window ? rows.a.window + a.T - 1 : capacity;
@@ -323,29 +392,32 @@ static int launch_few(const QueryArgs& a, const PagedRows& rows, int64_t queries
   int64_t blocks;
   KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 8, int64_t{8} * ctx().num_cus,
                   &cut, &blocks, "cache_attention"));
-  // the waves' sums, or (once they are joined in the first) the chunks' weights
+  // codes; then the waves' sums; then, beside the first's, the chunks' weights
   const int R = static_cast<int>(queries);
-  size_t floats = 2 * (kFewWaves + 1) * R + 4 + static_cast<size_t>(kFewWaves) * R * (a.D + 4);
-  const size_t joined = 2 * (kFewWaves + 1) * R + 4 + static_cast<size_t>(R) * (a.D + 4 + kMaxChunks);
-  floats = floats > joined ? floats : joined;
-  const void* kernel = reinterpret_cast<const void*>(few_paged_kernel<T, KH, NT>);
-  if (floats * 4 > 65536) KK_TRY(allow_large_lds(kernel));
-  KK_LAUNCH((few_paged_kernel<T, KH, NT>), dim3(static_cast<unsigned>(blocks)), dim3(kFewThreads), floats * 4,
+  const size_t codes = size_t{kFewWaves} * 2 * 64 * a.D, sums = size_t{kFewWaves} * R * (a.D + 4) * 4;
+  const size_t joined = static_cast<size_t>(R) * (a.D + 4 + kMaxChunks) * 4;
+  size_t bytes = codes > sums ? codes : sums;
+  bytes = (2 * (kFewWaves + 1) * R * 4 + 15) / 16 * 16 + (bytes > joined ? bytes : joined);
+  const void* kernel = reinterpret_cast<const void*>(few_paged_kernel<T, DT, NT, EXACT>);
+  if (bytes > 65536) KK_TRY(allow_large_lds(kernel));
+  KK_LAUNCH((few_paged_kernel<T, DT, NT, EXACT>), dim3(static_cast<unsigned>(blocks)), dim3(kFewThreads), bytes,
             ctx().stream, a, rows, cut);
   return check_launch("few_paged_kernel");
 }
 
 template <typename T, int NT>
 static int launch_few(const QueryArgs& a, const PagedRows& rows, int64_t queries) {
-  if (a.D <= 64) return launch_few<T, 1, NT>(a, rows, queries);
-  if constexpr (NT == 1)
-    if (a.D > 128) return launch_few<T, 4, 1>(a, rows, queries);
-  return launch_few<T, 2, NT>(a, rows, queries);
+  switch (a.D) {
+    case 64: return launch_few<T, 4, NT, true>(a, rows, queries);
+    case 96: return launch_few<T, 6, NT, true>(a, rows, queries);
+    case 128: return launch_few<T, 8, NT, true>(a, rows, queries);
+  }
+  return launch_few<T, 8, NT, false>(a, rows, queries);
 }
 
 bool few_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status) {
   const int64_t queries = int64_t{a.T} * a.group;
-  if (queries > (a.D > 128 ? 16 : 32)) return false;  // (two tiles of queries of 256 values pass the registers)
+  if (p.pages < 1 || p.columns < 1 || a.D > 128 || queries > 32) return false;
   const PagedRows rows{p, a.T, a.D};
   if (dtype == KK_F16)
     *status = queries > 16 ? launch_few<__half, 2>(a, rows, queries) : launch_few<__half, 1>(a, rows, queries);
