@@ -98,6 +98,75 @@ struct PagedRows {
   }
 };
 
+// Eight codes as halves, exactly: a byte with its sign turned over is the low
+// half of 1024 + 128 + code, from which a packed sum takes 1152.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ h8 codes_h8(uint32_t lo, uint32_t hi) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+  uint32_t w[4];
+  lo ^= 0x80808080u;
+  hi ^= 0x80808080u;
+  w[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05010400u);
+  w[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05030402u);
+  w[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05010400u);
+  w[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05030402u);
+  h8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const h2 v = __builtin_bit_cast(h2, w[i]) + off;
+    r[2 * i] = v[0];
+    r[2 * i + 1] = v[1];
+  }
+  return r;
+}
+
+// One wave a query: a lane scores one of 64 tokens, then owns every 64th
+// value of the output.  Right for every size, stride and type; qv is the
+// wave's own, kMaxHead floats of LDS.
+template <typename T, class Rows>
+__device__ __forceinline__ void one_query(const QueryArgs& a, const Rows& rows, int64_t b, int64_t t, int head, float* qv) {
+  const int lane = threadIdx.x % 64, h = head / a.group;
+  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int d = lane; d < a.D; d += 64) qv[d] = to_f32(q[d]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const Seen w = rows.seen(b, t);
+  float m = -INFINITY, l = 0.0f, acc[kMaxHead / 64] = {};
+  for (int64_t j0 = w.lo; j0 < w.hi; j0 += 64) {
+    const int64_t j = j0 + lane;
+    const bool sees = j < w.hi && rows.sees(b, t, j);
+    float s = 0.0f;
+    if (sees)
+      for (int d = 0; d < a.D; ++d) s = __builtin_fmaf(qv[d], rows.key(b, h, j, d), s);
+    s = sees ? s * a.scale : -INFINITY;
+    const float next = fmaxf(fmaxf(m, wave_max(s)), -3.4028235e38f);
+    const float keep = exp2f(m - next), p = exp2f(s - next);
+    m = next;
+    l = l * keep + wave_sum(p);
+#pragma unroll
+    for (int i = 0; i < kMaxHead / 64; ++i) acc[i] *= keep;
+    uint64_t live = __ballot(sees);
+    while (live) {
+      const int e = __builtin_ctzll(live);
+      live &= live - 1;
+      const float pe = __shfl(p, e, 64);
+#pragma unroll
+      for (int i = 0; i < kMaxHead / 64; ++i)
+        if (lane + 64 * i < a.D) acc[i] = __builtin_fmaf(pe, rows.value(b, h, j0 + e, lane + 64 * i), acc[i]);
+    }
+  }
+  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 64; ++i)
+    if (lane + 64 * i < a.D) from_f32(y[lane + 64 * i], l != 0.0f ? acc[i] / l : 0.0f);
+}
+
 // ---------------------------------------------- few queries, many tokens
 // A step reads a whole cache for a few queries: sequences are cut into chunks
 // so that every CU has some.  How long they are is known on the device only,
@@ -209,35 +278,49 @@ inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int
   return KK_OK;
 }
 
-// The block's sums of `rows` queries, each pitch floats apart in LDS (acc, not
-// yet divided; m[r] and l[r] its maximum and sum of powers of two), to the
-// output, or to the block's slot and, by the block that comes last of a
-// sequence's, joined from there: always in the chunks' order.  The order of
-// slot and counter is that of the row reductions: stores that write through
-// to where all XCDs read, a wait for them, then the count; no whole cache is
-// written back.  Called by all threads, after a barrier; lds is free for
-// kMaxChunks * rows floats from `weights` on.
+// What a block puts out: `rows` queries of key head h of sequence b from `first`
+// on, over one of `chunks` parts of their tokens; slots of rows * (D + 2) floats
+// from `slots` on, `next` apart, and the parts' counter.
+struct Part {
+  int64_t b;
+  int h, rows, chunk, chunks;
+  int64_t first;
+  float* slots;
+  int64_t next;
+  int* arrived;
+};
+
+// The block's sums of its queries, `pitch` floats apart in LDS (acc, not yet
+// divided; m[r] and l[r] a row's maximum and sum of powers of two), to the
+// output, or to the block's slot and, by the block that comes last of a row's,
+// joined from there: always in the chunks' order.  The order of slot and
+// counter is that of the row reductions: stores that write through to where
+// all XCDs read, a wait for them, then the count; no whole cache is written
+// back.  Called by all threads, after a barrier; `weights` holds chunks * rows
+// floats.  False, with nothing put out, where a row's maximum is NaN: a part
+// that the caller has marked as not to be used.
 template <typename T, int THREADS>
-__device__ __forceinline__ void put_rows(const QueryArgs& a, const Cut& cut, const Unit& u, const float* acc, int pitch,
+__device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, const float* acc, int pitch,
                                          const float* m, const float* l, float* weights) {
-  const int rows = static_cast<int>(cut.rows), D = a.D;
+  const int rows = u.rows, D = a.D;
   auto out = [&](int r, int d, float v) {
-    const int t = r / a.group, head = u.h * a.group + r % a.group;
+    const int64_t row = u.first + r, t = row / a.group, head = u.h * a.group + row % a.group;
     from_f32(static_cast<T*>(a.y)[u.b * a.ys[0] + t * a.ys[1] + head * a.ys[2] + d], v);
   };
+  __shared__ int shared;  // last to arrive; then: parts marked
   if (u.chunks == 1) {
+    if (m[0] != m[0]) return false;
     for (int i = threadIdx.x; i < rows * D; i += THREADS) {
       const int r = i / D, d = i - r * D;
       out(r, d, l[r] != 0.0f ? acc[r * pitch + d] / l[r] : 0.0f);
     }
-    return;
+    return true;
   }
-  const int64_t size = int64_t{rows} * (D + 2);
   auto put = [&](float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
   auto get = [&](const float* p) {
     return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   };
-  float* mine = cut.part + (u.slot + int64_t{u.chunk} * cut.heads) * size;
+  float* mine = u.slots + u.chunk * u.next;
   for (int i = threadIdx.x; i < rows * D; i += THREADS) {
     const int r = i / D, d = i - r * D;
     put(mine + i, acc[r * pitch + d]);
@@ -248,51 +331,59 @@ __device__ __forceinline__ void put_rows(const QueryArgs& a, const Cut& cut, con
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __shared__ int last;
   __syncthreads();
-  int* count = cut.arrived + u.b * cut.heads + u.h;
   if (threadIdx.x == 0)
-    last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.chunks - 1;
+    shared = __hip_atomic_fetch_add(u.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.chunks - 1;
   __syncthreads();
-  if (!last) return;
+  if (!shared) return true;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  const float* first = cut.part + u.slot * size;
-  const int64_t next = size * cut.heads;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    shared = 0;
+    __hip_atomic_store(u.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
   // weights[i][r] = 2^(m_i - max) / sum_i l_i 2^(m_i - max)
   for (int r = threadIdx.x; r < rows; r += THREADS) {
     float top = -INFINITY, sum = 0.0f;
+    bool marked = false;
     for (int i = 0; i < u.chunks; ++i) {
-      const float mi = get(first + i * next + rows * D + r);
+      const float mi = get(u.slots + i * u.next + rows * D + r);
       weights[i * rows + r] = mi;
+      marked = marked || mi != mi;
       top = fmaxf(top, mi);
     }
+    if (marked) shared = 1;
     for (int i = 0; i < u.chunks; ++i) {
       const float w = exp2f(weights[i * rows + r] - top);
       weights[i * rows + r] = w;
-      sum += w * get(first + i * next + rows * D + rows + r);
+      sum += w * get(u.slots + i * u.next + rows * D + rows + r);
     }
     const float by = sum != 0.0f ? 1.0f / sum : 0.0f;
     for (int i = 0; i < u.chunks; ++i) weights[i * rows + r] *= by;
   }
   __syncthreads();
+  if (shared) return false;
   for (int i = threadIdx.x; i < rows * D; i += THREADS) {
     const int r = i / D, d = i - r * D;
     float sum = 0.0f;
     for (int j0 = 0; j0 < u.chunks; j0 += 8) {
       float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j0 + j < u.chunks ? get(first + (j0 + j) * next + i) : 0.0f;
+      for (int j = 0; j < 8; ++j) x[j] = j0 + j < u.chunks ? get(u.slots + (j0 + j) * u.next + i) : 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (j0 + j < u.chunks) sum = __builtin_fmaf(weights[(j0 + j) * rows + r], x[j], sum);
     }
     out(r, d, sum);
   }
-  if (threadIdx.x == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
 }
 
 // Entry points of the kernels; false where a call is not theirs.
 bool few_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status);
 bool few_dense_try(const QueryArgs& a, const DenseArgs& d, int dtype, int* status);
+bool tiles_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status);
+bool tiles_dense_try(const QueryArgs& a, const DenseArgs& d, int dtype, int* status);
 
 }  // namespace kk

@@ -6,48 +6,12 @@ namespace kk {
 
 constexpr int kRowWaves = 4;
 
-// One wave a query: a lane scores one of 64 tokens, then owns every 64th
-// value of the output.  Right for every size, stride and type.
 template <typename T, class Rows>
 __global__ void __launch_bounds__(kRowWaves * 64) attention_row_kernel(QueryArgs a, Rows rows, int64_t queries) {
   __shared__ float qv[kRowWaves][kMaxHead];
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;
-  if (at >= queries) return;  // (no barrier below: a wave keeps to its own row of qv)
-  const int head = static_cast<int>(at % a.heads), h = head / a.group;
-  const int64_t t = at / a.heads % a.T, b = at / a.heads / a.T;
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
-  for (int d = lane; d < a.D; d += 64) qv[wave][d] = to_f32(q[d]);
-  __builtin_amdgcn_wave_barrier();
-  const Seen w = rows.seen(b, t);
-  float m = -INFINITY, l = 0.0f, acc[kMaxHead / 64] = {};
-  for (int64_t j0 = w.lo; j0 < w.hi; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const bool sees = j < w.hi && rows.sees(b, t, j);
-    float s = 0.0f;
-    if (sees)
-      for (int d = 0; d < a.D; ++d) s = __builtin_fmaf(qv[wave][d], rows.key(b, h, j, d), s);
-    s = sees ? s * a.scale : -INFINITY;
-    const float next = fmaxf(fmaxf(m, wave_max(s)), -3.4028235e38f);
-    const float keep = exp2f(m - next), p = exp2f(s - next);
-    m = next;
-    l = l * keep + wave_sum(p);
-#pragma unroll
-    for (int i = 0; i < kMaxHead / 64; ++i) acc[i] *= keep;
-    uint64_t live = __ballot(sees);
-    while (live) {
-      const int e = __builtin_ctzll(live);
-      live &= live - 1;
-      const float pe = __shfl(p, e, 64);
-#pragma unroll
-      for (int i = 0; i < kMaxHead / 64; ++i)
-        if (lane + 64 * i < a.D) acc[i] = __builtin_fmaf(pe, rows.value(b, h, j0 + e, lane + 64 * i), acc[i]);
-    }
-  }
-  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
-#pragma unroll
-  for (int i = 0; i < kMaxHead / 64; ++i)
-    if (lane + 64 * i < a.D) from_f32(y[lane + 64 * i], l != 0.0f ? acc[i] / l : 0.0f);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowWaves + threadIdx.x / 64;
+  if (at >= queries) return;  // (no barrier below)
+  one_query<T>(a, rows, at / a.heads / a.T, at / a.heads % a.T, static_cast<int>(at % a.heads), qv[threadIdx.x / 64]);
 }
 
 template <typename T, class Rows>
@@ -134,7 +98,7 @@ int kk_cache_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
   int status = KK_OK;
-  if (few_paged_try(a, p, q->dtype, &status)) return status;
+  if (few_paged_try(a, p, q->dtype, &status) || tiles_paged_try(a, p, q->dtype, &status)) return status;
   const PagedRows rows{p, a.T, a.D};
   return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
 }
@@ -182,7 +146,7 @@ int kk_cross_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
   int status = KK_OK;
-  if (few_dense_try(a, d, q->dtype, &status)) return status;
+  if (few_dense_try(a, d, q->dtype, &status) || tiles_dense_try(a, d, q->dtype, &status)) return status;
   return q->dtype == KK_F16 ? launch_rows<__half>(a, DenseRows<__half>{d})
                             : launch_rows<float>(a, DenseRows<float>{d});
 }

@@ -4,32 +4,6 @@
 
 namespace kk {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-
-// Eight codes as halves, exactly: a byte with its sign turned over is the low
-// half of 1024 + 128 + code, from which a packed sum takes 1152.
-__device__ __forceinline__ h8 codes_h8(uint32_t lo, uint32_t hi) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  const h2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-  uint32_t w[4];
-  lo ^= 0x80808080u;
-  hi ^= 0x80808080u;
-  w[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05010400u);
-  w[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05030402u);
-  w[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05010400u);
-  w[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05030402u);
-  h8 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const h2 v = __builtin_bit_cast(h2, w[i]) + off;
-    r[2 * i] = v[0];
-    r[2 * i + 1] = v[1];
-  }
-  return r;
-}
-
 constexpr int kFewThreads = 256;
 constexpr int kFewWaves = kFewThreads / 64;
 
@@ -381,7 +355,10 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
     at[0] = v;
   }
   __syncthreads();
-  put_rows<T, kFewThreads>(a, cut, u, sums, pitch, wm + kFewWaves * R, wl + kFewWaves * R, sums + R * pitch);
+  const int64_t slot = int64_t{R} * (D + 2);
+  const Part part{u.b,  u.h, R, u.chunk, u.chunks, 0, cut.part + u.slot * slot, slot * cut.heads,
+                  cut.arrived + u.b * cut.heads + u.h};
+  put_rows<T, kFewThreads>(a, part, sums, pitch, wm + kFewWaves * R, wl + kFewWaves * R, sums + R * pitch);
 }
 
 template <typename T, int DT, int NT, bool EXACT>
