@@ -310,6 +310,21 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
   __shared__ int shared;  // last to arrive; then: parts marked
   if (u.chunks == 1) {
     if (m[0] != m[0]) return false;
+    if (D % 4 == 0) {
+      const int D4 = D / 4;
+      for (int i = threadIdx.x; i < rows * D4; i += THREADS) {
+        const int r = i / D4, d = 4 * (i - r * D4);
+        const float by = l[r] != 0.0f ? 1.0f / l[r] : 0.0f;
+        const f4 v = *reinterpret_cast<const f4*>(acc + r * pitch + d) * by;
+        const int64_t row = u.first + r, t = row / a.group, head = u.h * a.group + row % a.group;
+        T* y = static_cast<T*>(a.y) + u.b * a.ys[0] + t * a.ys[1] + head * a.ys[2] + d;
+        T o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) from_f32(o[e], v[e]);
+        __builtin_memcpy(y, o, sizeof o);
+      }
+      return true;
+    }
     for (int i = threadIdx.x; i < rows * D; i += THREADS) {
       const int r = i / D, d = i - r * D;
       out(r, d, l[r] != 0.0f ? acc[r * pitch + d] / l[r] : 0.0f);

@@ -4,10 +4,12 @@
 
 namespace kk {
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int kTileThreads = 256;
 constexpr int kTileRows = 128;  // queries of a block: 32 a wave
+constexpr int kPutRows = 64;    // of them put out at a time
 
 struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
@@ -22,16 +24,24 @@ struct TileCut {
 enum Source { kPaged, kHalf, kFloat };
 
 // LDS of a block, in bytes: keys [TT][pitch], values [32 DT][pitch] (a copy for each
-// half of a split value), exponents and largest magnitudes of fp32 rows; later
+// half of a split value), of dense rows what is added to their scores (0, or -inf
+// where none is seen), of fp32 ones their largest magnitudes and scales; later
 // the sums.
 constexpr int key_pitch(int DT) { return 64 * DT + 16; }
 constexpr int value_pitch(int TT) { return 2 * TT + 16; }
 constexpr int tile_bytes(int SRC, int DT, int TT) {
-  return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 2 : 1) + (SRC == kFloat ? 6 * TT * 4 : 0);
+  return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 2 : 1) + (SRC == kFloat ? 7 : SRC == kHalf ? 1 : 0) * TT * 4;
 }
 
 __device__ __forceinline__ float other_half(float v) {  // the value of lane l ^ 32
   return __shfl_xor(v, 32, 64);
+}
+
+// Two values as the sum of two halves each.
+__device__ __forceinline__ void split2(float x, float y, h2* hi, h2* lo) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  *hi = __builtin_convertvector((f2{x, y}), h2);
+  *lo = __builtin_convertvector((f2{x - static_cast<float>((*hi)[0]), y - static_cast<float>((*hi)[1])}), h2);
 }
 
 // Whether a mask differs from query to query, and what it lets query t see of
@@ -72,7 +82,7 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // only queries that see it should be: a block that meets one marks its part, and
 // its queries are formed one by one.
 template <typename T, class Rows, int SRC, int DT, int TT>
-__global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 2 : 1)
+__global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeof(T) == 4 ? 3 : 4) ? 2 : 1)
     attention_tile_kernel(QueryArgs a, Rows rows, TileCut cut) {
   constexpr int PQ = sizeof(T) == 4 ? 2 : 1, PK = SRC == kFloat ? 2 : 1, PW = PQ;
   constexpr int KS = 2 * DT, NS = TT / 32, G = TT / 16;
@@ -83,7 +93,8 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
   char* lds_v = lds_k + PK * TT * KP;
   uint32_t* largest = reinterpret_cast<uint32_t*>(lds_v + PK * 32 * DT * VP);  // [2][keys, values][TT]
   float* key_scale = reinterpret_cast<float*>(largest + 4 * TT);
-  int* value_exp = reinterpret_cast<int*>(key_scale + TT);
+  float* value_scale = key_scale + TT;
+  float* key_bias = SRC == kFloat ? value_scale + TT : reinterpret_cast<float*>(largest);
 
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int n = lane % 32, hf = lane / 32, D = a.D;
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
     }
   }
 
-  // ---- from memory: a tile's values in registers, one tile ahead
+  // ---- from memory: a tile in registers, one tile ahead
   // token tk of 32 lies in row 8 j + 4 h + r, where its score comes out in
   // register 4 j + r of half h: tokens 16 (j / 2) + 8 h + 4 (j % 2) + r
   auto row_of = [](int tk) { return (tk & ~31) | (tk & 16) | (tk & 4) << 1 | (tk & 8) >> 1 | (tk & 3); };
@@ -180,177 +191,209 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
   constexpr int UK = (kKeyUnits + kTileThreads - 1) / kTileThreads;
   constexpr int UV = (kValueUnits + kTileThreads - 1) / kTileThreads;
   u4 ck[SRC == kFloat ? 2 * UK : UK], cv[SRC == kPaged ? UV : 4 * UV];
-
-  // paged: the units' table entries a tile before their codes, the scales of
-  // the wave's groups of 16 tokens (lane % G) with them
-  int entry_k[UK], entry_v[UV], entry_s = 0, page_s = -1;
-  float ks = 0.0f, vs = 0.0f, ks1 = 0.0f, vs1 = 0.0f;
-  // dense: bit j: token j of the tile may be seen by the block's queries
-  uint64_t word = 0;
-  uint8_t mask_byte = 0;
-
-  auto entry = [&](int64_t t) -> int {
-    if constexpr (SRC == kPaged) {
-      const int64_t column = t >> __builtin_ctz(rows.a.block);
-      return rows.a.table[b * rows.a.table_stride + (column < rows.a.columns ? column : rows.a.columns - 1)];
-    }
-    return 0;
+  // (threads past the last unit do it again; values past a head's are whatever
+  // lies at its start: against zeros of q, or in rows that are not put out)
+  auto key_unit = [&](int i) {
+    const int u = tid + kTileThreads * i;
+    return kKeyUnits % kTileThreads == 0 || u < kKeyUnits ? u : kKeyUnits - 1;
   };
-  auto entries = [&](int64_t t0) {
+  auto value_unit = [&](int i) {
+    const int u = tid + kTileThreads * i;
+    return kValueUnits % kTileThreads == 0 || u < kValueUnits ? u : kValueUnits - 1;
+  };
+  // dense: eight or four lanes next to each other read a token's values, the
+  // next ones the next four tokens'
+  auto value_d = [&](int u) { return kVD * (u % (32 / kVD) + 32 / kVD * (u / (32 / kVD * (TT / 4)))); };
+  auto value_tokens = [&](int u) { return u / (32 / kVD) % (TT / 4) * 4; };
+
+  // paged: the table's entry and, with its codes, the scales of 16 tokens, of
+  // group lane % G
+  int entry = 0, page1 = -1;
+  float ks1 = 0.0f, vs1 = 0.0f;
+  // dense: bit j: any of the block's queries may see token j
+  uint64_t word = 0;
+
+  auto find_entry = [&](int64_t t0) {
     if constexpr (SRC == kPaged) {
-#pragma unroll
-      for (int i = 0; i < UK; ++i) entry_k[i] = entry(t0 + (tid + kTileThreads * i) / (2 * DT) % TT);
-#pragma unroll
-      for (int i = 0; i < UV; ++i) entry_v[i] = entry(t0 + 16 * ((tid + kTileThreads * i) % G));
-      entry_s = entry(t0 + 16 * (lane % G));
+      const int64_t column = (t0 + 16 * (lane % G)) >> __builtin_ctz(rows.a.block);
+      entry = rows.a.table[b * rows.a.table_stride + (column < rows.a.columns ? column : rows.a.columns - 1)];
     }
   };
   auto fetch = [&](int64_t t0) {
     if constexpr (SRC == kPaged) {
       const auto& p = rows.a;
-      const int64_t page_bytes = int64_t{p.block} * D;
-      auto base = [&](int e) { return (int64_t{e >= 0 && e < p.pages ? e : 0} * p.heads + h) * page_bytes; };
-#pragma unroll
-      for (int i = 0; i < UK; ++i) {
-        const int u = tid + kTileThreads * i, tk = u / (2 * DT), c = u % (2 * DT);
-        ck[i] = u4{0, 0, 0, 0};
-        if (u < kKeyUnits && 16 * c < D)
-          ck[i] = *reinterpret_cast<const u4*>(p.k + base(entry_k[i]) +
-                                               static_cast<int>((t0 + tk) & (p.block - 1)) * D + 16 * c);
-      }
-#pragma unroll
-      for (int i = 0; i < UV; ++i) {
-        const int u = tid + kTileThreads * i, d = u / G, g = u % G;
-        cv[i] = u4{0, 0, 0, 0};
-        if (u < kValueUnits && d < D)
-          cv[i] = *reinterpret_cast<const u4*>(p.v + base(entry_v[i]) + d * p.block +
-                                               static_cast<int>((t0 + 16 * g) & (p.block - 1)));
-      }
       const int64_t t = t0 + 16 * (lane % G);
-      page_s = t < hi && t >> __builtin_ctz(p.block) < p.columns && entry_s < p.pages ? entry_s : -1;
-      const int64_t sc = int64_t{page_s < 0 ? 0 : page_s} * p.heads + h;
+      page1 = t < hi && t >> __builtin_ctz(p.block) < p.columns && entry < p.pages ? entry : -1;
+      const int pages = page1 < 0 ? 0 : page1;  // (page 0's codes, without weight)
+      const int64_t sc = int64_t{pages} * p.heads + h, page_bytes = int64_t{p.block} * D;
       ks1 = p.k_scale[sc];
       vs1 = p.v_scale[sc];
+      if (p.block >= TT) {
+        const int64_t at_page = (int64_t{__builtin_amdgcn_readfirstlane(pages)} * p.heads + h) * page_bytes;
+        const int in_page = static_cast<int>(t0 & (p.block - 1));
+        const int8_t* k = p.k + at_page + in_page * D;
+        const int8_t* v = p.v + at_page + in_page;
+#pragma unroll
+        for (int i = 0; i < UK; ++i) {
+          const int u = key_unit(i), tk = u / (2 * DT), c = 16 * (u % (2 * DT));
+          ck[i] = *reinterpret_cast<const u4*>(k + (tk * D + (c < D ? c : 0)));
+        }
+#pragma unroll
+        for (int i = 0; i < UV; ++i) {
+          const int u = value_unit(i), d = u / G, g = u % G;
+          cv[i] = *reinterpret_cast<const u4*>(v + ((d < D ? d : 0) * p.block + 16 * g));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < UK; ++i) {
+          const int u = key_unit(i), tk = u / (2 * DT), c = 16 * (u % (2 * DT));
+          const int64_t at_page = (int64_t{__shfl(pages, tk / 16, 64)} * p.heads + h) * page_bytes;
+          ck[i] = *reinterpret_cast<const u4*>(p.k + at_page + (static_cast<int>((t0 + tk) & (p.block - 1)) * D +
+                                                                (c < D ? c : 0)));
+        }
+#pragma unroll
+        for (int i = 0; i < UV; ++i) {
+          const int u = value_unit(i), d = u / G, g = u % G;
+          const int64_t at_page = (int64_t{__shfl(pages, g, 64)} * p.heads + h) * page_bytes;
+          cv[i] = *reinterpret_cast<const u4*>(p.v + at_page + ((d < D ? d : 0) * p.block +
+                                                                static_cast<int>((t0 + 16 * g) & (p.block - 1))));
+        }
+      }
     } else {
       using S = std::conditional_t<SRC == kHalf, __half, float>;
       const auto& p = rows.a;
-      const S* k = static_cast<const S*>(p.k) + b * p.ks[0] + h * p.ks[2];
-      const S* v = static_cast<const S*>(p.v) + b * p.vs[0] + h * p.vs[2];
-      // what no query of the block may see is not read
       bool sees = t0 + lane < hi && lane < TT;
       if (sees && p.mask && (p.ms[1] == 0 || a.T == 1)) sees = p.mask[b * p.ms[0] + (t0 + lane) * p.ms[2]] != 0;
       word = __ballot(sees);
-      auto load8 = [&](const S* from, int d, bool there, u4* to) {  // 16 bytes of half, 32 of float
-        constexpr int W = SRC == kFloat ? 2 : 1;
-        if (cut.wide) {
+      if (word == 0) return;
+      // a token that no query of the block may see is not read: in its place,
+      // without weight, the first that some do
+      const int visible = __builtin_ctzll(word);
+      const S* k = static_cast<const S*>(p.k) + b * p.ks[0] + h * p.ks[2] + t0 * p.ks[1];
+      const S* v = static_cast<const S*>(p.v) + b * p.vs[0] + h * p.vs[2] + t0 * p.vs[1];
+      constexpr int W = SRC == kFloat ? 2 : 1;
+      if (cut.wide) {
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            to[w] = there && d < D ? *reinterpret_cast<const u4*>(from + d + 4 * w) : u4{0, 0, 0, 0};
-        } else {
-          S e[8];
+        for (int i = 0; i < UK; ++i) {
+          const int u = key_unit(i), tk = u / (4 * DT), d = 8 * (u % (4 * DT));
+          const S* from = k + (word >> tk & 1 ? tk : visible) * p.ks[1] + (d < D ? d : 0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = there && d + i < D ? from[d + i] : S(0.0f);
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (SRC == kFloat)
-                to[w][i] = __float_as_uint(e[4 * w + i]);
-              else
-                to[w][i] = __half_as_ushort(e[2 * i]) | static_cast<uint32_t>(__half_as_ushort(e[2 * i + 1])) << 16;
-            }
+          for (int w = 0; w < W; ++w) ck[W * i + w] = *reinterpret_cast<const u4*>(from + 4 * w);
         }
-      };
 #pragma unroll
-      for (int i = 0; i < UK; ++i) {
-        const int u = tid + kTileThreads * i, tk = u / (4 * DT), d = 8 * (u % (4 * DT));
-        load8(k + (t0 + tk) * p.ks[1], d, u < kKeyUnits && (word >> (tk & 63) & 1), ck + (SRC == kFloat ? 2 * i : i));
-      }
+        for (int i = 0; i < UV; ++i) {
+          const int u = value_unit(i), d = value_d(u), tk = value_tokens(u);
+          const uint32_t there = static_cast<uint32_t>(word >> tk);
 #pragma unroll
-      for (int i = 0; i < UV; ++i) {
-        const int u = tid + kTileThreads * i;
-        const int d = kVD * (u % (32 / kVD) + 32 / kVD * (u / (32 / kVD * (TT / 4)))), tq = u / (32 / kVD) % (TT / 4);
+          for (int j = 0; j < 4; ++j)
+            cv[4 * i + j] = *reinterpret_cast<const u4*>(v + (there >> j & 1 ? tk + j : visible) * p.vs[1] +
+                                                         (d < D ? d : 0));
+        }
+      } else {
+        auto bits = [](S x) -> uint32_t {
+          if constexpr (SRC == kFloat)
+            return __float_as_uint(x);
+          else
+            return __half_as_ushort(x);
+        };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool there = u < kValueUnits && (word >> (4 * tq + j) & 1);
-          const S* from = v + (t0 + 4 * tq + j) * p.vs[1];
-          if constexpr (SRC == kHalf) {
-            load8(from, d, there, cv + 4 * i + j);
-          } else if (cut.wide) {
-            cv[4 * i + j] = there && d < D ? *reinterpret_cast<const u4*>(from + d) : u4{0, 0, 0, 0};
-          } else {
+        for (int i = 0; i < UK; ++i) {
+          const int u = key_unit(i), tk = u / (4 * DT), d = 8 * (u % (4 * DT));
+          u4 w[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) cv[4 * i + j][e] = there && d + e < D ? __float_as_uint(from[d + e]) : 0;
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t x = d + e < D ? bits(k[(word >> tk & 1 ? tk : visible) * p.ks[1] + d + e]) : 0u;
+            if constexpr (SRC == kFloat)
+              w[e / 4][e % 4] = x;
+            else
+              w[0][e / 2] = e % 2 ? w[0][e / 2] | x << 16 : x;
+          }
+#pragma unroll
+          for (int e = 0; e < W; ++e) ck[W * i + e] = w[e];
+        }
+#pragma unroll
+        for (int i = 0; i < UV; ++i) {
+          const int u = value_unit(i), d = value_d(u), tk = value_tokens(u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            u4 w;
+#pragma unroll
+            for (int e = 0; e < kVD; ++e) {
+              const uint32_t x = d + e < D ? bits(v[(word >> (tk + j) & 1 ? tk + j : visible) * p.vs[1] + d + e]) : 0u;
+              if constexpr (SRC == kFloat)
+                w[e % 4] = x;
+              else
+                w[e / 2] = e % 2 ? w[e / 2] | x << 16 : x;
+            }
+            cv[4 * i + j] = w;
           }
         }
       }
     }
   };
-  uint32_t bad = 0;  // bit 15 or 31: a half that is not finite; of fp32, all: an exponent of 255
-  auto magnitudes = [&](int which) {  // fp32: the rows' largest
+  uint32_t bad = 0;  // half: bit 15 or 31 for a value that is not finite; fp32: the largest magnitude's bits
+  auto magnitudes = [&](int which) {
     uint32_t* lk = largest + 2 * TT * which;
     uint32_t* lv = lk + TT;
 #pragma unroll
     for (int i = 0; i < UK; ++i) {
-      const int u = tid + kTileThreads * i;
       uint32_t m = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = max(m, ck[(2 * i + e / 4) % (2 * UK)][e % 4] & 0x7fffffffu);
-      if (u < kKeyUnits) atomicMax(lk + u / (4 * DT), m);
-      bad |= m >= 0x7f800000u ? 0x80000000u : 0u;
+      atomicMax(lk + key_unit(i) / (4 * DT), m);
+      bad = max(bad, m);
     }
 #pragma unroll
-    for (int i = 0; i < UV; ++i) {
-      const int u = tid + kTileThreads * i, tq = u / (32 / kVD) % (TT / 4);
+    for (int i = 0; i < UV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t m = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = max(m, cv[(4 * i + j) % (4 * UV)][e] & 0x7fffffffu);
-        if (u < kValueUnits) atomicMax(lv + 4 * tq + j, m);
-        bad |= m >= 0x7f800000u ? 0x80000000u : 0u;
+        atomicMax(lv + value_tokens(value_unit(i)) + j, m);
+        bad = max(bad, m);
       }
-    }
   };
+  float m = -3.4028235e38f, l = 0.0f, keep_r = 1.0f;
+  int er = SRC == kPaged ? 27 : 0;  // values are scaled by 2^-(er - 127) (paged), 2^-(er - 141) (fp32)
+
   auto stage = [&](int which) {
     if constexpr (SRC == kPaged) {
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
-        const int u = tid + kTileThreads * i, tk = u / (2 * DT), c = u % (2 * DT);
-        if (u >= kKeyUnits) continue;
+        const int u = key_unit(i), tk = u / (2 * DT), c = u % (2 * DT);
         h8* to = reinterpret_cast<h8*>(lds_k + row_of(tk) * KP + 32 * c);
         to[0] = codes_h8(ck[i][0], ck[i][1]);
         to[1] = codes_h8(ck[i][2], ck[i][3]);
       }
 #pragma unroll
       for (int i = 0; i < UV; ++i) {
-        const int u = tid + kTileThreads * i, d = u / G, g = u % G;
-        if (u >= kValueUnits) continue;
+        const int u = value_unit(i), d = u / G, g = u % G;
         h8* to = reinterpret_cast<h8*>(lds_v + d * VP + 32 * g);
         to[0] = codes_h8(cv[i][0], cv[i][1]);
         to[1] = codes_h8(cv[i][2], cv[i][3]);
       }
-    } else if constexpr (SRC == kHalf) {
+      return;
+    }
+    if (tid < TT) key_bias[tid] = word >> tid & 1 ? 0.0f : -INFINITY;
+    if constexpr (SRC == kHalf) {
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
-        const int u = tid + kTileThreads * i, tk = u / (4 * DT), c = u % (4 * DT);
-        if (u >= kKeyUnits) continue;
+        const int u = key_unit(i), tk = u / (4 * DT), c = u % (4 * DT);
         *reinterpret_cast<u4*>(lds_k + row_of(tk) * KP + 16 * c) = ck[i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) bad |= (ck[i][e] & 0x7c007c00u) + 0x04000400u;
       }
 #pragma unroll
       for (int i = 0; i < UV; ++i) {
-        const int u = tid + kTileThreads * i;
-        if (u >= kValueUnits) continue;
-        const int d = kVD * (u % (32 / kVD) + 32 / kVD * (u / (32 / kVD * (TT / 4)))), tq = u / (32 / kVD) % (TT / 4);
+        const int u = value_unit(i), d = value_d(u), tk = value_tokens(u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {  // the d-th value of four tokens
+        for (int e = 0; e < 8; ++e) {  // one value of four tokens
           const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
           typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-          const u2 w = {__builtin_amdgcn_perm(cv[(4 * i + 1) % (4 * UV)][e / 2], cv[4 * i][e / 2], sel),
+          const u2 w = {__builtin_amdgcn_perm(cv[(4 * i + 1) % (4 * UV)][e / 2], cv[4 * i % (4 * UV)][e / 2], sel),
                         __builtin_amdgcn_perm(cv[(4 * i + 3) % (4 * UV)][e / 2], cv[(4 * i + 2) % (4 * UV)][e / 2], sel)};
-          *reinterpret_cast<u2*>(lds_v + (d + e) * VP + 8 * tq) = w;
+          *reinterpret_cast<u2*>(lds_v + (d + e) * VP + 2 * tk) = w;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -360,50 +403,56 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
     } else {
       const uint32_t* lk = largest + 2 * TT * which;
       const uint32_t* lv = lk + TT;
-      auto split = [](float x, int up, _Float16* hi16, _Float16* lo16) {
-        const float y = __builtin_amdgcn_ldexpf(x, up);
-        *hi16 = static_cast<_Float16>(y);
-        *lo16 = static_cast<_Float16>(y - static_cast<float>(*hi16));
-      };
+      // the values' power of two: of the largest so far
+      const int top = static_cast<int>(__float_as_uint(wave_max_dpp(__uint_as_float(lv[lane % TT]))) >> 23);
+      const int up = top > er ? top : er;
+      keep_r = ldexpf(1.0f, er - up);
+      er = up;
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
-        const int u = tid + kTileThreads * i, tk = u / (4 * DT), c = u % (4 * DT);
-        if (u >= kKeyUnits) continue;
-        const int up = 141 - static_cast<int>(lk[tk] >> 23);
+        const int u = key_unit(i), tk = u / (4 * DT), c = u % (4 * DT);
+        const int by = 141 - static_cast<int>(lk[tk] >> 23);
         h8 y0, y1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          _Float16 p0, p1;
-          split(__uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4]), up, &p0, &p1);
-          y0[e] = p0;
-          y1[e] = p1;
+        for (int e = 0; e < 8; e += 2) {
+          h2 p0, p1;
+          split2(__builtin_amdgcn_ldexpf(__uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4]), by),
+                 __builtin_amdgcn_ldexpf(__uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4 + 1]), by), &p0, &p1);
+          y0[e] = p0[0];
+          y0[e + 1] = p0[1];
+          y1[e] = p1[0];
+          y1[e + 1] = p1[1];
         }
         *reinterpret_cast<h8*>(lds_k + row_of(tk) * KP + 16 * c) = y0;
         *reinterpret_cast<h8*>(lds_k + (TT + row_of(tk)) * KP + 16 * c) = y1;
       }
 #pragma unroll
       for (int i = 0; i < UV; ++i) {
-        const int u = tid + kTileThreads * i;
-        if (u >= kValueUnits) continue;
-        const int d = kVD * (u % (32 / kVD) + 32 / kVD * (u / (32 / kVD * (TT / 4)))), tq = u / (32 / kVD) % (TT / 4);
-        const u4 top = *reinterpret_cast<const u4*>(lv + 4 * tq);
+        const int u = value_unit(i), d = value_d(u), tk = value_tokens(u);
+        const u4 of = *reinterpret_cast<const u4*>(lv + tk);
+        int by[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) by[j] = 141 - static_cast<int>(of[j] >> 23);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           h4 y0, y1;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            _Float16 p0, p1;
-            split(__uint_as_float(cv[(4 * i + j) % (4 * UV)][e]), 141 - static_cast<int>(top[j] >> 23), &p0, &p1);
-            y0[j] = p0;
-            y1[j] = p1;
+          for (int j = 0; j < 4; j += 2) {
+            h2 p0, p1;
+            split2(__builtin_amdgcn_ldexpf(__uint_as_float(cv[(4 * i + j) % (4 * UV)][e]), by[j]),
+                   __builtin_amdgcn_ldexpf(__uint_as_float(cv[(4 * i + j + 1) % (4 * UV)][e]), by[j + 1]), &p0, &p1);
+            y0[j] = p0[0];
+            y0[j + 1] = p0[1];
+            y1[j] = p1[0];
+            y1[j + 1] = p1[1];
           }
-          *reinterpret_cast<h4*>(lds_v + (d + e) * VP + 8 * tq) = y0;
-          *reinterpret_cast<h4*>(lds_v + (32 * DT + d + e) * VP + 8 * tq) = y1;
+          *reinterpret_cast<h4*>(lds_v + (d + e) * VP + 2 * tk) = y0;
+          *reinterpret_cast<h4*>(lds_v + (32 * DT + d + e) * VP + 2 * tk) = y1;
         }
       }
-      if (tid < TT) key_scale[tid] = ldexpf(1.0f, static_cast<int>(lk[tid] >> 23) - 141);
-      if (tid >= 64 && tid < 64 + TT) value_exp[tid - 64] = static_cast<int>(lv[tid - 64] >> 23);
-      if (tid >= 128 && tid < 128 + 2 * TT) largest[2 * TT * (which ^ 1) + tid - 128] = 0;
+      if (tid >= 64 && tid < 64 + TT) key_scale[tid - 64] = ldexpf(1.0f, static_cast<int>(lk[tid - 64] >> 23) - 141);
+      if (tid >= 128 && tid < 128 + TT) value_scale[tid - 128] = ldexpf(1.0f, static_cast<int>(lv[tid - 128] >> 23) - er);
+      if (tid < 2 * TT) largest[2 * TT * (which ^ 1) + tid] = 0;
     }
   };
 
@@ -412,101 +461,59 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
-  float m = -3.4028235e38f, l = 0.0f;
-  int er = SRC == kPaged ? 27 : 0;  // values are scaled by 2^-(er - 127) (paged), 2^-(er - 141) (fp32)
+  // bounds of what the wave's queries see: some of [from, upto), all of [all_from, all_upto)
+  int64_t from = qs.lo, upto = qs.hi, all_from = qs.lo, all_upto = qs.hi;
+  for (int off = 1; off < 32; off <<= 1) {
+    auto least = [&](int64_t v) { const int64_t o = __shfl_xor(v, off, 64); return o < v ? o : v; };
+    auto most = [&](int64_t v) { const int64_t o = __shfl_xor(v, off, 64); return o > v ? o : v; };
+    from = least(from);
+    upto = most(upto);
+    all_from = most(all_from);
+    all_upto = least(all_upto);
+  }
+  from = uniform(from);
+  upto = uniform(upto);
+  all_from = uniform(all_from);
+  all_upto = uniform(all_upto);
+  const bool by_query = rows_masked_by_query(rows, a);
+  if (wave * 32 >= count) upto = from = 0;  // (no queries: the wave only helps to bring tiles)
 
   if constexpr (SRC == kFloat) {
     if (tid < 2 * TT) largest[tid] = 0;
     __syncthreads();
   }
-  if (lo < hi) {
-    entries(lo);
-    if (kAhead) fetch(lo);
-    if (kAhead) entries(lo + TT);
+  if (kAhead && lo < hi) {
+    find_entry(lo);
+    fetch(lo);
+    find_entry(lo + TT);
   }
-  const bool mine = wave * 32 < count;
   int which = 0;
   for (int64_t t0 = lo; t0 < hi; t0 += TT, which ^= 1) {
-    if (!kAhead) fetch(t0);
-    if constexpr (SRC == kFloat) magnitudes(which);
+    if (!kAhead) {
+      find_entry(t0);
+      fetch(t0);
+    }
+    const bool empty = SRC != kPaged && word == 0;  // the same in all waves
+    if (SRC == kFloat && !empty) magnitudes(which);
     __syncthreads();  // the tile before is read
-    stage(which);
-    const uint64_t here = word;
-    const int page = page_s;
-    ks = ks1;
-    vs = page < 0 ? 0.0f : vs1;
+    if (!empty) stage(which);
+    const int page = page1;
+    const float ks = ks1, vs = page < 0 ? 0.0f : vs1;
     if (kAhead && t0 + TT < hi) {
       fetch(t0 + TT);
-      entries(t0 + 2 * TT);
+      find_entry(t0 + 2 * TT);
     }
     __syncthreads();
-    if (!mine) continue;
-    // what the lane's query sees of its tokens 32 s + 16 (i / 8) + 8 hf + i % 8: bit 16 s + i
-    uint32_t seen = 0xffffffffu >> (32 - 16 * NS);
-    {
-      const int64_t below = qs.lo - t0, upto = qs.hi - t0;
-      const bool whole = below <= 0 && upto >= TT;
-      bool all = whole;
-      if constexpr (SRC == kPaged)
-        all = all && page >= 0 && (__float_as_uint(vs) & 0x7f800000u) != 0x7f800000u;
-      else
-        all = all && here == ~uint64_t{0} >> (64 - TT);
-      if (SRC != kPaged && rows_masked_by_query(rows, a)) all = false;
-      if (!__all(all)) {
-        uint64_t w = 0;  // by token
-        const int lo32 = below < 0 ? 0 : below > TT ? TT : static_cast<int>(below);
-        const int hi32 = upto < 0 ? 0 : upto > TT ? TT : static_cast<int>(upto);
-        if (hi32 > lo32) w = (~uint64_t{0} >> (64 - (hi32 - lo32))) << lo32;
-        if constexpr (SRC == kPaged) {
-          const uint64_t pages = __ballot(page >= 0);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-            if (!(pages >> g & 1)) w &= ~(uint64_t{0xffff} << (16 * g));
-        } else {
-          w = query_mask(rows, a, b, qt, t0, TT, w & here);
-        }
-        w >>= 8 * hf;
-        seen = 0;
-#pragma unroll
-        for (int s = 0; s < 2 * NS; ++s) seen |= (static_cast<uint32_t>(w >> (16 * s)) & 0xffu) << (8 * s);
-        if (!__any(seen != 0)) continue;
-      } else {
-        seen = 0xffffffffu;  // (no test below)
-      }
-    }
-    const bool tested = !__all(seen == 0xffffffffu) ;
-
-    f16v s[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[j][e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const char* from = lds_k + (32 * j + n) * KP + 32 * k + 16 * hf;
-        const h8 k0 = *reinterpret_cast<const h8*>(from);
-        if constexpr (PK == 2) {
-          const h8 k1 = *reinterpret_cast<const h8*>(from + TT * KP);
-          s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qf[k][0], s[j], 0, 0, 0);
-        }
-        if constexpr (PQ == 2) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][PQ - 1], s[j], 0, 0, 0);
-        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][0], s[j], 0, 0, 0);
-      }
-    }
-
-    // the values' power of two
-    float keep_r = 1.0f;
-    if constexpr (SRC != kHalf) {
-      int e1 = 0;
-      if constexpr (SRC == kPaged) {
-        const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
-        e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
-        e1 = e1 > 254 ? 254 : e1;
-      } else {
-        e1 = lane < TT ? value_exp[lane % TT] : 0;
-      }
+    if (empty) which ^= 1;  // (the magnitudes' other half is not cleared)
+    // the values' power of two, as far as all tiles so far are: the scales' (a page
+    // without one that is finite poisons what sees it)
+    if constexpr (SRC == kPaged) {
+      const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
+      int e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
+      e1 = e1 > 254 ? 254 : e1;
+      keep_r = 1.0f;
       if (__any(e1 > er)) {
-        for (int off = 1; off < 64; off <<= 1) {
+        for (int off = 1; off < G; off <<= 1) {
           const int o = __shfl_xor(e1, off, 64);
           e1 = o > e1 ? o : e1;
         }
@@ -515,6 +522,55 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
         er = up;
       }
     }
+    if (keep_r != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] *= keep_r;
+      keep_r = 1.0f;
+    }
+    if (empty || t0 >= upto || t0 + TT <= from) continue;
+    // what the lane's query sees of its tokens 32 j + 16 k + 8 hf + e: bit 16 j + 8 k + e
+    uint32_t seen = 0;
+    bool tested = t0 < all_from || t0 + TT > all_upto || by_query;
+    if constexpr (SRC == kPaged)
+      tested = tested || !__all(page >= 0 && (__float_as_uint(vs) & 0x7f800000u) != 0x7f800000u);
+    if (tested) {
+      const int64_t below = qs.lo - t0, past = qs.hi - t0;
+      const int lo32 = below < 0 ? 0 : below > TT ? TT : static_cast<int>(below);
+      const int hi32 = past < 0 ? 0 : past > TT ? TT : static_cast<int>(past);
+      uint64_t w = hi32 > lo32 ? ~uint64_t{0} >> (64 - (hi32 - lo32)) << lo32 : 0;  // by token
+      if constexpr (SRC == kPaged) {
+        const uint64_t pages = __ballot(page >= 0);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (!(pages >> g & 1)) w &= ~(uint64_t{0xffff} << (16 * g));
+      } else {
+        w = query_mask(rows, a, b, qt, t0, TT, w);
+      }
+      w >>= 8 * hf;
+#pragma unroll
+      for (int s = 0; s < 2 * NS; ++s) seen |= (static_cast<uint32_t>(w >> (16 * s)) & 0xffu) << (8 * s);
+    }
+
+    f16v s[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const char* at_k = lds_k + (32 * j + n) * KP + 32 * k + 16 * hf;
+        const h8 k0 = *reinterpret_cast<const h8*>(at_k);
+        if constexpr (PK == 2) {
+          const h8 k1 = *reinterpret_cast<const h8*>(at_k + TT * KP);
+          s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qf[k][0], s[j], 0, 0, 0);
+        }
+        if constexpr (PQ == 2) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][PQ - 1], s[j], 0, 0, 0);
+        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][0], s[j], 0, 0, 0);
+      }
+    }
+
     float by[G], vw[G];
     if constexpr (SRC == kPaged) {
       const float r1 = __uint_as_float(static_cast<uint32_t>(254 - er) << 23);
@@ -524,19 +580,24 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
         vw[g] = r1 * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), g));
       }
     }
-    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NS; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        f4 kc = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (SRC == kFloat)
-          kc = *reinterpret_cast<const f4*>(key_scale + 32 * j + 16 * (c / 2) + 8 * hf + 4 * (c % 2));
+        const int tk = 32 * j + 16 * (c / 2) + 8 * hf + 4 * (c % 2);
+        if constexpr (SRC == kPaged) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = s[j][4 * c + e] * (SRC == kPaged ? by[(2 * j + c / 2) % G] : cq);
-          if constexpr (SRC == kFloat) x *= kc[e];
-          s[j][4 * c + e] = x;
+          for (int e = 0; e < 4; ++e) s[j][4 * c + e] *= by[(2 * j + c / 2) % G];
+        } else {
+          const f4 bias = *reinterpret_cast<const f4*>(key_bias + tk);
+          if constexpr (SRC == kHalf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = __builtin_fmaf(s[j][4 * c + e], cq, bias[e]);
+          } else {
+            const f4 kc = *reinterpret_cast<const f4*>(key_scale + tk);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = __builtin_fmaf(s[j][4 * c + e] * cq, kc[e], bias[e]);
+          }
         }
       }
     if (tested) {
@@ -545,19 +606,20 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[j][e] = seen >> (16 * j + e) & 1 ? s[j][e] : -INFINITY;
     }
+    float top = m;
 #pragma unroll
     for (int j = 0; j < NS; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[j][e]);
-    top = fmaxf(fmaxf(top, other_half(top)), m);
-    if (__any(top > m) || keep_r != 1.0f) {
-      const float keep = __builtin_amdgcn_exp2f(m - top), both = keep * keep_r;
+    top = fmaxf(top, other_half(top));
+    if (__any(top > m)) {
+      const float keep = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= keep;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] *= both;
+        for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
     }
     const float less = m - 15.0f;  // weights are 2^15 times as large, and their sum
 #pragma unroll
@@ -581,24 +643,29 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
         if constexpr (SRC == kFloat) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            typedef int i4 __attribute__((ext_vector_type(4)));
-            const i4 ve = *reinterpret_cast<const i4*>(value_exp + 32 * j + 16 * k + 8 * hf + 4 * c);
+            const f4 vc = *reinterpret_cast<const f4*>(value_scale + 32 * j + 16 * k + 8 * hf + 4 * c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[4 * c + e] = __builtin_amdgcn_ldexpf(w[4 * c + e], ve[e] - er);
+            for (int e = 0; e < 4; ++e) w[4 * c + e] *= vc[e];
           }
         }
         h8 pf[PW];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pf[0][e] = static_cast<_Float16>(w[e]);
-          if constexpr (PW == 2) pf[PW - 1][e] = static_cast<_Float16>(w[e] - static_cast<float>(pf[0][e]));
+        for (int e = 0; e < 8; e += 2) {
+          h2 p0, p1;
+          split2(w[e], w[e + 1], &p0, &p1);
+          pf[0][e] = p0[0];
+          pf[0][e + 1] = p0[1];
+          if constexpr (PW == 2) {
+            pf[PW - 1][e] = p1[0];
+            pf[PW - 1][e + 1] = p1[1];
+          }
         }
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
-          const char* from = lds_v + (32 * i + n) * VP + 64 * j + 32 * k + 16 * hf;
-          const h8 v0 = *reinterpret_cast<const h8*>(from);
+          const char* at_v = lds_v + (32 * i + n) * VP + 64 * j + 32 * k + 16 * hf;
+          const h8 v0 = *reinterpret_cast<const h8*>(at_v);
           if constexpr (PK == 2) {
-            const h8 v1 = *reinterpret_cast<const h8*>(from + 32 * DT * VP);
+            const h8 v1 = *reinterpret_cast<const h8*>(at_v + 32 * DT * VP);
             acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pf[0], acc[i], 0, 0, 0);
           }
           if constexpr (PW == 2) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pf[PW - 1], acc[i], 0, 0, 0);
@@ -607,39 +674,49 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : 4) ? 
       }
   }
 
-  // the sums by rows, in LDS
-  if (SRC == kHalf) bad &= 0x80008000u;
-  const bool marked = __syncthreads_or(SRC != kPaged && bad != 0);
+  // the sums by rows, half of them at a time, in LDS
+  const uint32_t none = SRC == kHalf ? bad & 0x80008000u : SRC == kFloat ? static_cast<uint32_t>(bad >= 0x7f800000u) : 0u;
+  const bool marked = __syncthreads_or(none != 0);
   const int pitch = D + 4;
   float* sums = reinterpret_cast<float*>(tile_lds);
-  float* wm = sums + kTileRows * pitch;
-  float* wl = wm + kTileRows;
+  float* wm = sums + kPutRows * pitch;
+  float* wl = wm + kPutRows;
   l += other_half(l);
-  const int r = wave * 32 + n;
-  if (r < count) {
-    const float by = SRC == kHalf ? 1.0f : ldexpf(1.0f, er - (SRC == kPaged ? 127 : 141));
+  const float scale = SRC == kHalf ? 1.0f : ldexpf(1.0f, er - (SRC == kPaged ? 127 : 141));
+  const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile, slot = int64_t{kPutRows} * (D + 2);
+  for (int part = 0; part * kPutRows < count; ++part) {
+    const int r = wave * 32 + n - part * kPutRows, here = count - part * kPutRows < kPutRows ? count - part * kPutRows : kPutRows;
+    __syncthreads();
+    if (r >= 0 && r < here) {
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int d = 32 * i + 8 * c + 4 * hf;
+        for (int c = 0; c < 4; ++c) {
+          const int d = 32 * i + 8 * c + 4 * hf;
+          const f4 v = f4{acc[i][4 * c], acc[i][4 * c + 1], acc[i][4 * c + 2], acc[i][4 * c + 3]} * scale;
+          if (D % 4 == 0) {
+            if (d < D) *reinterpret_cast<f4*>(sums + r * pitch + d) = v;
+          } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < D) sums[r * pitch + d + e] = acc[i][4 * c + e] * by;
+            for (int e = 0; e < 4; ++e)
+              if (d + e < D) sums[r * pitch + d + e] = v[e];
+          }
+        }
+      if (hf == 0) {
+        wm[r] = marked ? NAN : m;
+        wl[r] = l;
       }
-    if (hf == 0) {
-      wm[r] = marked ? NAN : m;
-      wl[r] = l;
     }
-  }
-  __syncthreads();
-  const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile, slot = int64_t{kTileRows} * (D + 2);
-  const Part part{b, h, count, chunk, chunks, first, cut.part + pair * cut.splits * slot, slot, cut.arrived + pair};
-  if (put_rows<T, kTileThreads>(a, part, sums, pitch, wm, wl, wl + kTileRows)) return;
-  __syncthreads();
-  for (int i = wave; i < count; i += kTileThreads / 64) {
-    const int64_t at_row = first + i;
-    one_query<T>(a, rows, b, at_row / a.group, h * a.group + static_cast<int>(at_row % a.group), sums + wave * kMaxHead);
+    __syncthreads();
+    const int64_t id = pair * (kTileRows / kPutRows) + part;
+    const Part out{b, h, here, chunk, chunks, first + part * kPutRows, cut.part + id * cut.splits * slot, slot,
+                   cut.arrived + id};
+    if (put_rows<T, kTileThreads>(a, out, sums, pitch, wm, wl, wl + kPutRows)) continue;
+    __syncthreads();
+    for (int i = wave; i < here; i += kTileThreads / 64) {
+      const int64_t at_row = out.first + i;
+      one_query<T>(a, rows, b, at_row / a.group, h * a.group + static_cast<int>(at_row % a.group), sums + wave * kMaxHead);
+    }
   }
 }
 
@@ -661,12 +738,12 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
   splits = splits < parts ? splits : parts;
   splits = splits < kMaxChunks ? splits : kMaxChunks;
   splits = splits < room ? splits : room;
-  if (splits < 1 || blocks > kRowCounters) splits = 1;
+  if (splits < 1 || blocks * (kTileRows / kPutRows) > kRowCounters) splits = 1;
   cut.splits = static_cast<int>(splits);
   cut.tiles = static_cast<int>(tiles);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
-  int64_t bytes = (int64_t{kTileRows} * (a.D + 4) + 2 * kTileRows + (splits > 1 ? splits * kTileRows : 0)) * 4;
+  int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows + (splits > 1 ? splits * kPutRows : 0)) * 4;
   if (bytes < tile_bytes(SRC, DT, TT)) bytes = tile_bytes(SRC, DT, TT);
   if (bytes < 4 * kMaxHead * 4) bytes = 4 * kMaxHead * 4;
   if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(attention_tile_kernel<T, Rows, SRC, DT, TT>)));
