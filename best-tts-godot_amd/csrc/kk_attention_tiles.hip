@@ -10,6 +10,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTileThreads = 256;
 constexpr int kTileRows = 128;  // queries of a block: 32 a wave
 constexpr int kPutRows = 64;    // of them put out at a time
+constexpr float kSlack = 7.0f;
 
 struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
@@ -33,8 +34,14 @@ constexpr int tile_bytes(int SRC, int DT, int TT) {
   return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 2 : 1) + (SRC == kFloat ? 7 : SRC == kHalf ? 1 : 0) * TT * 4;
 }
 
-__device__ __forceinline__ float other_half(float v) {  // the value of lane l ^ 32
-  return __shfl_xor(v, 32, 64);
+// The larger of, or the sum of, the values of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
 // Two values as the sum of two halves each.
@@ -75,8 +82,8 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // two, after a power of two for each row that brings its largest to 2^14, so
 // that 22 bits are kept whatever the rows' sizes, and the product of the two
 // low halves (2^-22) is left out.  Weights of fp16 queries are rounded to fp16
-// (half a step of the output's type); 2^15 p <= 2^15 keeps 24 bits above
-// fp16's smallest value.
+// (half a step of the output's type); that they are 2^8 times as large keeps 32
+// bits between the largest and fp16's smallest value.
 //
 // A state that is not finite poisons whole sums here (0 times it is NaN) where
 // only queries that see it should be: a block that meets one marks its part, and
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(x[s][i]));
-      top = fmaxf(top, other_half(top));
+      top = max_halves(top);
       const int up = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
       cq = ldexpf(a.scale, -up);
 #pragma unroll
@@ -553,24 +560,6 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       for (int s = 0; s < 2 * NS; ++s) seen |= (static_cast<uint32_t>(w >> (16 * s)) & 0xffu) << (8 * s);
     }
 
-    f16v s[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[j][e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const char* at_k = lds_k + (32 * j + n) * KP + 32 * k + 16 * hf;
-        const h8 k0 = *reinterpret_cast<const h8*>(at_k);
-        if constexpr (PK == 2) {
-          const h8 k1 = *reinterpret_cast<const h8*>(at_k + TT * KP);
-          s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qf[k][0], s[j], 0, 0, 0);
-        }
-        if constexpr (PQ == 2) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][PQ - 1], s[j], 0, 0, 0);
-        s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][0], s[j], 0, 0, 0);
-      }
-    }
-
     float by[G], vw[G];
     if constexpr (SRC == kPaged) {
       const float r1 = __uint_as_float(static_cast<uint32_t>(254 - er) << 23);
@@ -581,55 +570,66 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       }
     }
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
+    for (int j = 0; j < NS; ++j) {
+      f16v s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const char* at_k = lds_k + (32 * j + n) * KP + 32 * k + 16 * hf;
+        const h8 k0 = *reinterpret_cast<const h8*>(at_k);
+        if constexpr (PK == 2) {
+          const h8 k1 = *reinterpret_cast<const h8*>(at_k + TT * KP);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qf[k][0], s, 0, 0, 0);
+        }
+        if constexpr (PQ == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][PQ - 1], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][0], s, 0, 0, 0);
+      }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int tk = 32 * j + 16 * (c / 2) + 8 * hf + 4 * (c % 2);
         if constexpr (SRC == kPaged) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][4 * c + e] *= by[(2 * j + c / 2) % G];
+          for (int e = 0; e < 4; ++e) s[4 * c + e] *= by[(2 * j + c / 2) % G];
         } else {
           const f4 bias = *reinterpret_cast<const f4*>(key_bias + tk);
           if constexpr (SRC == kHalf) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = __builtin_fmaf(s[j][4 * c + e], cq, bias[e]);
+            for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e], cq, bias[e]);
           } else {
             const f4 kc = *reinterpret_cast<const f4*>(key_scale + tk);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = __builtin_fmaf(s[j][4 * c + e] * cq, kc[e], bias[e]);
+            for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e] * cq, kc[e], bias[e]);
           }
         }
       }
-    if (tested) {
+      if (tested) {
 #pragma unroll
-      for (int j = 0; j < NS; ++j)
+        for (int e = 0; e < 16; ++e) s[e] = seen >> (16 * j + e) & 1 ? s[e] : -INFINITY;
+      }
+      float top = s[0];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[j][e] = seen >> (16 * j + e) & 1 ? s[j][e] : -INFINITY;
-    }
-    float top = m;
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = max_halves(top);
+      // m follows a row's maximum only where that is kSlack above it: weights are
+      // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again
+      if (__any(top > m + kSlack)) {
+        top = fmaxf(top, m);
+        const float keep = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= keep;
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[j][e]);
-    top = fmaxf(top, other_half(top));
-    if (__any(top > m)) {
-      const float keep = __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      l *= keep;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
-    }
-    const float less = m - 15.0f;  // weights are 2^15 times as large, and their sum
-#pragma unroll
-    for (int j = 0; j < NS; ++j)
+          for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
+      }
+      const float less = m - 8.0f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(s[j][8 * k + e] - less);
+          w[e] = __builtin_amdgcn_exp2f(s[8 * k + e] - less);
           l += w[e];
         }
         if constexpr (SRC == kPaged) {
@@ -672,6 +672,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pf[0], acc[i], 0, 0, 0);
         }
       }
+    }
   }
 
   // the sums by rows, half of them at a time, in LDS
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   float* sums = reinterpret_cast<float*>(tile_lds);
   float* wm = sums + kPutRows * pitch;
   float* wl = wm + kPutRows;
-  l += other_half(l);
+  l = sum_halves(l);
   const float scale = SRC == kHalf ? 1.0f : ldexpf(1.0f, er - (SRC == kPaged ? 127 : 141));
   const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile, slot = int64_t{kPutRows} * (D + 2);
   for (int part = 0; part * kPutRows < count; ++part) {
