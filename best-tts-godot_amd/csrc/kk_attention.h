@@ -395,6 +395,14 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
   return true;
 }
 
+// Whether rows of an operand start at multiples of 16 bytes.
+inline bool rows_of_16(const void* p, const int64_t* strides, int size) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] * size % 16) return false;
+  return true;
+}
+
 // Entry points of the kernels; false where a call is not theirs.
 bool few_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status);
 bool few_dense_try(const QueryArgs& a, const DenseArgs& d, int dtype, int* status);

@@ -761,14 +761,6 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
                       : launch_tiles<T, Rows, SRC, 8, 32>(a, rows, tokens, wide, who);
 }
 
-// Whether rows of an operand start at multiples of 16 bytes.
-static bool rows_of_16(const void* p, const int64_t* strides, int size) {
-  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
-  for (int i = 0; i < 3; ++i)
-    if (strides[i] * size % 16) return false;
-  return true;
-}
-
 // (past the grid's axes: one query a wave)
 static bool too_many(const QueryArgs& a) {
   return a.B * (a.heads / a.group) > 65535 || int64_t{a.T} * a.group > int64_t{65535} * kTileRows;
