@@ -172,15 +172,19 @@ __device__ __forceinline__ void one_query(const QueryArgs& a, const Rows& rows, 
 // so that every CU has some.  How long they are is known on the device only,
 // so the blocks find their chunk there: with n_b steps of kStep tokens in
 // sequence b, a chunk is c = max(least, ceil(sum n_b / units)) steps, one and
-// the same for all, so that ragged batches load the CUs evenly.  At most
-// units + B chunks come of that, times the key heads: the grid.
+// the same for all, so that ragged batches load the CUs evenly: with as many
+// units as run at once, or, once those would pass kLongChunk steps, with
+// `most`, which even out what some take longer.  At most most + B chunks come of
+// that, times the key heads: the grid.  (24 sequences of up to 8000 tokens, 4 key
+// heads of 96: 54 us in chunks of 8 steps, 44 in one round of blocks.)
 constexpr int kStep = 64;
-constexpr int kMaxChunks = 64;  // of a sequence: what the block that joins them reads
+constexpr int kLongChunk = 64;
+constexpr int kMaxChunks = 64;  // of a sequence: a wave of the block that joins them has a lane for each
 
 struct Cut {
   int64_t B;
   int heads;           // key heads
-  int64_t units;       // chunks to aim for, for each head
+  int64_t units, most; // chunks to aim for, for each head: as many as run at once, as many as long ones make
   int64_t least;       // steps of a chunk at least
   int64_t rows;        // queries of a key head: T * group
   float* part;         // a slot of rows * (D + 2) floats a block
@@ -220,6 +224,10 @@ __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit
   for (int64_t b = 64 + lane; b < cut.B; b += 64) total += steps_of(b);
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
   int64_t c = ceil_div(total, cut.units);
+  if (c > kLongChunk && cut.most > cut.units) {
+    c = ceil_div(total, cut.most);
+    c = c < kLongChunk ? kLongChunk : c;
+  }
   c = c < cut.least ? cut.least : c;
   int64_t before = 0;
   for (int64_t b0 = 0; b0 < cut.B; b0 += 64) {
@@ -250,26 +258,30 @@ __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit
   return false;
 }
 
-// Chunks and grid for `most` tokens a sequence at the most; *blocks the grid.
+// Chunks and grid for `most` tokens a sequence at the most, `round` blocks running
+// at once; *blocks the grid.
 // Where scratch or counters do not hold a slot for each, sequences stay whole.
-inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int64_t least, int64_t aim, Cut* cut,
+inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int64_t least, int64_t round, Cut* cut,
                     int64_t* blocks, const char* who) {
   const int64_t slots = static_cast<int64_t>(kScratchBytes / 4) / (rows * (D + 2)) / heads;
   cut->B = B;
   cut->heads = heads;
   cut->rows = rows;
   cut->least = least;
-  cut->units = ceil_div(aim, heads);
+  cut->units = ceil_div(round, heads);
+  cut->most = ceil_div(8 * ctx().num_cus, heads);
+  if (cut->most < cut->units) cut->most = cut->units;
   cut->part = static_cast<float*>(ctx().scratch);
   cut->arrived = ctx().row_counters;
   int64_t n = B * (most / kStep / least + 2);  // (two: a window's first step may hold tokens it does not see)
-  if (n > B + cut->units) n = B + cut->units;
+  if (n > B + cut->most) n = B + cut->most;
   if (n > slots) {
-    cut->units = slots - B;
+    cut->most = slots - B;
+    if (cut->units > cut->most) cut->units = cut->most;
     n = slots;
   }
   if (cut->units < 1 || B * heads > kRowCounters) {
-    cut->units = 1;
+    cut->units = cut->most = 1;
     cut->least = int64_t{1} << 40;
     n = B;
   }
@@ -296,8 +308,8 @@ struct Part {
 // joined from there: always in the chunks' order.  The order of slot and
 // counter is that of the row reductions: stores that write through to where
 // all XCDs read, a wait for them, then the count; no whole cache is written
-// back.  Called by all threads, after a barrier; `weights` holds chunks * rows
-// floats.  False, with nothing put out, where a row's maximum is NaN: a part
+// back.  Called by all threads, after a barrier; `weights` holds
+// 2 * chunks * rows floats.  False, with nothing put out, where a row's maximum is NaN: a part
 // that the caller has marked as not to be used.
 template <typename T, int THREADS>
 __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, const float* acc, int pitch,
@@ -358,37 +370,41 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
     __hip_atomic_store(u.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  // weights[i][r] = 2^(m_i - max) / sum_i l_i 2^(m_i - max)
-  for (int r = threadIdx.x; r < rows; r += THREADS) {
-    float top = -INFINITY, sum = 0.0f;
-    bool marked = false;
-    for (int i = 0; i < u.chunks; ++i) {
-      const float mi = get(u.slots + i * u.next + rows * D + r);
-      weights[i * rows + r] = mi;
-      marked = marked || mi != mi;
-      top = fmaxf(top, mi);
-    }
-    if (marked) shared = 1;
-    for (int i = 0; i < u.chunks; ++i) {
-      const float w = exp2f(weights[i * rows + r] - top);
-      weights[i * rows + r] = w;
-      sum += w * get(u.slots + i * u.next + rows * D + rows + r);
-    }
-    const float by = sum != 0.0f ? 1.0f / sum : 0.0f;
-    for (int i = 0; i < u.chunks; ++i) weights[i * rows + r] *= by;
+  // weights[i][r] = 2^(m_i - max) / sum_i l_i 2^(m_i - max), from all parts' m and
+  // l at once (one after the other, each would wait its whole way)
+  float* sums = weights + u.chunks * rows;
+  for (int i = threadIdx.x; i < u.chunks * rows; i += THREADS) {
+    const float* at = u.slots + (i / rows) * u.next + rows * D + i % rows;
+    weights[i] = get(at);
+    sums[i] = get(at + rows);
+  }
+  __syncthreads();
+  for (int r = threadIdx.x / 64; r < rows; r += THREADS / 64) {  // a wave a row, a lane a part
+    const int i = threadIdx.x % 64;
+    const float mi = i < u.chunks ? weights[i * rows + r] : -INFINITY;
+    if (mi != mi) shared = 1;
+    const float w = exp2f(mi - wave_max_dpp(mi));
+    const float sum = wave_sum_dpp(i < u.chunks ? w * sums[i * rows + r] : 0.0f);
+    if (i < u.chunks) weights[i * rows + r] = sum != 0.0f ? w / sum : 0.0f;
   }
   __syncthreads();
   if (shared) return false;
   for (int i = threadIdx.x; i < rows * D; i += THREADS) {
     const int r = i / D, d = i - r * D;
     float sum = 0.0f;
-    for (int j0 = 0; j0 < u.chunks; j0 += 8) {
-      float x[8];
+    auto some = [&](int j0, auto batch) {  // (past the last part: it again, without weight)
+      constexpr int N = decltype(batch)::value;
+      float x[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j0 + j < u.chunks ? get(u.slots + (j0 + j) * u.next + i) : 0.0f;
+      for (int j = 0; j < N; ++j) x[j] = get(u.slots + (j0 + j < u.chunks ? j0 + j : u.chunks - 1) * u.next + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < N; ++j)
         if (j0 + j < u.chunks) sum = __builtin_fmaf(weights[(j0 + j) * rows + r], x[j], sum);
+    };
+    if (u.chunks <= 4) {
+      some(0, std::integral_constant<int, 4>{});
+    } else {
+      for (int j0 = 0; j0 < u.chunks; j0 += 16) some(j0, std::integral_constant<int, 16>{});
     }
     out(r, d, sum);
   }

@@ -367,12 +367,12 @@ static int launch_few(const QueryArgs& a, const PagedRows& rows, int64_t queries
   const int64_t seen = rows.a.window ? rows.a.window + a.T - 1 : capacity;
   Cut cut;
   int64_t blocks;
-  KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 8, int64_t{8} * ctx().num_cus,
+  KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 16, int64_t{2} * ctx().num_cus,
                   &cut, &blocks, "cache_attention"));
   // codes; then the waves' sums; then, beside the first's, the chunks' weights
   const int R = static_cast<int>(queries);
   const size_t codes = size_t{kFewWaves} * 2 * 64 * a.D, sums = size_t{kFewWaves} * R * (a.D + 4) * 4;
-  const size_t joined = static_cast<size_t>(R) * (a.D + 4 + kMaxChunks) * 4;
+  const size_t joined = static_cast<size_t>(R) * (a.D + 4 + 2 * kMaxChunks) * 4;
   size_t bytes = codes > sums ? codes : sums;
   bytes = (2 * (kFewWaves + 1) * R * 4 + 15) / 16 * 16 + (bytes > joined ? bytes : joined);
   const void* kernel = reinterpret_cast<const void*>(few_paged_kernel<T, DT, NT, EXACT>);

@@ -196,11 +196,11 @@ static int launch_states(const QueryArgs& a, const DenseRows<T>& rows, int64_t q
   constexpr int U = R > 4 ? 2 : 4;
   Cut cut;
   int64_t blocks;
-  KK_TRY(plan_cut(a.B, a.heads / a.group, queries, a.D, rows.a.S, 4, int64_t{8} * ctx().num_cus, &cut, &blocks,
+  KK_TRY(plan_cut(a.B, a.heads / a.group, queries, a.D, rows.a.S, R > 4 ? 1 : 4, int64_t{8} * ctx().num_cus, &cut, &blocks,
                   "cross_attention"));
   // the waves' sums; then, beside the first's, the chunks' weights
   const int pitch = (a.D + 7) / 4 * 4;
-  const size_t sums = size_t{kStateWaves} * R * pitch, joined = size_t{R} * (pitch + kMaxChunks);
+  const size_t sums = size_t{kStateWaves} * R * pitch, joined = size_t{R} * (pitch + 2 * kMaxChunks);
   const size_t bytes = 4 * (2 * (kStateWaves + 1) * R + 4 + (sums > joined ? sums : joined));
   KK_LAUNCH((few_states_kernel<T, LANES, R, U>), dim3(static_cast<unsigned>(blocks)), dim3(kStateThreads), bytes,
             ctx().stream, a, rows, cut);

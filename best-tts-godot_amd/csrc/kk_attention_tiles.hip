@@ -744,7 +744,7 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
   cut.tiles = static_cast<int>(tiles);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
-  int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows + (splits > 1 ? splits * kPutRows : 0)) * 4;
+  int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows + (splits > 1 ? 2 * splits * kPutRows : 0)) * 4;
   if (bytes < tile_bytes(SRC, DT, TT)) bytes = tile_bytes(SRC, DT, TT);
   if (bytes < 4 * kMaxHead * 4) bytes = 4 * kMaxHead * 4;
   if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(attention_tile_kernel<T, Rows, SRC, DT, TT>)));
