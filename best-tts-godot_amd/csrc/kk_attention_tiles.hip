@@ -10,6 +10,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTileThreads = 256;
 constexpr int kTileRows = 128;  // queries of a block: 32 a wave
 constexpr int kPutRows = 64;    // of them put out at a time
+constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
 constexpr float kSlack = 7.0f;
 
 struct TileCut {
@@ -17,9 +18,12 @@ struct TileCut {
   int tiles;           // of kTileRows queries in a sequence and key head
   int64_t rows;        // queries of a sequence and key head: T * group
   int wide;            // rows of q, k and v take 16-byte accesses
+  // of each tile of queries, where splits > 1: the parts that it has, and those
+  // parts' sums [kTileRows][D], maxima and sums of powers [kTileRows]
+  int* parts;
   float* part;
-  int* arrived;
 };
+constexpr int64_t part_floats(int D) { return int64_t{kTileRows} * (D + 2); }
 
 // Where the tile kernel's operands come from.
 enum Source { kPaged, kHalf, kFloat };
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   lo = lo / TT * TT;
   const int64_t steps = ceil_div(hi - lo, TT);
   int64_t each = ceil_div(steps, cut.splits);
-  each = each < 4 ? 4 : each;
+  each = each < kLeastTiles ? kLeastTiles : each;
   const int chunks = steps <= each ? 1 : static_cast<int>(ceil_div(steps, each));
   const int chunk = static_cast<int>(at.x);
   if (chunk >= chunks) return;
@@ -684,7 +688,33 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   float* wl = wm + kPutRows;
   l = sum_halves(l);
   const float scale = SRC == kHalf ? 1.0f : ldexpf(1.0f, er - (SRC == kPaged ? 127 : 141));
-  const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile, slot = int64_t{kPutRows} * (D + 2);
+  const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile;
+  if (cut.splits > 1 && chunk == 0 && tid == 0) cut.parts[pair] = chunks;
+  if (chunks > 1) {
+    float* to = cut.part + (pair * cut.splits + chunk) * part_floats(D);
+    const int r = wave * 32 + n;
+    if (r < count) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int d = 32 * i + 8 * c + 4 * hf;
+          const f4 v = f4{acc[i][4 * c], acc[i][4 * c + 1], acc[i][4 * c + 2], acc[i][4 * c + 3]} * scale;
+          if (D % 4 == 0) {
+            if (d < D) *reinterpret_cast<f4*>(to + r * D + d) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d + e < D) to[r * D + d + e] = v[e];
+          }
+        }
+      if (hf == 0) {
+        to[kTileRows * D + r] = marked ? NAN : m;
+        to[kTileRows * D + kTileRows + r] = l;
+      }
+    }
+    return;
+  }
   for (int part = 0; part * kPutRows < count; ++part) {
     const int r = wave * 32 + n - part * kPutRows, here = count - part * kPutRows < kPutRows ? count - part * kPutRows : kPutRows;
     __syncthreads();
@@ -709,15 +739,48 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       }
     }
     __syncthreads();
-    const int64_t id = pair * (kTileRows / kPutRows) + part;
-    const Part out{b, h, here, chunk, chunks, first + part * kPutRows, cut.part + id * cut.splits * slot, slot,
-                   cut.arrived + id};
-    if (put_rows<T, kTileThreads>(a, out, sums, pitch, wm, wl, wl + kPutRows)) continue;
+    const Part out{b, h, here, 0, 1, first + part * kPutRows, nullptr, 0, nullptr};
+    if (put_rows<T, kTileThreads>(a, out, sums, pitch, wm, wl, nullptr)) continue;
     __syncthreads();
     for (int i = wave; i < here; i += kTileThreads / 64) {
       const int64_t at_row = out.first + i;
       one_query<T>(a, rows, b, at_row / a.group, h * a.group + static_cast<int>(at_row % a.group), sums + wave * kMaxHead);
     }
+  }
+}
+
+// Joins the parts of queries whose tokens were shared by several blocks, a wave a
+// query: weights 2^(m_i - max) / sum_i l_i 2^(m_i - max), a lane a part.
+template <typename T, class Rows>
+__global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, Rows rows, TileCut cut) {
+  __shared__ float qv[kTileThreads / 64][kMaxHead];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = a.D;
+  constexpr int kRows = kTileThreads / 64;
+  const int64_t unit = blockIdx.x / (kTileRows / kRows);
+  const int r = blockIdx.x % (kTileRows / kRows) * kRows + wave;
+  const int64_t row = unit % cut.tiles * kTileRows + r, pair = unit / cut.tiles;
+  const int parts = cut.parts[unit];
+  if (row >= cut.rows || parts <= 1) return;
+  const int heads = a.heads / a.group;
+  const int64_t b = pair / heads, t = row / a.group;
+  const int head = static_cast<int>(pair % heads) * a.group + static_cast<int>(row % a.group);
+  const float* from = cut.part + unit * cut.splits * part_floats(D);
+  const float* ml = from + kTileRows * D + r;
+  const float m = lane < parts ? ml[lane * part_floats(D)] : -INFINITY;
+  const float l = lane < parts ? ml[lane * part_floats(D) + kTileRows] : 0.0f;
+  if (__any(m != m)) {
+    one_query<T>(a, rows, b, t, head, qv[wave]);
+    return;
+  }
+  const float w = exp2f(m - wave_max_dpp(m)), sum = wave_sum_dpp(w * l);
+  const float by = sum != 0.0f ? w / sum : 0.0f;
+  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
+  for (int d = lane; d < D; d += 64) {
+    float v = 0.0f;
+    for (int i = 0; i < parts; ++i)
+      v = __builtin_fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(by), i)),
+                         from[i * part_floats(D) + r * D + d], v);
+    from_f32(y[d], v);
   }
 }
 
@@ -728,29 +791,33 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
   TileCut cut{};
   cut.rows = queries;
   cut.wide = wide;
-  cut.part = static_cast<float*>(ctx().scratch);
-  cut.arrived = ctx().row_counters;
   // where there are fewer blocks than two a CU, the tokens are cut, into parts
-  // of four tiles at least
-  const int64_t blocks = pairs * tiles;
+  // of two tiles at least
+  const int64_t blocks = pairs * tiles, head = (blocks * 4 + 15) / 16 * 16;
   int64_t splits = ceil_div(2 * ctx().num_cus, blocks);
-  const int64_t room = static_cast<int64_t>(kScratchBytes / 4) / (int64_t{kTileRows} * (a.D + 2)) / blocks;
-  const int64_t parts = ceil_div(tokens, 4 * TT);
+  const int64_t room = (static_cast<int64_t>(kScratchBytes) - head) / 4 / part_floats(a.D) / blocks;
+  const int64_t parts = ceil_div(tokens, kLeastTiles * TT);
   splits = splits < parts ? splits : parts;
   splits = splits < kMaxChunks ? splits : kMaxChunks;
   splits = splits < room ? splits : room;
-  if (splits < 1 || blocks * (kTileRows / kPutRows) > kRowCounters) splits = 1;
+  if (splits < 1) splits = 1;
+  cut.parts = static_cast<int*>(ctx().scratch);
+  cut.part = reinterpret_cast<float*>(static_cast<char*>(ctx().scratch) + head);
   cut.splits = static_cast<int>(splits);
   cut.tiles = static_cast<int>(tiles);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
-  int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows + (splits > 1 ? 2 * splits * kPutRows : 0)) * 4;
+  int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows) * 4;
   if (bytes < tile_bytes(SRC, DT, TT)) bytes = tile_bytes(SRC, DT, TT);
   if (bytes < 4 * kMaxHead * 4) bytes = 4 * kMaxHead * 4;
   if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(attention_tile_kernel<T, Rows, SRC, DT, TT>)));
   KK_LAUNCH((attention_tile_kernel<T, Rows, SRC, DT, TT>), grid, dim3(kTileThreads), static_cast<unsigned>(bytes),
             ctx().stream, a, rows, cut);
-  return check_launch("attention_tile_kernel");
+  KK_TRY(check_launch("attention_tile_kernel"));
+  if (splits == 1) return KK_OK;
+  KK_LAUNCH((join_parts_kernel<T, Rows>), dim3(static_cast<unsigned>(blocks * (kTileRows / (kTileThreads / 64)))),
+            dim3(kTileThreads), 0, ctx().stream, a, rows, cut);
+  return check_launch("join_parts_kernel");
 }
 
 template <typename T, class Rows, int SRC>
