@@ -544,8 +544,11 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
     // what the lane's query sees of its tokens 32 j + 16 k + 8 hf + e: bit 16 j + 8 k + e
     uint32_t seen = 0;
     bool tested = t0 < all_from || t0 + TT > all_upto || by_query;
-    if constexpr (SRC == kPaged)
-      tested = tested || !__all(page >= 0 && (__float_as_uint(vs) & 0x7f800000u) != 0x7f800000u);
+    bool poisoned = false;
+    if constexpr (SRC == kPaged) {
+      poisoned = __any((__float_as_uint(vs) & 0x7f800000u) == 0x7f800000u);
+      tested = tested || poisoned || !__all(page >= 0);
+    }
     if (tested) {
       const int64_t below = qs.lo - t0, past = qs.hi - t0;
       const int lo32 = below < 0 ? 0 : below > TT ? TT : static_cast<int>(below);
@@ -572,108 +575,140 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
         by[g] = cq * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), g));
         vw[g] = r1 * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), g));
       }
+      if (poisoned) {  // a scale that is not finite, for the queries that see its tokens
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (!(__builtin_fabsf(vw[g]) < INFINITY)) {
+            vw[g] = 0.0f;
+            if (seen >> (8 * g) & 0xff) l = NAN;
+          }
+      }
     }
+    {
+      // fragments of keys or values are read a batch ahead of their products
+      constexpr int KB = DT > 4 ? 1 : 2, BATCHES = KS / KB, VB = DT > 4 || DT % 2 ? 1 : 2, VBATCHES = DT / VB;
+      h8 kf[2][KB][PK], vf[2][VB][PK];
+      auto read_keys = [&](int j, int batch, h8 (&to)[KB][PK]) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      f16v s;
+        for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+          for (int part = 0; part < PK; ++part)
+            to[k][part] = *reinterpret_cast<const h8*>(lds_k + (part * TT + 32 * j + n) * KP + 32 * (batch * KB + k) + 16 * hf);
+      };
+      auto read_values = [&](int step, int batch, h8 (&to)[VB][PK]) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const char* at_k = lds_k + (32 * j + n) * KP + 32 * k + 16 * hf;
-        const h8 k0 = *reinterpret_cast<const h8*>(at_k);
-        if constexpr (PK == 2) {
-          const h8 k1 = *reinterpret_cast<const h8*>(at_k + TT * KP);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qf[k][0], s, 0, 0, 0);
+        for (int i = 0; i < VB; ++i)
+#pragma unroll
+          for (int part = 0; part < PK; ++part)
+            to[i][part] = *reinterpret_cast<const h8*>(lds_v + (part * 32 * DT + 32 * (batch * VB + i) + n) * VP + 32 * step + 16 * hf);
+      };
+      read_keys(0, 0, kf[0]);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        f16v s;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+        for (int batch = 0; batch < BATCHES; ++batch) {
+          const int now = (j * BATCHES + batch) % 2;
+          if (batch + 1 < BATCHES)
+            read_keys(j, batch + 1, kf[now ^ 1]);
+          else
+            read_values(2 * j, 0, vf[0]);
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            const int q = batch * KB + k;
+            if constexpr (PK == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][PK - 1], qf[q][0], s, 0, 0, 0);
+            if constexpr (PQ == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][0], qf[q][PQ - 1], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][0], qf[q][0], s, 0, 0, 0);
+          }
         }
-        if constexpr (PQ == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][PQ - 1], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qf[k][0], s, 0, 0, 0);
-      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int tk = 32 * j + 16 * (c / 2) + 8 * hf + 4 * (c % 2);
-        if constexpr (SRC == kPaged) {
+        for (int c = 0; c < 4; ++c) {
+          const int tk = 32 * j + 16 * (c / 2) + 8 * hf + 4 * (c % 2);
+          if constexpr (SRC == kPaged) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * c + e] *= by[(2 * j + c / 2) % G];
-        } else {
-          const f4 bias = *reinterpret_cast<const f4*>(key_bias + tk);
-          if constexpr (SRC == kHalf) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e], cq, bias[e]);
+            for (int e = 0; e < 4; ++e) s[4 * c + e] *= by[(2 * j + c / 2) % G];
           } else {
-            const f4 kc = *reinterpret_cast<const f4*>(key_scale + tk);
+            const f4 bias = *reinterpret_cast<const f4*>(key_bias + tk);
+            if constexpr (SRC == kHalf) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e] * cq, kc[e], bias[e]);
+              for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e], cq, bias[e]);
+            } else {
+              const f4 kc = *reinterpret_cast<const f4*>(key_scale + tk);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e] * cq, kc[e], bias[e]);
+            }
           }
         }
-      }
-      if (tested) {
+        if (tested) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = seen >> (16 * j + e) & 1 ? s[e] : -INFINITY;
-      }
-      float top = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top = max_halves(top);
-      // m follows a row's maximum only where that is kSlack above it: weights are
-      // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again
-      if (__any(top > m + kSlack)) {
-        top = fmaxf(top, m);
-        const float keep = __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        l *= keep;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
-      }
-      const float less = m - 8.0f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(s[8 * k + e] - less);
-          l += w[e];
+          for (int e = 0; e < 16; ++e) s[e] = seen >> (16 * j + e) & 1 ? s[e] : -INFINITY;
         }
-        if constexpr (SRC == kPaged) {
+        float top = s[0];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] *= vw[(2 * j + k) % G];
-          if (tested) {  // (past a scale that is not finite)
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+        top = max_halves(top);
+        // m follows a row's maximum only where that is kSlack above it: weights are
+        // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again
+        if (__any(top > m + kSlack)) {
+          top = fmaxf(top, m);
+          const float keep = __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          l *= keep;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = seen >> (16 * j + 8 * k + e) & 1 ? w[e] : 0.0f;
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
+        }
+        const float less = m - 8.0f;
+        h8 pf[2][PW];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w[e] = __builtin_amdgcn_exp2f(s[8 * k + e] - less);
+            l += w[e];
           }
-        }
-        if constexpr (SRC == kFloat) {
+          if constexpr (SRC == kPaged) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const f4 vc = *reinterpret_cast<const f4*>(value_scale + 32 * j + 16 * k + 8 * hf + 4 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[4 * c + e] *= vc[e];
+            for (int e = 0; e < 8; ++e) w[e] *= vw[(2 * j + k) % G];
           }
-        }
-        h8 pf[PW];
+          if constexpr (SRC == kFloat) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          h2 p0, p1;
-          split2(w[e], w[e + 1], &p0, &p1);
-          pf[0][e] = p0[0];
-          pf[0][e + 1] = p0[1];
-          if constexpr (PW == 2) {
-            pf[PW - 1][e] = p1[0];
-            pf[PW - 1][e + 1] = p1[1];
+            for (int c = 0; c < 2; ++c) {
+              const f4 vc = *reinterpret_cast<const f4*>(value_scale + 32 * j + 16 * k + 8 * hf + 4 * c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[4 * c + e] *= vc[e];
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            h2 p0, p1;
+            split2(w[e], w[e + 1], &p0, &p1);
+            pf[k][0][e] = p0[0];
+            pf[k][0][e + 1] = p0[1];
+            if constexpr (PW == 2) {
+              pf[k][PW - 1][e] = p1[0];
+              pf[k][PW - 1][e + 1] = p1[1];
+            }
           }
         }
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const char* at_v = lds_v + (32 * i + n) * VP + 64 * j + 32 * k + 16 * hf;
-          const h8 v0 = *reinterpret_cast<const h8*>(at_v);
-          if constexpr (PK == 2) {
-            const h8 v1 = *reinterpret_cast<const h8*>(at_v + 32 * DT * VP);
-            acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pf[0], acc[i], 0, 0, 0);
+        for (int step = 0; step < 2 * VBATCHES; ++step) {
+          const int k = step / VBATCHES, batch = step % VBATCHES;
+          if (step + 1 < 2 * VBATCHES)
+            read_values(2 * j + (step + 1) / VBATCHES, (step + 1) % VBATCHES, vf[(step + 1) % 2]);
+          else if (j + 1 < NS)
+            read_keys(j + 1, 0, kf[(j + 1) * BATCHES % 2]);
+#pragma unroll
+          for (int i = 0; i < VB; ++i) {
+            f16v& o = acc[batch * VB + i];
+            if constexpr (PK == 2) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][PK - 1], pf[k][0], o, 0, 0, 0);
+            if constexpr (PW == 2) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][0], pf[k][PW - 1], o, 0, 0, 0);
+            o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][0], pf[k][0], o, 0, 0, 0);
           }
-          if constexpr (PW == 2) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pf[PW - 1], acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pf[0], acc[i], 0, 0, 0);
         }
       }
     }
