@@ -122,6 +122,7 @@ PROTOTYPES = {
     "kk_fir_pcm16": [_T, _T, _T, _i, _f],
     "kk_qk_norm_rotary": [_T] * 8 + [_f, _i, _f],
     "kk_cache_append": [_T] * 9,
+    "kk_cache_values": [_T] * 6,
     "kk_cache_attention": [_T] * 9 + [_f, ctypes.c_int64],
     "kk_cross_attention": [_T] * 6 + [_f],
     "kk_process_logits": [_T] * 9,

@@ -41,9 +41,7 @@ class KVCache:
     def values(self):
         """What the codes stand for, as float32: keys [pages, heads, block, D]
         and values [pages, heads, D, block]."""
-        shape = self.k_scale.shape + (1, 1)
-        return (ops.dequantize(self.k, self.k_scale.reshape(shape)),
-                ops.dequantize(self.v, self.v_scale.reshape(shape)))
+        return ops.cache_values(self)
 
 
 def rotary_turns(dim, base=10000.0, factor=1.0, old_length=None, low=1.0, high=4.0):

@@ -67,9 +67,9 @@ struct CacheShape {
   int64_t pages, heads, block, D, columns, table_stride;
 };
 
-// Checks a cache's four tensors and a table of its pages against each other.
-inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
-                       const kk_tensor* v_scales, const kk_tensor* table, CacheShape* c, const char* who) {
+// Checks a cache's four tensors against each other.
+inline int check_codes(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                       const kk_tensor* v_scales, CacheShape* c, const char* who) {
   const kk_tensor *codes[2] = {k_codes, v_codes}, *scales[2] = {k_scales, v_scales};
   const char *names[2] = {"k_codes", "v_codes"}, *snames[2] = {"k_scales", "v_scales"};
   for (int i = 0; i < 2; ++i) {
@@ -98,6 +98,14 @@ inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, cons
                      static_cast<long long>(c->D));
   if (c->heads < 1 || c->heads > 65535) return set_error(KK_E_UNSUPPORTED, "%s: %lld heads", who,
                                                          static_cast<long long>(c->heads));
+  c->columns = c->table_stride = 0;
+  return KK_OK;
+}
+
+// The same with a table of its pages.
+inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                       const kk_tensor* v_scales, const kk_tensor* table, CacheShape* c, const char* who) {
+  KK_TRY(check_codes(k_codes, k_scales, v_codes, v_scales, c, who));
   KK_TRY(check_tensor(table, "table"));
   if (table->dtype != KK_I32 || table->rank != 2)
     return set_error(KK_E_ARG, "%s: table must be int32 [sequences, pages]", who);

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_rotary_kernel(RotArgs a, 
 // Whether rows of t start at multiples of `bytes` (VEC-wide accesses).
 static bool rows_aligned(const kk_tensor* t, int bytes) {
   if (reinterpret_cast<uintptr_t>(t->data) % bytes) return false;
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i + 1 < t->rank; ++i)
     if (t->shape[i] > 1 && (t->strides[i] * dtype_size(t->dtype)) % bytes) return false;
   return true;
 }
@@ -238,11 +238,16 @@ constexpr int kAppendThreads = 256;
 // keys (blockIdx.z even) or values (odd): the block that has a page alone
 // reads and writes it, so no two blocks meet.  s' = max(s, largest / 127)
 // where the page holds rows before the new ones (which are brought to s'),
-// largest / 127 where it holds none.
-template <typename T>
+// largest / 127 where it holds none.  Bound by memory (long calls): rows come in
+// 16 bytes a lane, the second time from the caches; keys' codes go out as they
+// come, values' codes through LDS, where a row of the page is 16 tokens of one
+// value, so that both write whole pieces of lines.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(AppendArgs a) {
   __shared__ float part[kAppendThreads / 64];
-  const int b = blockIdx.x, h = blockIdx.y, which = blockIdx.z & 1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t turned[];  // values: [D][block + 4]
+  constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
+  const int b = blockIdx.x, h = blockIdx.y, which = blockIdx.z & 1, D = a.D;
   int64_t count = a.T;
   if (a.counts) count = load_index(a.counts, a.counts_dt, b * a.counts_st);
   const PageRows w = page_rows(load_index(a.starts, a.starts_dt, b * a.starts_st), count, a.T, a.block, a.columns,
@@ -250,15 +255,20 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(AppendArgs
   if (w.rows <= 0) return;
   const int64_t page = a.table[b * a.table_stride + w.column];
   if (page < 0 || page >= a.pages) return;
-  const T* x = static_cast<const T*>(a.x[which]) + b * a.xs[which][0] + w.token * a.xs[which][1] +
-               h * a.xs[which][2];
-  const int n = w.rows * a.D;
+  const int64_t xt = a.xs[which][1];
+  const T* x = static_cast<const T*>(a.x[which]) + b * a.xs[which][0] + w.token * xt + h * a.xs[which][2];
+  const int per = D / VEC, n = w.rows * per;  // pieces of a row, and all
   float top = 0.0f;
   for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    const float v = __builtin_fabsf(to_f32(x[(i / a.D) * a.xs[which][1] + i % a.D]));
-    if (v < INFINITY) top = fmaxf(top, v);
+    const int r = i / per, d = (i - r * per) * VEC;
+    const Chunk<T, VEC> c = *reinterpret_cast<const Chunk<T, VEC>*>(x + r * xt + d);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float v = __builtin_fabsf(to_f32(c.v[e]));
+      if (v < INFINITY) top = fmaxf(top, v);
+    }
   }
-  top = wave_max(top);
+  top = wave_max_dpp(top);
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
   float* scale = a.scales[which] + page * a.Hk + h;
   const float before = w.held ? *scale : 0.0f;
@@ -267,20 +277,91 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(AppendArgs
   // a page of values below 2^-119 keeps a scale that can be divided by
   const float want = top > 0.0f ? fmaxf(top / 127.0f, 0x1p-126f) : 0.0f;
   const float s = fmaxf(before, want);
-  int8_t* codes = a.codes[which] + (page * a.Hk + h) * a.block * a.D;
+  int8_t* codes = a.codes[which] + (page * a.Hk + h) * a.block * D;
   if (threadIdx.x == 0) *scale = s;
   if (w.held && s != before) {
-    const double from = before;
-    for (int i = threadIdx.x; i < w.held * a.D; i += kAppendThreads) {
-      int8_t* c = which ? codes + (i % a.D) * a.block + i / a.D : codes + i;
-      *c = static_cast<int8_t>(rint(*c * (from / s)));
+    // what the page holds, four codes at once: of a row of keys, or of a value's tokens
+    const double by = static_cast<double>(before) / s;
+    uint32_t* words = reinterpret_cast<uint32_t*>(codes);
+    const int row = which ? a.block / 4 : w.held * D / 4, used = which ? (w.held + 3) / 4 : row;
+    for (int i = threadIdx.x; i < (which ? D : 1) * used; i += kAppendThreads) {
+      const int r = i / used, at = i - r * used;
+      const uint32_t old = words[r * row + at];
+      uint32_t now = old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (which && 4 * at + e >= w.held) continue;
+        const int c = static_cast<int8_t>(old >> (8 * e));
+        const uint32_t q = static_cast<uint8_t>(static_cast<int8_t>(rint(c * by)));
+        now = (now & ~(0xffu << (8 * e))) | q << (8 * e);
+      }
+      if (now != old) words[r * row + at] = now;
     }
+    __syncthreads();  // (a word may hold rows of both kinds)
   }
   const float rs = s > 0.0f ? 1.0f / s : 0.0f;
+  const int pitch = a.block + 4;
   for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    const int r = i / a.D, d = i - r * a.D;
-    const int q = quantised(to_f32(x[r * a.xs[which][1] + d]), s, rs);
-    codes[which ? d * a.block + w.held + r : (w.held + r) * a.D + d] = static_cast<int8_t>(q);
+    const int r = i / per, d = (i - r * per) * VEC;
+    const Chunk<T, VEC> c = *reinterpret_cast<const Chunk<T, VEC>*>(x + r * xt + d);
+    Chunk<int8_t, VEC> q;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) q.v[e] = static_cast<int8_t>(quantised(to_f32(c.v[e]), s, rs));
+    if (which) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) turned[(d + e) * pitch + w.held + r] = static_cast<uint8_t>(q.v[e]);
+    } else {
+      *reinterpret_cast<Chunk<int8_t, VEC>*>(codes + (w.held + r) * D + d) = q;
+    }
+  }
+  if (!which) return;
+  __syncthreads();
+  const int first = w.held / 16, groups = (w.held + w.rows + 15) / 16 - first;
+  for (int i = threadIdx.x; i < D * groups; i += kAppendThreads) {
+    const int d = i / groups, t = 16 * (first + i - d * groups);
+    const uint8_t* from = turned + d * pitch + t;
+    int8_t* to = codes + d * a.block + t;
+    if (t >= w.held && t + 16 <= w.held + w.rows) {
+      uint32_t v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = reinterpret_cast<const uint32_t*>(from)[e];
+      *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+      for (int e = 0; e < 16; ++e)
+        if (t + e >= w.held && t + e < w.held + w.rows) to[e] = static_cast<int8_t>(from[e]);
+    }
+  }
+}
+
+// What the codes of a cache stand for: codes in, four times their bytes out.  A
+// wave takes 256 codes of one page and head at a time (pages hold a multiple
+// of that), so the scale is one value a wave, and stores whole lines.
+constexpr int kValuesEach = 4;  // rounds of a block
+__global__ void __launch_bounds__(256) cache_values_kernel(const int8_t* k, const int8_t* v, const float* ks,
+                                                           const float* vs, float* out_k, float* out_v, int64_t waves,
+                                                           int64_t waves_a_page) {
+  const int lane = threadIdx.x % 64;
+  const int8_t* codes = blockIdx.y ? v : k;
+  const float* scales = blockIdx.y ? vs : ks;
+  float* out = blockIdx.y ? out_v : out_k;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (4 * kValuesEach) + threadIdx.x / 64;
+  uint32_t w[kValuesEach];
+  float s[kValuesEach];
+#pragma unroll
+  for (int i = 0; i < kValuesEach; ++i) {
+    const int64_t at = first + 4 * i < waves ? first + 4 * i : waves - 1;
+    w[i] = reinterpret_cast<const uint32_t*>(codes)[at * 64 + lane];
+    s[i] = scales[at / waves_a_page];
+  }
+#pragma unroll
+  for (int i = 0; i < kValuesEach; ++i) {
+    if (first + 4 * i >= waves) continue;
+    float4 x;
+    x.x = static_cast<float>(static_cast<int8_t>(w[i])) * s[i];
+    x.y = static_cast<float>(static_cast<int8_t>(w[i] >> 8)) * s[i];
+    x.z = static_cast<float>(static_cast<int8_t>(w[i] >> 16)) * s[i];
+    x.w = static_cast<float>(static_cast<int8_t>(w[i] >> 24)) * s[i];
+    st_stream4(out + ((first + 4 * i) * 64 + lane) * 4, x);
   }
 }
 
@@ -308,14 +389,17 @@ constexpr int kLogitTile = 8192;
 
 // x = a logit, c how often its token is in the row's history:
 // c > 0: x / r where x > 0, else x r; less f c + p; then the bias, and -inf
-// where the mask has no bit.  A block takes kLogitTile tokens of a row and
-// counts the row's history among them in LDS (whole numbers: no order of the
-// atomic additions shows).
+// where the mask has no bit.  Bound by memory.  A block takes kLogitTile tokens
+// of a row and counts the row's history among them in LDS (whole numbers: no
+// order of the atomic additions shows), while four logits a lane are on
+// their way.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs a) {
-  __shared__ uint32_t count[kLogitTile];
+  __shared__ __attribute__((aligned(16))) uint32_t count[kLogitTile];
   const int64_t row = blockIdx.y, lo = static_cast<int64_t>(blockIdx.x) * kLogitTile;
   const int n = static_cast<int>(a.V - lo < kLogitTile ? a.V - lo : kLogitTile);
-  if (a.history) {
+  const bool counted = a.history != nullptr;
+  if (counted) {
     for (int i = threadIdx.x; i < n; i += kLogitThreads) count[i] = 0;
     __syncthreads();
     int64_t len = a.L;
@@ -323,25 +407,56 @@ __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs
       const int64_t l = load_index(a.lengths, a.lengths_dt, row * a.lengths_st);
       len = l < 0 ? 0 : (l < a.L ? l : a.L);
     }
-    for (int64_t i = threadIdx.x; i < len; i += kLogitThreads) {
-      const int64_t id = load_index(a.history, a.history_dt, row * a.hs + i) - lo;
-      if (id >= 0 && id < n) atomicAdd(&count[id], 1u);
+    constexpr int kIds = 4;  // in flight
+    for (int64_t i = threadIdx.x; i < len; i += kIds * kLogitThreads) {
+      int64_t id[kIds];
+#pragma unroll
+      for (int e = 0; e < kIds; ++e) {
+        const int64_t at = i + e * kLogitThreads;
+        id[e] = at < len ? load_index(a.history, a.history_dt, row * a.hs + at) - lo : -1;
+      }
+#pragma unroll
+      for (int e = 0; e < kIds; ++e)
+        if (id[e] >= 0 && id[e] < n) atomicAdd(&count[id[e]], 1u);
     }
     __syncthreads();
   }
   const float rep = a.rep ? a.rep[row * a.rep_st] : 1.0f, pres = a.pres ? a.pres[row * a.pres_st] : 0.0f;
   const float freq = a.freq ? a.freq[row * a.freq_st] : 0.0f;
-  for (int i = threadIdx.x; i < n; i += kLogitThreads) {
-    const int64_t v = lo + i;
-    float x = load_as_f32(a.x, a.x_dt, row * a.xs + v);
-    const uint32_t c = a.history ? count[i] : 0;
+  const T* x = static_cast<const T*>(a.x) + row * a.xs + lo;
+  const float* bias = a.bias ? a.bias + row * a.bias_st + lo : nullptr;
+  const int32_t* allowed = a.allowed ? a.allowed + row * a.allowed_st + lo / 32 : nullptr;
+  float* y = a.y + row * a.ys + lo;
+  auto one = [&](float v, uint32_t c, float add, bool there) {
     if (c) {
-      x = x > 0.0f ? x / rep : x * rep;
-      x = x - freq * static_cast<float>(c) - pres;
+      v = v > 0.0f ? v / rep : v * rep;
+      v = v - freq * static_cast<float>(c) - pres;
     }
-    if (a.bias) x += a.bias[row * a.bias_st + v];
-    if (a.allowed && !((a.allowed[row * a.allowed_st + (v >> 5)] >> (v & 31)) & 1)) x = -INFINITY;
-    a.y[row * a.ys + v] = x;
+    v += add;
+    return there ? v : -INFINITY;
+  };
+  for (int i = threadIdx.x * VEC; i < n; i += kLogitThreads * VEC) {
+    if (VEC > 1 && i + VEC <= n) {
+      const Chunk<T, VEC> c = *reinterpret_cast<const Chunk<T, VEC>*>(x + i);
+      Chunk<float, VEC> add = {}, out;
+      Chunk<uint32_t, VEC> often = {};
+      if (bias) add = *reinterpret_cast<const Chunk<float, VEC>*>(bias + i);
+      if (counted) often = *reinterpret_cast<const Chunk<uint32_t, VEC>*>(count + i);
+      const uint32_t bits = allowed ? static_cast<uint32_t>(allowed[i >> 5]) >> (i & 31) : 0xffffffffu;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = one(to_f32(c.v[e]), often.v[e], add.v[e], bits >> e & 1);
+        out.v[e] = bias || often.v[e] || !(bits >> e & 1) ? v : to_f32(c.v[e]);  // (-0 stays -0)
+      }
+      st_stream4(y + i, *reinterpret_cast<const float4*>(&out));
+      continue;
+    }
+    for (int e = i; e < n && e < i + VEC; ++e) {
+      const float v = to_f32(x[e]);
+      const uint32_t often = counted ? count[e] : 0;
+      const bool there = !allowed || (allowed[e >> 5] >> (e & 31) & 1);
+      y[e] = bias || often || !there ? one(v, often, bias ? bias[e] : 0.0f, there) : v;
+    }
   }
 }
 
@@ -486,11 +601,43 @@ int kk_cache_append(const kk_tensor* k_codes, const kk_tensor* k_scales, const k
   const int64_t reach = (T + c.block - 2) / c.block + 1;
   if (2 * reach > 65535) return set_error(KK_E_UNSUPPORTED, "%s: too many tokens in a call", who);
   const dim3 grid(static_cast<unsigned>(B), static_cast<unsigned>(c.heads), static_cast<unsigned>(2 * reach));
-  if (k->dtype == KK_F16)
-    KK_LAUNCH((cache_append_kernel<__half>), grid, dim3(kAppendThreads), 0, ctx().stream, a);
-  else
-    KK_LAUNCH((cache_append_kernel<float>), grid, dim3(kAppendThreads), 0, ctx().stream, a);
-  return check_launch("cache_append_kernel");
+  const size_t lds = c.D * (c.block + 4);
+  const bool wide = rows_aligned(k, 16) && rows_aligned(v, 16);
+  auto launch = [&](auto kernel) {
+    if (lds > 60000) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(kernel)));
+    KK_LAUNCH(kernel, grid, dim3(kAppendThreads), lds, ctx().stream, a);
+    return check_launch("cache_append_kernel");
+  };
+  if (k->dtype == KK_F16) return wide ? launch(cache_append_kernel<__half, true>) : launch(cache_append_kernel<__half, false>);
+  return wide ? launch(cache_append_kernel<float, true>) : launch(cache_append_kernel<float, false>);
+}
+
+int kk_cache_values(const kk_tensor* out_k, const kk_tensor* out_v, const kk_tensor* k_codes,
+                    const kk_tensor* k_scales, const kk_tensor* v_codes, const kk_tensor* v_scales) {
+  const char* who = "cache_values";
+  CacheShape c;
+  KK_TRY(check_codes(k_codes, k_scales, v_codes, v_scales, &c, who));
+  const kk_tensor *outs[2] = {out_k, out_v}, *codes[2] = {k_codes, v_codes};
+  const char* names[2] = {"out_k", "out_v"};
+  for (int i = 0; i < 2; ++i) {
+    KK_TRY(check_tensor(outs[i], names[i]));
+    if (outs[i]->dtype != KK_F32 || outs[i]->rank != 4 || !is_contiguous(outs[i]) ||
+        reinterpret_cast<uintptr_t>(outs[i]->data) % 16)
+      return set_error(KK_E_ARG, "%s: %s must be f32 of four axes in one piece, 16-byte aligned", who, names[i]);
+    for (int j = 0; j < 4; ++j)
+      if (outs[i]->shape[j] != codes[i]->shape[j])
+        return set_error(KK_E_ARG, "%s: %s must have the shape of its codes", who, names[i]);
+  }
+  KK_TRY(require_ready());
+  const int64_t waves_a_page = c.block * c.D / 256, waves = c.pages * c.heads * waves_a_page;
+  if (waves == 0) return KK_OK;
+  const int64_t blocks = ceil_div(waves, 4 * kValuesEach);
+  if (blocks > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "%s: too many pages", who);
+  KK_LAUNCH(cache_values_kernel, dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, ctx().stream,
+            static_cast<const int8_t*>(k_codes->data), static_cast<const int8_t*>(v_codes->data),
+            static_cast<const float*>(k_scales->data), static_cast<const float*>(v_scales->data),
+            static_cast<float*>(out_k->data), static_cast<float*>(out_v->data), waves, waves_a_page);
+  return check_launch("cache_values_kernel");
 }
 
 int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_tensor* history,
@@ -553,9 +700,17 @@ int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_te
   if (B * V == 0) return KK_OK;
   const int64_t tiles = ceil_div(V, kLogitTile);
   if (B > 65535 || tiles > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "%s: too many rows", who);
-  KK_LAUNCH(process_logits_kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(B)),
-            dim3(kLogitThreads), 0, ctx().stream, a);
-  return check_launch("process_logits_kernel");
+  // four logits at once where rows start so
+  const bool wide = rows_aligned(logits, 4 * dtype_size(logits->dtype)) && rows_aligned(out, 16) &&
+                    (!bias || rows_aligned(bias, 16));
+  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(B));
+  auto launch = [&](auto kernel) {
+    KK_LAUNCH(kernel, grid, dim3(kLogitThreads), 0, ctx().stream, a);
+    return check_launch("process_logits_kernel");
+  };
+  if (logits->dtype == KK_F16)
+    return wide ? launch(process_logits_kernel<__half, 4>) : launch(process_logits_kernel<__half, 1>);
+  return wide ? launch(process_logits_kernel<float, 4>) : launch(process_logits_kernel<float, 1>);
 }
 
 }  // extern "C"

@@ -610,6 +610,14 @@ def cache_append(cache, k, v, table, starts, counts=None):
               k.desc(), v.desc(), table.desc(), starts.desc(), _d(counts))
 
 
+def cache_values(cache):
+    """(keys [pages, Hk, block, D], values [pages, Hk, D, block]) of a KVCache as float32."""
+    k, v = DeviceTensor.empty(cache.k.shape, np.float32), DeviceTensor.empty(cache.v.shape, np.float32)
+    _lib.call("kk_cache_values", k.desc(), v.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
+              cache.v_scale.desc())
+    return k, v
+
+
 def cache_attention(q, cache, table, lengths, counts=None, scale=None, window=0):
     """Causal attention of q [B, T, Hq, D], the newest counts[b] (T) of the
     lengths[b] tokens of each sequence, over a KVCache; scale 1 / sqrt(D)

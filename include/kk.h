@@ -529,6 +529,10 @@ int kk_qk_norm_rotary(const kk_tensor* out_q, const kk_tensor* out_k, const kk_t
 int kk_cache_append(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
                     const kk_tensor* v_scales, const kk_tensor* k, const kk_tensor* v,
                     const kk_tensor* table, const kk_tensor* starts, const kk_tensor* counts);
+/* What the codes of such a cache stand for: out_k f32 [pages, Hk, block, D] and out_v
+ * f32 [pages, Hk, D, block], in one piece and 16-byte aligned. */
+int kk_cache_values(const kk_tensor* out_k, const kk_tensor* out_v, const kk_tensor* k_codes,
+                    const kk_tensor* k_scales, const kk_tensor* v_codes, const kk_tensor* v_scales);
 /* Attention over such a cache: q and out [B, T, Hq, D], Hq a multiple of Hk
  * (query head h reads key head h / (Hq / Hk)).  lengths[b] tokens are cached,
  * the counts[b] (NULL: T) newest of them q's own: query t is at place
