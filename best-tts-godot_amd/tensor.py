@@ -239,7 +239,7 @@ class DeviceTensor:
         return NP_TO_CODE[self.dtype]
 
     def is_contiguous(self):
-        if self.size == 0:
+        if self.strides == _contig_strides(self.shape) or self.size == 0:
             return True
         acc = 1
         for d, s in zip(reversed(self.shape), reversed(self.strides)):
