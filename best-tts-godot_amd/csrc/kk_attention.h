@@ -177,10 +177,6 @@ __device__ __forceinline__ void one_query(const QueryArgs& a, const Rows& rows, 
 // `most`, which even out what some take longer.  At most most + B chunks come of
 // that, times the key heads: the grid.  (24 sequences of up to 8000 tokens, 4 key
 // heads of 96: 54 us in chunks of 8 steps, 44 in one round of blocks.)
-constexpr int kStep = 64;
-constexpr int kLongChunk = 64;
-constexpr int kMaxChunks = 64;  // of a sequence: a wave of the block that joins them has a lane for each
-
 struct Cut {
   int64_t B;
   int heads;           // key heads
@@ -196,11 +192,6 @@ struct Unit {
   int h, chunk, chunks;
   int64_t slot;        // of the sequence's first chunk and this head; the next chunk's is `heads` later
 };
-
-__device__ __forceinline__ int64_t chunk_steps(int64_t steps, int64_t c) {
-  const int64_t most = ceil_div(steps, kMaxChunks);
-  return c < most ? most : c;
-}
 
 __device__ __forceinline__ int64_t uniform(int64_t v) {  // the same in all lanes: in scalar registers
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
@@ -223,17 +214,11 @@ __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit
   int64_t total = mine;
   for (int64_t b = 64 + lane; b < cut.B; b += 64) total += steps_of(b);
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-  int64_t c = ceil_div(total, cut.units);
-  if (c > kLongChunk && cut.most > cut.units) {
-    c = ceil_div(total, cut.most);
-    c = c < kLongChunk ? kLongChunk : c;
-  }
-  c = c < cut.least ? cut.least : c;
+  const int64_t c = chunk_size(total, cut.units, cut.most, cut.least);
   int64_t before = 0;
   for (int64_t b0 = 0; b0 < cut.B; b0 += 64) {
     const int64_t b = b0 + lane, n = b0 ? steps_of(b) : mine;
-    const int64_t each = chunk_steps(n, c);
-    const int64_t chunks = b >= cut.B ? 0 : n <= each ? 1 : ceil_div(n, each);
+    const int64_t each = chunk_steps(n, c), chunks = b >= cut.B ? 0 : chunk_count(n, c);
     int64_t upto = chunks;
     for (int off = 1; off < 64; off <<= 1) {
       const int64_t o = __shfl_up(upto, off, 64);
@@ -273,8 +258,7 @@ inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int
   if (cut->most < cut->units) cut->most = cut->units;
   cut->part = static_cast<float*>(ctx().scratch);
   cut->arrived = ctx().row_counters;
-  int64_t n = B * (most / kStep / least + 2);  // (two: a window's first step may hold tokens it does not see)
-  if (n > B + cut->most) n = B + cut->most;
+  int64_t n = grid_chunks(B, most, cut->most, least);
   if (n > slots) {
     cut->most = slots - B;
     if (cut->units > cut->most) cut->units = cut->most;

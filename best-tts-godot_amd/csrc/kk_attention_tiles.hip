@@ -11,6 +11,7 @@ constexpr int kTileThreads = 256;
 constexpr int kTileRows = 128;  // queries of a block: 32 a wave
 constexpr int kPutRows = 64;    // of them put out at a time
 constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
+constexpr int kSpread = 11;
 constexpr float kSlack = 7.0f;
 
 struct TileCut {
@@ -85,11 +86,13 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // 8-bit codes and fp16 values are exact as halves; fp32 operands are the sum of
 // two, after a power of two for each row that brings its largest to 2^14, so
 // that 22 bits are kept whatever the rows' sizes, and the product of the two
-// low halves (2^-22) is left out.  Weights of fp16 queries are rounded to fp16
+// low halves (2^-22) is left out.  Weights carry the rows' powers of two, or the
+// pages' scales, over that of the largest seen.  Weights of fp16 queries are rounded to fp16
 // (half a step of the output's type); that they are 2^8 times as large keeps 32
 // bits between the largest and fp16's smallest value.
 //
-// A state that is not finite poisons whole sums here (0 times it is NaN) where
+// A state that is not finite (or, where queries see different ones, whose size
+// is too far from another's) poisons whole sums here (0 times it is NaN) where
 // only queries that see it should be: a block that meets one marks its part, and
 // its queries are formed one by one.
 template <typename T, class Rows, int SRC, int DT, int TT>
@@ -366,7 +369,9 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       }
   };
   float m = -3.4028235e38f, l = 0.0f, keep_r = 1.0f;
-  int er = SRC == kPaged ? 27 : 0;  // values are scaled by 2^-(er - 127) (paged), 2^-(er - 141) (fp32)
+  // values are scaled by 2^-(er - 127) (paged: of the lane's query), 2^-(er - 141)
+  // (fp32: of the block); least: the smallest row's exponent
+  int er = SRC == kPaged ? 27 : 0, least = 255;
 
   auto stage = [&](int which) {
     if constexpr (SRC == kPaged) {
@@ -419,6 +424,9 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       const int up = top > er ? top : er;
       keep_r = ldexpf(1.0f, er - up);
       er = up;
+      const float low = lv[lane % TT] ? __uint_as_float(lv[lane % TT]) : INFINITY;
+      const int bottom = static_cast<int>(__float_as_uint(-wave_max_dpp(-low)) >> 23);
+      least = bottom < least ? bottom : least;
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
         const int u = key_unit(i), tk = u / (4 * DT), c = u % (4 * DT);
@@ -516,24 +524,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
     }
     __syncthreads();
     if (empty) which ^= 1;  // (the magnitudes' other half is not cleared)
-    // the values' power of two, as far as all tiles so far are: the scales' (a page
-    // without one that is finite poisons what sees it)
-    if constexpr (SRC == kPaged) {
-      const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
-      int e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
-      e1 = e1 > 254 ? 254 : e1;
-      keep_r = 1.0f;
-      if (__any(e1 > er)) {
-        for (int off = 1; off < G; off <<= 1) {
-          const int o = __shfl_xor(e1, off, 64);
-          e1 = o > e1 ? o : e1;
-        }
-        const int up = __builtin_amdgcn_readfirstlane(e1 > er ? e1 : er);
-        keep_r = ldexpf(1.0f, er - up);
-        er = up;
-      }
-    }
-    if (keep_r != 1.0f) {
+    if (SRC == kFloat && keep_r != 1.0f) {
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -542,7 +533,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
     }
     if (empty || t0 >= upto || t0 + TT <= from) continue;
     // what the lane's query sees of its tokens 32 j + 16 k + 8 hf + e: bit 16 j + 8 k + e
-    uint32_t seen = 0;
+    uint32_t seen = 0, groups = 0;  // (groups: bit g: some of tokens 16 g .. 16 g + 15)
     bool tested = t0 < all_from || t0 + TT > all_upto || by_query;
     bool poisoned = false;
     if constexpr (SRC == kPaged) {
@@ -562,6 +553,8 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       } else {
         w = query_mask(rows, a, b, qt, t0, TT, w);
       }
+#pragma unroll
+      for (int g = 0; g < G; ++g) groups |= (w >> (16 * g) & 0xffff ? 1u : 0u) << g;
       w >>= 8 * hf;
 #pragma unroll
       for (int s = 0; s < 2 * NS; ++s) seen |= (static_cast<uint32_t>(w >> (16 * s)) & 0xffu) << (8 * s);
@@ -569,19 +562,42 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
 
     float by[G], vw[G];
     if constexpr (SRC == kPaged) {
+      // the power of two above all scales that the lane's query has seen
+      const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
+      int e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
+      e1 = e1 > 254 ? 254 : e1;
+      if (__any(e1 > er)) {
+        int up = er;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int eg = __builtin_amdgcn_readlane(e1, g);
+          up = eg > up && (!tested || groups >> g & 1) ? eg : up;
+        }
+        keep_r = ldexpf(1.0f, er - up);
+        er = up;
+        if (__any(keep_r != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][e] *= keep_r;
+        }
+      }
       const float r1 = __uint_as_float(static_cast<uint32_t>(254 - er) << 23);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         by[g] = cq * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), g));
         vw[g] = r1 * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), g));
       }
-      if (poisoned) {  // a scale that is not finite, for the queries that see its tokens
+      if (tested) {  // a group that the query does not see (its scale may pass r), or one whose scale is not finite
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          const bool sees = groups >> g & 1;
+          if (!sees) vw[g] = 0.0f;
           if (!(__builtin_fabsf(vw[g]) < INFINITY)) {
             vw[g] = 0.0f;
-            if (seen >> (8 * g) & 0xff) l = NAN;
+            l = NAN;
           }
+        }
       }
     }
     {
@@ -715,6 +731,9 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   }
 
   // the sums by rows, half of them at a time, in LDS
+  // (rows of values more than 2^kSpread apart keep their bits beside each other
+  // only if all queries see the same of them)
+  if (SRC == kFloat && by_query && er - least > kSpread) bad = 0x7f800000u;
   const uint32_t none = SRC == kHalf ? bad & 0x80008000u : SRC == kFloat ? static_cast<uint32_t>(bad >= 0x7f800000u) : 0u;
   const bool marked = __syncthreads_or(none != 0);
   const int pitch = D + 4;
@@ -871,7 +890,8 @@ static bool too_many(const QueryArgs& a) {
 bool tiles_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* status) {
   if (p.pages < 1 || p.columns < 1) return false;
   const PagedRows rows{p, a.T, a.D};
-  const int64_t capacity = p.columns * p.block, seen = p.window ? p.window + a.T - 1 : capacity;
+  const int64_t capacity = p.columns * p.block;
+  const int64_t seen = p.window && p.window < capacity ? p.window + a.T - 1 : capacity;
   const int64_t tokens = seen < capacity ? seen : capacity;
   if (too_many(a)) return false;
   const int wide = rows_of_16(a.q, a.qs, dtype == KK_F16 ? 2 : 4);

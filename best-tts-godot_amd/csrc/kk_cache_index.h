@@ -56,4 +56,34 @@ KK_HD Seen seen_tokens(int64_t place, int64_t window, int64_t capacity) {
   return s;
 }
 
+// Long sequences cut into chunks over blocks (kk_attention.h).  A sequence of
+// `steps` steps has chunk_count chunks of chunk_steps each; chunk_size is the
+// size for a batch of `total` steps: `units` chunks of it, or, once those pass
+// kLongChunk steps, `most`; `least` steps at least.  At most kMaxChunks a sequence.
+constexpr int kStep = 64;        // tokens
+constexpr int kLongChunk = 64;   // steps
+constexpr int kMaxChunks = 64;   // a wave of the block that joins them has a lane for each
+KK_HD int64_t chunk_size(int64_t total, int64_t units, int64_t most, int64_t least) {
+  int64_t c = (total + units - 1) / units;
+  if (c > kLongChunk && most > units) {
+    c = (total + most - 1) / most;
+    c = c < kLongChunk ? kLongChunk : c;
+  }
+  return c < least ? least : c;
+}
+KK_HD int64_t chunk_steps(int64_t steps, int64_t c) {
+  const int64_t fewest = (steps + kMaxChunks - 1) / kMaxChunks;
+  return c < fewest ? fewest : c;
+}
+KK_HD int64_t chunk_count(int64_t steps, int64_t c) {
+  const int64_t each = chunk_steps(steps, c);
+  return steps <= each ? 1 : (steps + each - 1) / each;
+}
+// What B sequences of at most `tokens` seen tokens each come to at the most
+// (their first step may hold tokens that a window has left behind).
+KK_HD int64_t grid_chunks(int64_t B, int64_t tokens, int64_t most, int64_t least) {
+  const int64_t by_length = B * (tokens / kStep / least + 2);
+  return by_length < B + most ? by_length : B + most;
+}
+
 }  // namespace kk

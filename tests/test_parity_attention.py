@@ -1,0 +1,291 @@
+"""Attention where its kernels' ways part: sequences cut over blocks and joined,
+many queries, states and scales that are not finite for some queries only,
+batches past a wave's lanes, windows, operands of mixed sizes.
+
+Tolerances are test_parity_decode's, from the operations counted there."""
+import numpy as np
+import pytest
+
+from conftest import assert_bitexact, rng
+from oracle import decode_ops as D
+from test_parity_decode import attention_tol, on_device, pool, random_cache, within
+
+pytestmark = pytest.mark.gpu
+DTYPES = [np.float32, np.float16]
+
+
+def run_cache(kk, q, parts, table, lengths, counts=None, scale=None, window=0):
+    dev = kk.to_device
+    return kk.to_host(kk.ops.cache_attention(dev(q), on_device(kk, parts), dev(table), dev(lengths),
+                                             None if counts is None else dev(counts), scale, window))
+
+
+def check_cache(kk, out, q, parts, table, lengths, b, scale, window=0, counts=None, queries=None):
+    T, n = q.shape[1], int(lengths[b])
+    c = T if counts is None else int(counts[b])
+    k, there = D.cached(parts[0], parts[1], table[b], n)
+    v, _ = D.cached(parts[2], parts[3], table[b], n, tokens_last=True)
+
+    def seen(i):
+        place = n - c + queries[i]
+        if queries[i] >= c or place < 0:
+            return []
+        at = np.arange(max(0, place - window + 1) if window else 0, place + 1)
+        return at[there[at]]
+    queries = np.arange(T) if queries is None else queries
+    qs = q[b][queries]
+    want = D.attention(qs, k, v, seen, scale)
+    within(out[b][queries], want, attention_tol(qs, k, v, want, scale, q.dtype.type, n), f"sequence {b}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("window", [0, 70, 2 ** 62])
+def test_a_batch_past_a_waves_lanes(gpu, t, window):
+    """150 sequences, lengths from 0: the blocks' search runs over three rounds of lanes."""
+    kk = gpu
+    r = rng(150)
+    B, block, dim, longest = 150, 16, 32, 900
+    lengths = np.where(r.random(B) < 0.1, 0, (longest * r.random(B) ** 3).astype(int)).astype(np.int32)
+    lengths[[0, 64, 149]] = longest, 0, longest - 3
+    table, pages = pool(r, B, -(-longest // block))
+    parts = random_cache(r, pages, 2, block, dim)
+    q = r.normal(size=(B, 1, 6, dim)).astype(t)
+    out = run_cache(kk, q, parts, table, lengths, scale=0.2, window=window)
+    assert not out[lengths == 0].any()
+    for b in [*range(0, 8), 62, 63, 64, 65, 127, 128, 129, 148, 149]:
+        if lengths[b]:
+            check_cache(kk, out, q, parts, table, lengths, b, 0.2, min(window, 2 ** 20))
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hk,dim,block,longest,window", [
+    (1, 2, 1, 128, 64, 20011, 0), (1, 7, 1, 96, 32, 9000, 0), (1, 24, 1, 64, 16, 7001, 5000), (3, 8, 1, 64, 256, 6000, 0),
+    (2, 12, 1, 112, 64, 4100, 130), (1, 16, 2, 192, 64, 5003, 0)])
+def test_long_sequences_are_cut_and_joined(gpu, t, T, Hq, Hk, dim, block, longest, window):
+    kk = gpu
+    r = rng(longest)
+    table, pages = pool(r, 2, -(-longest // block))
+    lengths = np.array([longest, longest // 3], np.int64)
+    parts = random_cache(r, pages, Hk, block, dim)
+    q = (1.5 * r.normal(size=(2, T, Hq, dim))).astype(t)
+    out = run_cache(kk, q, parts, table, lengths, scale=0.05, window=window)
+    for b in range(2):
+        check_cache(kk, out, q, parts, table, lengths, b, 0.05, window)
+    assert_bitexact(run_cache(kk, q, parts, table, lengths, scale=0.05, window=window), out)
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hk,dim,block,longest,window", [
+    (40, 7, 1, 64, 32, 1500, 0), (33, 4, 1, 96, 16, 700, 100), (300, 2, 1, 128, 64, 1111, 0), (17, 8, 2, 80, 128, 900, 0),
+    (130, 3, 1, 256, 64, 600, 0), (700, 1, 1, 64, 64, 700, 33), (65, 2, 2, 144, 16, 333, 0)])
+def test_chunks_of_tokens_over_a_cache(gpu, t, T, Hq, Hk, dim, block, longest, window):
+    """Parts of the tokens joined where there are few queries; counts that leave queries without a place."""
+    kk = gpu
+    r = rng(T + longest)
+    table, pages = pool(r, 2, -(-longest // block))
+    lengths, counts = np.array([longest, longest - 7], np.int32), np.array([T, T - T // 3], np.int32)
+    parts = random_cache(r, pages, Hk, block, dim)
+    q = r.normal(size=(2, T, Hq, dim)).astype(t)
+    out = run_cache(kk, q, parts, table, lengths, counts, 0.1, window)
+    for b in range(2):
+        some = np.unique(np.concatenate([[0, 1, T - 1, T // 2, int(counts[b]) - 1], r.integers(0, T, 12)]))
+        check_cache(kk, out, q, parts, table, lengths, b, 0.1, window, counts, some)
+        assert not out[b, counts[b]:].any()
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,group", [(3, 2), (20, 2), (90, 1)])
+def test_scales_that_are_not_finite_stay_with_the_queries_that_see_them(gpu, t, T, group):
+    """Pages of NaN and infinite scales near the end: what comes before them does not know them."""
+    kk = gpu
+    r = rng(T)
+    block, dim, n = 16, 64, 400
+    table, pages = pool(r, 1, n // block)
+    parts = list(random_cache(r, pages, 2, block, dim))
+    first = n - T + T // 3  # the first poisoned token: its page's rows before it are poisoned too
+    page = first // block
+    parts[1 if T == 20 else 3][table[0, page]] = np.nan if T != 90 else np.inf
+    q = r.normal(size=(1, T, 2 * group, dim)).astype(t)
+    out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=0.1)
+    place = n - T + np.arange(T)
+    clean = np.flatnonzero(place < page * block)
+    if clean.size:
+        clean_parts = [np.nan_to_num(x, nan=0.0, posinf=0.0) if x.dtype == np.float32 else x for x in parts]
+        check_cache(kk, out, q, clean_parts, table, [n], 0, 0.1, queries=clean)
+    assert not np.isfinite(out[0][place >= (page + 1) * block - 1]).any()
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,Hq,S", [(1, 4, 300), (5, 1, 300), (40, 2, 300), (200, 3, 200), (40, 2, 2000)])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_states_that_are_not_finite_stay_with_the_queries_that_see_them(gpu, t, T, Hq, S, what):
+    kk = gpu
+    r = rng(S)
+    k, v = (r.normal(size=(1, S, 1, 64)).astype(t) for _ in range(2))
+    q = r.normal(size=(1, T, Hq, 64)).astype(t)
+    mask = r.random((1, T, S)) < 0.8
+    bad = S - 31
+    mask[0, :, bad] = np.arange(T) % 3 == 1
+    clean_k, clean_v = k.copy(), v.copy()
+    (k if what != what else v)[0, bad, 0, 5] = what
+    dev = kk.to_device
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), mask=dev(mask), scale=0.1))
+    rows = np.flatnonzero(~mask[0, :, bad])
+    want = D.attention(q[0][rows], clean_k[0], clean_v[0], lambda i: np.flatnonzero(mask[0, rows[i]]), 0.1)
+    within(out[0][rows], want, attention_tol(q[0], clean_k[0], clean_v[0], want, 0.1, t, S))
+    for i in np.flatnonzero(mask[0, :, bad]):
+        assert not np.isfinite(out[0, i, :, 5]).any()
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,S,Hq,Hk,dim,axes", [
+    (1, 5000, 8, 1, 128, 2), (2, 999, 4, 1, 80, 0), (1, 3001, 5, 5, 64, 2), (4, 2000, 2, 1, 256, 0), (8, 700, 1, 1, 48, 2),
+    (9, 3000, 3, 1, 128, 2), (60, 2500, 2, 1, 96, 3), (260, 300, 2, 2, 160, 0), (500, 130, 12, 12, 64, 2), (33, 1000, 1, 1, 200, 3),
+    (150, 257, 1, 1, 8, 0), (20, 90, 1, 1, 7, 3)])
+def test_cross_attention_of_every_way(gpu, t, T, S, Hq, Hk, dim, axes):
+    """Few and many queries, long and short states, tokens shared by blocks, heads past 128 values and of odd sizes."""
+    kk = gpu
+    r = rng(T + S)
+    q = (1.5 * r.normal(size=(2, T, Hq, dim))).astype(t)
+    k, v = (r.normal(size=(2, S, Hk, dim)).astype(t) for _ in range(2))
+    lengths = np.array([S, S - S // 3], np.int64)
+    mask = np.ones((2, T, S), bool)
+    if axes == 2:
+        mask &= (r.random((2, 1, S)) < 0.6)
+        mask[:, :, S // 4:S // 4 + 130] = False  # whole tiles that nobody sees
+    if axes == 3:
+        mask &= r.random((2, T, S)) < 0.6
+        mask[1, T // 2] = False
+    dev = kk.to_device
+    m = None if not axes else dev(mask[:, 0] if axes == 2 else mask)
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), dev(lengths), m, 0.1))
+    for b in range(2):
+        some = np.unique(np.concatenate([[0, T - 1, T // 2], r.integers(0, T, 10)]))
+
+        def seen(i):
+            return np.flatnonzero(mask[b, some[i]] & (np.arange(S) < lengths[b]))
+        want = D.attention(q[b][some], k[b], v[b], seen, 0.1)
+        within(out[b][some], want, attention_tol(q[b][some], k[b], v[b], want, 0.1, t, S), f"sequence {b}")
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_states_of_mixed_sizes(gpu, T):
+    """Rows of keys and values, and queries, from 1e-12 to 1e12 next to each other: each keeps its own bits."""
+    kk = gpu
+    r = rng(40)
+    S, size = 200, 10.0 ** np.linspace(-12, 12, 200)
+    v = (size[None, :, None, None] * r.normal(size=(1, S, 1, 64))).astype(np.float32)
+    k = (r.permutation(size)[None, :, None, None] * r.normal(size=(1, S, 1, 64))).astype(np.float32)
+    q = (1e-12 * r.normal(size=(1, T, 2, 64))).astype(np.float32)
+    dev = kk.to_device
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), scale=0.3))
+    want = D.attention(q[0], k[0], v[0], lambda i: np.arange(S), 0.3)
+    within(out[0], want, attention_tol(q[0], k[0], v[0], want, 0.3, np.float32, S))
+    # a query that sees the smallest alone gets it to the last bits
+    mask = np.zeros((1, S), bool)
+    mask[0, 0] = True
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), mask=dev(mask), scale=0.3))
+    want = np.broadcast_to(v[0, 0].astype(np.float64), out[0].shape)
+    within(out[0], want, (8 + 8) * 2.0 ** -24 * np.abs(want).max())
+
+
+def test_masks_by_query_over_states_of_mixed_sizes(gpu):
+    """Query i sees the i + 1 smallest of states that grow from 1e-12 to 1e12: to its own last bits."""
+    kk = gpu
+    r = rng(44)
+    T = S = 90
+    size = 10.0 ** np.linspace(-12, 12, S)
+    v = (size[None, :, None, None] * r.normal(size=(1, S, 1, 64))).astype(np.float32)
+    k, q = r.normal(size=(1, S, 1, 64)).astype(np.float32), r.normal(size=(1, T, 2, 64)).astype(np.float32)
+    mask = np.tril(np.ones((1, T, S), bool))
+    dev = kk.to_device
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), mask=dev(mask), scale=0.1))
+    want = D.attention(q[0], k[0], v[0], lambda i: np.arange(i + 1), 0.1)
+    for i in range(T):
+        within(out[0, i], want[i], attention_tol(q[0, i:i + 1], k[0, :i + 1], v[0, :i + 1], want[i], 0.1, np.float32, S), f"query {i}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T", [1, 50])
+def test_cache_pages_of_mixed_scales(gpu, t, T):
+    """Pages whose scales lie 1e25 apart, one of zeros: the smallest, seen alone, keeps its bits."""
+    kk = gpu
+    r = rng(41)
+    block, dim, n = 16, 64, 160
+    table, pages = pool(r, 1, n // block)
+    parts = list(random_cache(r, pages, 1, block, dim))
+    parts[1][:] = 0.01
+    parts[3][table[0], 0] = (10.0 ** np.linspace(-25, 0, n // block)).astype(np.float32)
+    parts[3][table[0, 4], 0] = 0
+    q = r.normal(size=(1, T, 2, dim)).astype(t)
+    for length in (T, n):
+        out = run_cache(kk, q, parts, table, np.array([length], np.int32), scale=0.1)
+        v, _ = D.cached(parts[2], parts[3], table[0], length, tokens_last=True)
+        check_cache(kk, out, q, parts, table, [length], 0, 0.1)
+        if length == T and t == np.float32:  # one token alone is itself
+            within(out[0, 0], np.broadcast_to(v[0], out[0, 0].shape), 16 * 2.0 ** -24 * np.abs(v[0]).max())
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scores_that_rise_all_the_way(gpu, t, T, scale):
+    """Each token's score above the last one's, so that the maximum moves with every tile; a scale of 0 and below."""
+    kk = gpu
+    r = rng(42)
+    S = 600
+    k = (np.linspace(-40, 40, S)[None, :, None, None] * np.ones((1, S, 1, 64)) / 8).astype(t)
+    v = r.normal(size=(1, S, 1, 64)).astype(t)
+    q = np.abs(r.normal(size=(1, T, 2, 64))).astype(t)
+    dev = kk.to_device
+    for s in (scale, -scale):
+        out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), scale=s))
+        want = D.attention(q[0], k[0], v[0], lambda i: np.arange(S), s)
+        within(out[0], want, attention_tol(q[0], k[0], v[0], want, s, t, S))
+
+
+def test_empty_pools_and_tables(gpu):
+    kk = gpu
+    q = kk.to_device(np.ones((2, 1, 2, 64), np.float32))
+    zero = kk.to_device(np.full(2, 3, np.int32))
+    for pages, columns in ((0, 2), (3, 0)):
+        cache = kk.KVCache.zeros(pages, 1, 64, 16)
+        table = kk.DeviceTensor.empty((2, columns), np.int32)
+        if columns:
+            table = kk.to_device(np.zeros((2, columns), np.int32))
+        for x in (q, kk.to_device(np.ones((2, 50, 2, 64), np.float32))):
+            assert not kk.to_host(kk.ops.cache_attention(x, cache, table, zero)).any()
+        k, v = cache.values()
+        assert k.shape == (pages, 1, 16, 64) and v.shape == (pages, 1, 64, 16)
+
+
+def test_shared_tokens_replay(gpu):
+    """Calls that cut their tokens, one after the other through the same scratch memory, recorded and replayed."""
+    import ctypes
+    kk = gpu
+    r = rng(43)
+    dev = kk.to_device
+    k, v = (dev(r.normal(size=(1, 3000, 2, 64)).astype(np.float32)) for _ in range(2))
+    q1, q2 = (dev(r.normal(size=(1, T, 2, 64)).astype(np.float32)) for T in (1, 70))
+    o1, o2 = kk.DeviceTensor.empty(q1.shape), kk.DeviceTensor.empty(q2.shape)
+
+    def both():
+        kk._lib.call("kk_cross_attention", o1.desc(), q1.desc(), k.desc(), v.desc(), None, None, 0.1)
+        kk._lib.call("kk_cross_attention", o2.desc(), q2.desc(), k.desc(), v.desc(), None, None, 0.1)
+    both()
+    kk.sync()
+    kk._lib.call("kk_graph_begin")
+    both()
+    g = ctypes.c_int(-1)
+    kk._lib.call("kk_graph_end", ctypes.byref(g))
+    for i in range(6):
+        for t in (q1, q2):
+            kk.ops.copy_into(t, dev(r.normal(size=t.shape).astype(np.float32)))
+        both()
+        eager = [kk.to_host(o1), kk.to_host(o2)]
+        for t in (o1, o2):
+            kk.ops.copy_into(t, kk.ops.fill(t.shape, float("nan")))
+        kk._lib.call("kk_graph_launch", g.value)
+        assert_bitexact(kk.to_host(o1), eager[0], f"replay {i}")
+        assert_bitexact(kk.to_host(o2), eager[1], f"replay {i}")
+    kk._lib.call("kk_graph_destroy", g.value)
