@@ -62,7 +62,10 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
     for (int s = 0; s < 2 * KH; ++s) {
       const int d = 64 * (s / 2) + 16 * g + 8 * (s % 2);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[s][i] = d < D ? q[d + i] : T(0.0f);
+      for (int i = 0; i < 8; ++i) {
+        const T v = q[(d < D ? d : 0) + i];
+        x[s][i] = d < D ? v : T(0.0f);
+      }
     }
     cq[nt] = a.scale;
     if constexpr (P == 1) {

@@ -18,7 +18,6 @@ struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
   int tiles;           // of kTileRows queries in a sequence and key head
   int64_t rows;        // queries of a sequence and key head: T * group
-  int wide;            // rows of q, k and v take 16-byte accesses
   // of each tile of queries, where splits > 1: the parts that it has, and those
   // parts' sums [kTileRows][D], maxima and sums of powers [kTileRows]
   int* parts;
@@ -95,8 +94,8 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // is too far from another's) poisons whole sums here (0 times it is NaN) where
 // only queries that see it should be: a block that meets one marks its part, and
 // its queries are formed one by one.
-template <typename T, class Rows, int SRC, int DT, int TT>
-__global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeof(T) == 4 ? 3 : 4) ? 2 : 1)
+template <typename T, class Rows, int SRC, int DT, int TT, bool WIDE>
+__global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2 : sizeof(T) == 4 ? 3 : 4) ? 2 : 1)
     attention_tile_kernel(QueryArgs a, Rows rows, TileCut cut) {
   constexpr int PQ = sizeof(T) == 4 ? 2 : 1, PK = SRC == kFloat ? 2 : 1, PW = PQ;
   constexpr int KS = 2 * DT, NS = TT / 32, G = TT / 16;
@@ -147,50 +146,56 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   h8 qf[KS][PQ];
   {
     const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + qt * a.qs[1] + qhead * a.qs[2];
-    T x[KS][8];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = 16 * s + 8 * hf;
-      if (cut.wide && d < D) {
-        if constexpr (PQ == 1) {
-          const h8 v = *reinterpret_cast<const h8*>(q + d);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[s][i] = __builtin_bit_cast(__half, static_cast<_Float16>(v[i]));
-        } else {
-          const f4 v0 = *reinterpret_cast<const f4*>(q + d), v1 = *reinterpret_cast<const f4*>(q + d + 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[s][i] = v0[i];
-            x[s][i + 4] = v1[i];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[s][i] = d + i < D ? q[d + i] : T(0.0f);
-      }
-    }
     if constexpr (PQ == 1) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * hf;
+        if constexpr (WIDE) {
+          const u4 v = *reinterpret_cast<const u4*>(q + (d < D ? d : 0));
+          qf[s][0] = __builtin_bit_cast(h8, d < D ? v : u4{0, 0, 0, 0});
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) qf[s][0][i] = __builtin_bit_cast(_Float16, x[s][i]);
+          for (int i = 0; i < 8; ++i) {
+            const T v = q[d + i < D ? d + i : 0];
+            qf[s][0][i] = d + i < D ? __builtin_bit_cast(_Float16, v) : static_cast<_Float16>(0.0f);
+          }
+        }
+      }
     } else {
-      float top = 0.0f;
+      float x[KS][8], top = 0.0f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * hf;
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const f4 v = *reinterpret_cast<const f4*>(q + (d < D ? d : 0) + 4 * w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[s][4 * w + i] = d < D ? v[i] : 0.0f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float v = to_f32(q[d + i < D ? d + i : 0]);
+            x[s][i] = d + i < D ? v : 0.0f;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(x[s][i]));
+      }
       top = max_halves(top);
       const int up = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
       cq = ldexpf(a.scale, -up);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = ldexpf(x[s][i], up);
-          const _Float16 y0 = static_cast<_Float16>(y);
-          qf[s][0][i] = y0;
-          qf[s][PQ - 1][i] = static_cast<_Float16>(y - static_cast<float>(y0));
+        for (int i = 0; i < 8; i += 2) {
+          h2 y0, y1;
+          split2(ldexpf(x[s][i], up), ldexpf(x[s][i + 1], up), &y0, &y1);
+          qf[s][0][i] = y0[0];
+          qf[s][0][i + 1] = y0[1];
+          qf[s][PQ - 1][i] = y1[0];
+          qf[s][PQ - 1][i + 1] = y1[1];
         }
     }
   }
@@ -220,17 +225,24 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
   auto value_d = [&](int u) { return kVD * (u % (32 / kVD) + 32 / kVD * (u / (32 / kVD * (TT / 4)))); };
   auto value_tokens = [&](int u) { return u / (32 / kVD) % (TT / 4) * 4; };
 
-  // paged: the table's entry and, with its codes, the scales of 16 tokens, of
-  // group lane % G
+  // paged: the table's entry (a tile before its codes) and, with its codes, the
+  // scales of 16 tokens, of group lane % G
   int entry = 0, page1 = -1;
   float ks1 = 0.0f, vs1 = 0.0f;
   // dense: bit j: any of the block's queries may see token j
   uint64_t word = 0;
+  bool sees1 = false;  // whether token `lane` of the tile after may be seen
 
   auto find_entry = [&](int64_t t0) {
     if constexpr (SRC == kPaged) {
       const int64_t column = (t0 + 16 * (lane % G)) >> __builtin_ctz(rows.a.block);
       entry = rows.a.table[b * rows.a.table_stride + (column < rows.a.columns ? column : rows.a.columns - 1)];
+    } else {
+      const auto& p = rows.a;
+      const int64_t t = t0 + lane;
+      sees1 = t < hi && lane < TT;
+      if (p.mask && (p.ms[1] == 0 || a.T == 1))  // (past the end: the last, without effect)
+        sees1 = (p.mask[b * p.ms[0] + (t < p.S ? t : p.S - 1) * p.ms[2]] != 0) & sees1;
     }
   };
   auto fetch = [&](int64_t t0) {
@@ -276,9 +288,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
     } else {
       using S = std::conditional_t<SRC == kHalf, __half, float>;
       const auto& p = rows.a;
-      bool sees = t0 + lane < hi && lane < TT;
-      if (sees && p.mask && (p.ms[1] == 0 || a.T == 1)) sees = p.mask[b * p.ms[0] + (t0 + lane) * p.ms[2]] != 0;
-      word = __ballot(sees);
+      word = __ballot(sees1);
       if (word == 0) return;
       // a token that no query of the block may see is not read: in its place,
       // without weight, the first that some do
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(kTileThreads, DT <= (SRC == kFloat ? 2 : sizeo
       const S* k = static_cast<const S*>(p.k) + b * p.ks[0] + h * p.ks[2] + t0 * p.ks[1];
       const S* v = static_cast<const S*>(p.v) + b * p.vs[0] + h * p.vs[2] + t0 * p.vs[1];
       constexpr int W = SRC == kFloat ? 2 : 1;
-      if (cut.wide) {
+      if constexpr (WIDE) {
 #pragma unroll
         for (int i = 0; i < UK; ++i) {
           const int u = key_unit(i), tk = u / (4 * DT), d = 8 * (u % (4 * DT));
@@ -838,13 +848,12 @@ __global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, R
   }
 }
 
-template <typename T, class Rows, int SRC, int DT, int TT>
-static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, int wide, const char* who) {
+template <typename T, class Rows, int SRC, int DT, int TT, bool WIDE>
+static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, const char* who) {
   const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * (a.heads / a.group);
   const int64_t tiles = ceil_div(queries, kTileRows);
   TileCut cut{};
   cut.rows = queries;
-  cut.wide = wide;
   // where there are fewer blocks than two a CU, the tokens are cut, into parts
   // of two tiles at least
   const int64_t blocks = pairs * tiles, head = (blocks * 4 + 15) / 16 * 16;
@@ -864,8 +873,8 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
   int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows) * 4;
   if (bytes < tile_bytes(SRC, DT, TT)) bytes = tile_bytes(SRC, DT, TT);
   if (bytes < 4 * kMaxHead * 4) bytes = 4 * kMaxHead * 4;
-  if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(attention_tile_kernel<T, Rows, SRC, DT, TT>)));
-  KK_LAUNCH((attention_tile_kernel<T, Rows, SRC, DT, TT>), grid, dim3(kTileThreads), static_cast<unsigned>(bytes),
+  if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(attention_tile_kernel<T, Rows, SRC, DT, TT, WIDE>)));
+  KK_LAUNCH((attention_tile_kernel<T, Rows, SRC, DT, TT, WIDE>), grid, dim3(kTileThreads), static_cast<unsigned>(bytes),
             ctx().stream, a, rows, cut);
   KK_TRY(check_launch("attention_tile_kernel"));
   if (splits == 1) return KK_OK;
@@ -874,12 +883,19 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, in
   return check_launch("join_parts_kernel");
 }
 
+// WIDE: rows of q, and of dense keys and values, take 16-byte accesses.
+template <typename T, class Rows, int SRC, bool WIDE>
+static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, const char* who) {
+  return a.D <= 64    ? launch_tiles<T, Rows, SRC, 2, 64, WIDE>(a, rows, tokens, who)
+         : a.D <= 96  ? launch_tiles<T, Rows, SRC, 3, 64, WIDE>(a, rows, tokens, who)
+         : a.D <= 128 ? launch_tiles<T, Rows, SRC, 4, 64, WIDE>(a, rows, tokens, who)
+                      : launch_tiles<T, Rows, SRC, 8, 32, WIDE>(a, rows, tokens, who);
+}
+
 template <typename T, class Rows, int SRC>
-static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, int wide, const char* who) {
-  return a.D <= 64    ? launch_tiles<T, Rows, SRC, 2, 64>(a, rows, tokens, wide, who)
-         : a.D <= 96  ? launch_tiles<T, Rows, SRC, 3, 64>(a, rows, tokens, wide, who)
-         : a.D <= 128 ? launch_tiles<T, Rows, SRC, 4, 64>(a, rows, tokens, wide, who)
-                      : launch_tiles<T, Rows, SRC, 8, 32>(a, rows, tokens, wide, who);
+static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, bool wide, const char* who) {
+  return wide ? launch_tiles<T, Rows, SRC, true>(a, rows, tokens, who)
+              : launch_tiles<T, Rows, SRC, false>(a, rows, tokens, who);
 }
 
 // (past the grid's axes: one query a wave)
@@ -894,7 +910,7 @@ bool tiles_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* sta
   const int64_t seen = p.window && p.window < capacity ? p.window + a.T - 1 : capacity;
   const int64_t tokens = seen < capacity ? seen : capacity;
   if (too_many(a)) return false;
-  const int wide = rows_of_16(a.q, a.qs, dtype == KK_F16 ? 2 : 4);
+  const bool wide = rows_of_16(a.q, a.qs, dtype == KK_F16 ? 2 : 4);
   const char* who = "cache_attention";
   *status = dtype == KK_F16 ? launch_tiles<__half, PagedRows, kPaged>(a, rows, tokens, wide, who)
                             : launch_tiles<float, PagedRows, kPaged>(a, rows, tokens, wide, who);
@@ -904,7 +920,7 @@ bool tiles_paged_try(const QueryArgs& a, const PagedArgs& p, int dtype, int* sta
 bool tiles_dense_try(const QueryArgs& a, const DenseArgs& d, int dtype, int* status) {
   if (d.S < 1 || too_many(a)) return false;
   const int size = dtype == KK_F16 ? 2 : 4;
-  const int wide = a.D % 8 == 0 && d.ks[3] == 1 && d.vs[3] == 1 && rows_of_16(a.q, a.qs, size) &&
+  const bool wide = a.D % 8 == 0 && d.ks[3] == 1 && d.vs[3] == 1 && rows_of_16(a.q, a.qs, size) &&
                    rows_of_16(d.k, d.ks, size) && rows_of_16(d.v, d.vs, size);
   const char* who = "cross_attention";
   *status = dtype == KK_F16

@@ -572,6 +572,9 @@ def fir_pcm16(x, taps, center=-1, gain=1.0):
 
 
 # ------------------------------------------------------------ token decoder
+_F32 = np.dtype(np.float32)
+
+
 # (a copy that _inner or _flat makes must be held until the call: its buffer goes back to the pool with it)
 def _inner(t):
     """t with its last axis in one piece."""
@@ -590,8 +593,8 @@ def qk_norm_rotary(q, k, positions=None, turns=None, q_weight=None, k_weight=Non
     [B, T]."""
     q, k, turns = _inner(q), _inner(k), _flat(turns)
     q_weight, k_weight = _flat(q_weight), _flat(k_weight)
-    out_q = DeviceTensor.empty(q.shape, q.dtype)
-    out_k = None if k is None else DeviceTensor.empty(k.shape, k.dtype)
+    out_q = DeviceTensor._fresh(q.shape, q.dtype)
+    out_k = None if k is None else DeviceTensor._fresh(k.shape, k.dtype)
     _lib.call("kk_qk_norm_rotary", out_q.desc(), _d(out_k), q.desc(), _d(k), _d(q_weight), _d(k_weight),
               _d(positions), _d(turns), float(eps), int(bool(interleaved)), float(amplitude))
     return out_q, out_k
@@ -612,7 +615,7 @@ def cache_append(cache, k, v, table, starts, counts=None):
 
 def cache_values(cache):
     """(keys [pages, Hk, block, D], values [pages, Hk, D, block]) of a KVCache as float32."""
-    k, v = DeviceTensor.empty(cache.k.shape, np.float32), DeviceTensor.empty(cache.v.shape, np.float32)
+    k, v = DeviceTensor._fresh(cache.k.shape, _F32), DeviceTensor._fresh(cache.v.shape, _F32)
     _lib.call("kk_cache_values", k.desc(), v.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
               cache.v_scale.desc())
     return k, v
@@ -623,7 +626,7 @@ def cache_attention(q, cache, table, lengths, counts=None, scale=None, window=0)
     lengths[b] tokens of each sequence, over a KVCache; scale 1 / sqrt(D)
     where None, window 0 for all tokens."""
     q, table = _inner(q), _inner(table)
-    out = DeviceTensor.empty(q.shape, q.dtype)
+    out = DeviceTensor._fresh(q.shape, q.dtype)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     _lib.call("kk_cache_attention", out.desc(), q.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
               cache.v_scale.desc(), table.desc(), lengths.desc(), _d(counts), scale, int(window))
@@ -635,7 +638,7 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     [B, S, Hk, D]: those below lengths[b] whose mask (bool [B, S] or
     [B, T, S]) is set; scale 1 / sqrt(D) where None."""
     q, k, v = _inner(q), _inner(k), _inner(v)
-    out = DeviceTensor.empty(q.shape, q.dtype)
+    out = DeviceTensor._fresh(q.shape, q.dtype)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     _lib.call("kk_cross_attention", out.desc(), q.desc(), k.desc(), v.desc(), _d(lengths), _d(mask), scale)
     return out
@@ -647,7 +650,7 @@ def process_logits(logits, history=None, history_lengths=None, repetition=None, 
     [V] or [B, V] and the grammar's mask (bits of int32 words; allowed_bits),
     as float32."""
     logits, history, bias, allowed = _inner(logits), _inner(history), _inner(bias), _inner(allowed)
-    out = DeviceTensor.empty(logits.shape, np.float32)
+    out = DeviceTensor._fresh(logits.shape, _F32)
     _lib.call("kk_process_logits", out.desc(), logits.desc(), _d(history), _d(history_lengths), _d(repetition),
               _d(presence), _d(frequency), _d(bias), _d(allowed))
     return out

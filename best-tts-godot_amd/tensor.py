@@ -80,7 +80,6 @@ class Storage:
         alloc = _fast.get("kk_alloc")
         if alloc is None:
             alloc = _fast["kk_alloc"] = _lib.load().kk_alloc
-        nbytes = int(nbytes)
         rc = alloc(nbytes if nbytes > 0 else 1, _alloc_ref)
         if rc:
             _lib.raise_error("kk_alloc", rc)
@@ -121,6 +120,7 @@ def signal_stream(stream=0):
 
 
 _PROTOS = {}  # (shape, strides, dtype) -> KKTensor with data unset
+_INTERFACES = {}  # (shape, strides, dtype) -> array interface but for the address
 
 
 @functools.lru_cache(maxsize=4096)
@@ -160,6 +160,11 @@ class DeviceTensor:
             raise TypeError(f"unsupported device dtype {dtype}")
         if len(shape) > _lib.KK_MAX_RANK:
             raise ValueError(f"rank {len(shape)} exceeds {_lib.KK_MAX_RANK}")
+        return cls._fresh(shape, dtype)
+
+    @classmethod
+    def _fresh(cls, shape, dtype):
+        """empty() of another tensor's shape (a tuple of int) and dtype."""
         t = object.__new__(cls)  # a fresh contiguous tensor: no view checks
         t.storage = Storage(math.prod(shape) * dtype.itemsize)
         t.shape = shape
@@ -217,9 +222,15 @@ class DeviceTensor:
         """This tensor's memory for another library (torch.as_tensor(t,
         device="cuda") makes a view that keeps it alive).  Not synchronised:
         call sync(), or signal_stream() with the stream that reads it."""
-        item = self.dtype.itemsize
-        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr if self.size else 0, False),
-                "strides": None if self.is_contiguous() else tuple(st * item for st in self.strides), "version": 2}
+        key = (self.shape, self.strides, self.dtype)
+        fixed = _INTERFACES.get(key)
+        if fixed is None:
+            item = self.dtype.itemsize
+            fixed = {"shape": self.shape, "typestr": self.dtype.str, "version": 2, "strides":
+                     None if self.is_contiguous() else tuple(st * item for st in self.strides)}
+            if len(_INTERFACES) < 4096:
+                _INTERFACES[key] = fixed
+        return dict(fixed, data=(self.storage.ptr + self.offset * self.dtype.itemsize if 0 not in self.shape else 0, False))
 
     # ------------------------------------------------------------ queries
     @property
