@@ -402,8 +402,9 @@ constexpr int kLogitTile = 8192;
 // of a row and counts the row's history among them in LDS (whole numbers: no
 // order of the atomic additions shows), while four logits a lane are on
 // their way.
-template <typename T, int VEC>
+template <typename T>
 __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs a) {
+  constexpr int VEC = 4;
   __shared__ __attribute__((aligned(16))) uint32_t count[kLogitTile];
   const int64_t row = blockIdx.y, lo = static_cast<int64_t>(blockIdx.x) * kLogitTile;
   const int n = static_cast<int>(a.V - lo < kLogitTile ? a.V - lo : kLogitTile);
@@ -445,19 +446,21 @@ __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs
     return there ? v : -INFINITY;
   };
   for (int i = threadIdx.x * VEC; i < n; i += kLogitThreads * VEC) {
-    if (VEC > 1 && i + VEC <= n) {
-      const Chunk<T, VEC> c = *reinterpret_cast<const Chunk<T, VEC>*>(x + i);
-      Chunk<float, VEC> add = {}, out;
+    if (i + VEC <= n) {
+      Chunk<T, VEC> c;  // (rows start anywhere)
+      Chunk<float, VEC> add = {};
       Chunk<uint32_t, VEC> often = {};
-      if (bias) add = *reinterpret_cast<const Chunk<float, VEC>*>(bias + i);
+      kk_f4u out;
+      __builtin_memcpy(&c, x + i, sizeof c);
+      if (bias) __builtin_memcpy(&add, bias + i, sizeof add);
       if (counted) often = *reinterpret_cast<const Chunk<uint32_t, VEC>*>(count + i);
       const uint32_t bits = allowed ? static_cast<uint32_t>(allowed[i >> 5]) >> (i & 31) : 0xffffffffu;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float v = one(to_f32(c.v[e]), often.v[e], add.v[e], bits >> e & 1);
-        out.v[e] = bias || often.v[e] || !(bits >> e & 1) ? v : to_f32(c.v[e]);  // (-0 stays -0)
+        out[e] = bias || often.v[e] || !(bits >> e & 1) ? v : to_f32(c.v[e]);  // (-0 stays -0)
       }
-      st_stream4(y + i, *reinterpret_cast<const float4*>(&out));
+      __builtin_nontemporal_store(out, reinterpret_cast<kk_f4u*>(y + i));
       continue;
     }
     for (int e = i; e < n && e < i + VEC; ++e) {
@@ -716,17 +719,12 @@ int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_te
   if (B * V == 0) return KK_OK;
   const int64_t tiles = ceil_div(V, kLogitTile);
   if (B > 65535 || tiles > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "%s: too many rows", who);
-  // four logits at once where rows start so
-  const bool wide = rows_aligned(logits, 4 * dtype_size(logits->dtype)) && rows_aligned(out, 16) &&
-                    (!bias || rows_aligned(bias, 16));
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(B));
-  auto launch = [&](auto kernel) {
-    KK_LAUNCH(kernel, grid, dim3(kLogitThreads), 0, ctx().stream, a);
-    return check_launch("process_logits_kernel");
-  };
   if (logits->dtype == KK_F16)
-    return wide ? launch(process_logits_kernel<__half, 4>) : launch(process_logits_kernel<__half, 1>);
-  return wide ? launch(process_logits_kernel<float, 4>) : launch(process_logits_kernel<float, 1>);
+    KK_LAUNCH((process_logits_kernel<__half>), grid, dim3(kLogitThreads), 0, ctx().stream, a);
+  else
+    KK_LAUNCH((process_logits_kernel<float>), grid, dim3(kLogitThreads), 0, ctx().stream, a);
+  return check_launch("process_logits_kernel");
 }
 
 }  // extern "C"
