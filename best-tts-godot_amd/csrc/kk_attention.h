@@ -172,15 +172,16 @@ __device__ __forceinline__ void one_query(const QueryArgs& a, const Rows& rows, 
 // so that every CU has some.  How long they are is known on the device only,
 // so the blocks find their chunk there: with n_b steps of kStep tokens in
 // sequence b, a chunk is c = max(least, ceil(sum n_b / units)) steps, one and
-// the same for all, so that ragged batches load the CUs evenly: with as many
-// units as run at once, or, once those would pass kLongChunk steps, with
-// `most`, which even out what some take longer.  At most most + B chunks come of
-// that, times the key heads: the grid.  (24 sequences of up to 8000 tokens, 4 key
-// heads of 96: 54 us in chunks of 8 steps, 44 in one round of blocks.)
+// the same for all, so that ragged batches load the CUs evenly: `units` blocks
+// for each CU to have a few, or, once their chunks would pass kLongChunk steps,
+// `most`, which even out what some take longer.  At most most + B chunks come
+// of that, times the key heads: the grid.  (24 sequences of up to 8000 tokens,
+// 4 key heads of 96: 54 us in chunks of 8 steps, 49 in 16; 12 heads of 96: 104
+// us with two blocks a CU, 97 with four.)
 struct Cut {
   int64_t B;
   int heads;           // key heads
-  int64_t units, most; // chunks to aim for, for each head: as many as run at once, as many as long ones make
+  int64_t units, most; // chunks to aim for, for each head: of ordinary calls, of long ones
   int64_t least;       // steps of a chunk at least
   int64_t rows;        // queries of a key head: T * group
   float* part;         // a slot of rows * (D + 2) floats a block
@@ -243,17 +244,17 @@ __device__ __forceinline__ bool find_unit(const Rows& rows, const Cut& cut, Unit
   return false;
 }
 
-// Chunks and grid for `most` tokens a sequence at the most, `round` blocks running
-// at once; *blocks the grid.
+// Chunks and grid for `most` tokens a sequence at the most and `aim` blocks;
+// *blocks the grid.
 // Where scratch or counters do not hold a slot for each, sequences stay whole.
-inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int64_t least, int64_t round, Cut* cut,
+inline int plan_cut(int64_t B, int heads, int64_t rows, int D, int64_t most, int64_t least, int64_t aim, Cut* cut,
                     int64_t* blocks, const char* who) {
   const int64_t slots = static_cast<int64_t>(kScratchBytes / 4) / (rows * (D + 2)) / heads;
   cut->B = B;
   cut->heads = heads;
   cut->rows = rows;
   cut->least = least;
-  cut->units = ceil_div(round, heads);
+  cut->units = ceil_div(aim, heads);
   cut->most = ceil_div(8 * ctx().num_cus, heads);
   if (cut->most < cut->units) cut->most = cut->units;
   cut->part = static_cast<float*>(ctx().scratch);

@@ -373,7 +373,7 @@ static int launch_few(const QueryArgs& a, const PagedRows& rows, int64_t queries
   const int64_t seen = rows.a.window && rows.a.window < capacity ? rows.a.window + a.T - 1 : capacity;
   Cut cut;
   int64_t blocks;
-  KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 16, int64_t{2} * ctx().num_cus,
+  KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 16, int64_t{4} * ctx().num_cus,
                   &cut, &blocks, "cache_attention"));
   // codes; then the waves' sums; then, beside the first's, the chunks' weights
   const int R = static_cast<int>(queries);

@@ -804,11 +804,14 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
     }
     __syncthreads();
     const Part out{b, h, here, 0, 1, first + part * kPutRows, nullptr, 0, nullptr};
-    if (put_rows<T, kTileThreads>(a, out, sums, pitch, wm, wl, nullptr)) continue;
-    __syncthreads();
-    for (int i = wave; i < here; i += kTileThreads / 64) {
-      const int64_t at_row = out.first + i;
-      one_query<T>(a, rows, b, at_row / a.group, h * a.group + static_cast<int>(at_row % a.group), sums + wave * kMaxHead);
+    const bool out_is_there = put_rows<T, kTileThreads>(a, out, sums, pitch, wm, wl, nullptr);
+    if constexpr (SRC != kPaged) {  // (no page marks a part)
+      if (out_is_there) continue;
+      __syncthreads();
+      for (int i = wave; i < here; i += kTileThreads / 64) {
+        const int64_t at_row = out.first + i;
+        one_query<T>(a, rows, b, at_row / a.group, h * a.group + static_cast<int>(at_row % a.group), sums + wave * kMaxHead);
+      }
     }
   }
 }
@@ -832,7 +835,7 @@ __global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, R
   const float* ml = from + kTileRows * D + r;
   const float m = lane < parts ? ml[lane * part_floats(D)] : -INFINITY;
   const float l = lane < parts ? ml[lane * part_floats(D) + kTileRows] : 0.0f;
-  if (__any(m != m)) {
+  if (!std::is_same<Rows, PagedRows>::value && __any(m != m)) {
     one_query<T>(a, rows, b, t, head, qv[wave]);
     return;
   }
