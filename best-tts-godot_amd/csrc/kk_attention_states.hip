@@ -31,7 +31,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // token lies over LANES lanes of 16 bytes, U times 64 / LANES tokens are a
 // wave's step, and the next step's are loaded while it works.  Each group of
 // LANES lanes keeps a maximum, sum and outputs of its own tokens; they are joined
-// at the end.
+// at the end.  32 sequences of 1500 to 2999 states: 93 us for 12 heads of 64 in
+// fp32 (4.7 TB/s of the 6.2 that reading alone reaches; 193 us in tiles for the
+// matrix cores, which bring states to halves for one query in 128), 71 us for 8
+// key heads of 128 under 32 query heads in fp16 (4.1 TB/s).
 template <typename T, int LANES, int R, int U>
 __global__ void __launch_bounds__(kStateThreads, 2) few_states_kernel(QueryArgs a, DenseRows<T> rows, Cut cut) {
   constexpr int VEC = 16 / sizeof(T), TOK = 64 / LANES, STEP = TOK * U;
@@ -193,7 +196,9 @@ __global__ void __launch_bounds__(kStateThreads, 2) few_states_kernel(QueryArgs 
 
 template <typename T, int LANES, int R>
 static int launch_states(const QueryArgs& a, const DenseRows<T>& rows, int64_t queries) {
-  constexpr int U = R > 4 ? 2 : 4;
+  constexpr int U = R > 4 ? 2 : 4;  // (eight queries' sums leave registers for two tokens a lane in flight)
+  // chunks of four steps at least, of one where each takes eight queries' products
+  // (7 queries over 700 states: 33 us in chunks of 8 steps, 25 in 4, 22 in 1)
   Cut cut;
   int64_t blocks;
   KK_TRY(plan_cut(a.B, a.heads / a.group, queries, a.D, rows.a.S, R > 4 ? 1 : 4, int64_t{8} * ctx().num_cus, &cut, &blocks,

@@ -90,6 +90,15 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // (half a step of the output's type); that they are 2^8 times as large keeps 32
 // bits between the largest and fp16's smallest value.
 //
+// Bound by the vector units beside the products: 32 x 64 scores a wave take some
+// 300 vector instructions for their softmax against 32 (fp16, 128 values) or 48
+// (fp32, 64) products, bringing a tile 120 (codes), 30 (fp16) or 400 (fp32) a
+// wave.  2 x 1531 queries of 32 heads of 128 over up to 4099 cached tokens: 257
+// us, 452 TFLOP/s; 2 x 3000 over 1500 fp16 states: 160 us, 690 TFLOP/s; 2 x 3380
+// of 12 heads of 64 over up to 509 fp32 states: 65 us.  64 tokens a tile: keys and
+// values of 128 take 36 KB, so that two blocks a CU overlap one's loads with the
+// other's products; 256 queries a block, for half the loads, gave 256 and 86 us.
+//
 // A state that is not finite (or, where queries see different ones, whose size
 // is too far from another's) poisons whole sums here (0 times it is NaN) where
 // only queries that see it should be: a block that meets one marks its part, and
@@ -817,7 +826,10 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 }
 
 // Joins the parts of queries whose tokens were shared by several blocks, a wave a
-// query: weights 2^(m_i - max) / sum_i l_i 2^(m_i - max), a lane a part.
+// query: weights 2^(m_i - max) / sum_i l_i 2^(m_i - max), a lane a part.  A launch
+// of its own, so that parts go by ordinary stores and many CUs join them (2 x 100
+// queries of 28 heads over up to 2000 tokens: 35 us with it, 101 where the last
+// block of a tile joins its parts).
 template <typename T, class Rows>
 __global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, Rows rows, TileCut cut) {
   __shared__ float qv[kTileThreads / 64][kMaxHead];
@@ -858,7 +870,8 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, co
   TileCut cut{};
   cut.rows = queries;
   // where there are fewer blocks than two a CU, the tokens are cut, into parts
-  // of two tiles at least
+  // of two tiles at least (100 fp32 queries of 12 heads of 128 over 1400 states: 31
+  // us; in parts of four tiles 83)
   const int64_t blocks = pairs * tiles, head = (blocks * 4 + 15) / 16 * 16;
   int64_t splits = ceil_div(2 * ctx().num_cus, blocks);
   const int64_t room = (static_cast<int64_t>(kScratchBytes) - head) / 4 / part_floats(a.D) / blocks;

