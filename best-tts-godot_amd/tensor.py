@@ -75,10 +75,9 @@ class Storage:
     __slots__ = ("ptr", "nbytes", "__weakref__")
 
     def __init__(self, nbytes):
-        if _state["device"] is None:
-            init()
         alloc = _fast.get("kk_alloc")
         if alloc is None:
+            init()
             alloc = _fast["kk_alloc"] = _lib.load().kk_alloc
         rc = alloc(nbytes if nbytes > 0 else 1, _alloc_ref)
         if rc:
@@ -119,8 +118,8 @@ def signal_stream(stream=0):
     _lib.call("kk_stream_signal", int(stream))
 
 
-_PROTOS = {}  # (shape, strides, dtype) -> KKTensor with data unset
-_INTERFACES = {}  # (shape, strides, dtype) -> array interface but for the address
+_PROTOS = {}  # (shape, strides, dtype's letter) -> KKTensor with data unset
+_INTERFACES = {}  # (shape, strides, dtype's letter) -> array interface but for the address
 
 
 @functools.lru_cache(maxsize=4096)
@@ -222,7 +221,7 @@ class DeviceTensor:
         """This tensor's memory for another library (torch.as_tensor(t,
         device="cuda") makes a view that keeps it alive).  Not synchronised:
         call sync(), or signal_stream() with the stream that reads it."""
-        key = (self.shape, self.strides, self.dtype)
+        key = (self.shape, self.strides, self.dtype.char)
         fixed = _INTERFACES.get(key)
         if fixed is None:
             item = self.dtype.itemsize
@@ -263,8 +262,9 @@ class DeviceTensor:
         """The kk_tensor descriptor (cached; views are immutable).  Descriptors
         of one (shape, strides, dtype) differ only in the data pointer: each
         is copied from a cached prototype."""
-        if self._desc is None:
-            key = (self.shape, self.strides, self.dtype)
+        ref = self._desc
+        if ref is None:
+            key = (self.shape, self.strides, self.dtype.char)
             proto = _PROTOS.get(key)
             if proto is None:
                 proto = _lib.KKTensor()
@@ -277,8 +277,8 @@ class DeviceTensor:
                     _PROTOS[key] = proto
             d = _lib.KKTensor.from_buffer_copy(proto)
             d.data = self.storage.ptr + self.offset * self.dtype.itemsize
-            self._desc = d
-        return ctypes.byref(self._desc)
+            ref = self._desc = ctypes.byref(d)  # (which keeps d)
+        return ref
 
     def __repr__(self):
         return f"DeviceTensor(shape={self.shape}, dtype={self.dtype}, strides={self.strides})"
