@@ -189,6 +189,45 @@ def test_states_of_mixed_sizes(gpu, T):
     within(out[0], want, (8 + 8) * 2.0 ** -24 * np.abs(want).max())
 
 
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("dim", [3, 90, 100, 129, 250, 255])
+@pytest.mark.parametrize("T,S", [(1, 300), (40, 150), (200, 70)])
+def test_heads_whose_rows_start_anywhere(gpu, t, dim, T, S):
+    kk = gpu
+    r = rng(dim + T)
+    q = r.normal(size=(1, T, 2, dim)).astype(t)
+    k, v = (r.normal(size=(1, S, 1, dim)).astype(t) for _ in range(2))
+    mask = r.random((1, S)) < 0.7
+    dev = kk.to_device
+    out = kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), mask=dev(mask), scale=0.08))
+    some = np.unique([0, T // 2, T - 1])
+    want = D.attention(q[0][some], k[0], v[0], lambda i: np.flatnonzero(mask[0]), 0.08)
+    within(out[0][some], want, attention_tol(q[0][some], k[0], v[0], want, 0.08, t, S))
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("dim", [48, 64, 96, 128, 240, 256])
+@pytest.mark.parametrize("T", [1, 20, 50])
+def test_cache_queries_that_start_anywhere(gpu, t, dim, T):
+    """Queries and outputs one value behind a multiple of 16 bytes, head-major."""
+    kk = gpu
+    r = rng(dim + T)
+    table, pages = pool(r, 1, 10)
+    parts = random_cache(r, pages, 1, 32, dim)
+    base = r.normal(size=(1, 2, T, dim + 1)).astype(t)
+    q = np.ascontiguousarray(base.transpose(0, 2, 1, 3)[..., 1:])
+    dev = kk.to_device
+    view = dev(base).transpose([0, 2, 1, 3]).slice_axis(3, 1, dim + 1)
+    room = dev(np.zeros_like(base))
+    out = room.transpose([0, 2, 1, 3]).slice_axis(3, 1, dim + 1)
+    cache, lengths = on_device(kk, parts), np.array([310], np.int32)
+    dt, dl = dev(table), dev(lengths)
+    kk._lib.call("kk_cache_attention", out.desc(), view.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
+                 cache.v_scale.desc(), dt.desc(), dl.desc(), None, 0.06, 0)
+    check_cache(kk, kk.to_host(out), q, parts, table, lengths, 0, 0.06, queries=np.unique([0, T // 2, T - 1]))
+    assert not kk.to_host(room)[..., 0].any()
+
+
 def test_masks_by_query_over_states_of_mixed_sizes(gpu):
     """Query i sees the i + 1 smallest of states that grow from 1e-12 to 1e12: to its own last bits."""
     kk = gpu
