@@ -585,13 +585,17 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
       int e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
       e1 = e1 > 254 ? 254 : e1;
-      if (__any(e1 > er)) {
+      // (e1 is of group lane % G, er of query lane % 32: any group against any query)
+      int eg[G], most = 0;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        eg[g] = __builtin_amdgcn_readlane(e1, g);
+        most = eg[g] > most ? eg[g] : most;
+      }
+      if (__any(most > er)) {
         int up = er;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int eg = __builtin_amdgcn_readlane(e1, g);
-          up = eg > up && (!tested || groups >> g & 1) ? eg : up;
-        }
+        for (int g = 0; g < G; ++g) up = eg[g] > up && (!tested || groups >> g & 1) ? eg[g] : up;
         keep_r = ldexpf(1.0f, er - up);
         er = up;
         if (__any(keep_r != 1.0f)) {

@@ -1,0 +1,91 @@
+"""Attention whose values are of far sizes: pages and rows that are large
+beside the others, seen by some queries only, or seen and given no weight.
+
+The bounds go by what a query weighs, sum_j p_j |v_j| from the 64-bit oracle
+(|v_j| a row's largest), not by the largest value that it sees.  Per query:
+scores are D products and sums in fp32 of |q| |k| in size, and a weight is a power
+of two of them, so that each is off by twice the scores' share; sums over the
+tokens in parts of 16 at the least; powers and quotient 8 U; a weight in two
+halves keeps 2^-24 of itself and 2^-38 of the largest weight times size, in one
+half (fp16 operands) 2^-11 and 2^-31."""
+import numpy as np
+import pytest
+
+from conftest import rng
+from oracle import decode_ops as D
+from test_parity_attention import run_cache
+from test_parity_decode import U, half_step, pool, random_cache, within
+
+pytestmark = pytest.mark.gpu
+DTYPES = [np.float32, np.float16]
+
+
+def check(out, q, k, v, seen, scale, what=""):
+    """out, q [T, Hq, D]; k, v [S, Hk, D]."""
+    t = q.dtype.type
+    q64, k64, v64 = (np.asarray(x, np.float64) for x in (q, k, v))
+    want = D.attention(q64, k64, v64, seen, scale)
+    group, tol = q.shape[1] // k.shape[1], np.zeros(want.shape)
+    for i in range(q.shape[0]):
+        at = np.asarray(seen(i), int)
+        if not at.size:
+            continue
+        for h in range(q.shape[1]):
+            g = h // group
+            s = k64[at, g] @ q64[i, h] * scale
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            size = p @ np.abs(v64[at, g]).max(-1)
+            share = 2 * (q.shape[-1] + 8) * U * (np.abs(k64[at, g]) @ np.abs(q64[i, h])).max() * abs(scale)
+            share += (at.size / 16 + 16) * U + at.size * 2.0 ** -38
+            if t == np.float16:
+                share += half_step(t) + at.size * 2.0 ** -31
+            tol[i, h] = 2 * share * size
+    tol += half_step(t) * np.abs(want) + 2.0 ** -25 * (t == np.float16)
+    within(out, want, tol, what)
+
+
+def check_cache(out, q, parts, table, n, scale, window=0, what=""):
+    """One sequence of n cached tokens, the newest q's own."""
+    k, _ = D.cached(parts[0], parts[1], table, n)
+    v, _ = D.cached(parts[2], parts[3], table, n, tokens_last=True)
+    place = n - q.shape[0] + np.arange(q.shape[0])
+    check(out, q, k, v, lambda i: np.arange(max(0, place[i] - window + 1) if window else 0, place[i] + 1), scale, what)
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("group", [1, 2])
+@pytest.mark.parametrize("jump", [4, 8, 12])
+def test_windows_over_pages_whose_scales_jump(gpu, t, block, group, jump):
+    """Large pages leave the windows of a wave's last queries as those before them still see them."""
+    kk = gpu
+    r = rng(100 * jump + block + group)
+    T, dim, window = 96, 64, 200
+    for n in (408, 409, 410):  # (the window passes a page's end at a wave's queries 31, 30, 29)
+        table, pages = pool(r, 1, -(-n // block))
+        parts = list(random_cache(r, pages, 8, block, dim))
+        parts[1][table[0]] = np.linspace(0.005, 0.03, table.shape[1], dtype=np.float32)[:, None]
+        parts[3] = (0.01 * np.where(r.random((pages, 8)) < 0.1, 2.0 ** jump, 1.0)).astype(np.float32)
+        q = (1.5 * r.normal(size=(1, T, 8 * group, dim))).astype(t)
+        out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=0.3, window=window)
+        check_cache(out[0], q[0], parts, table[0], n, 0.3, window, f"{n} tokens")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("n", [360, 361, 362])
+def test_one_large_page_behind_another_that_a_window_left(gpu, t, n):
+    """Two pages of 100 among pages of 0.01: a query that has left the first behind meets the second."""
+    kk = gpu
+    r = rng(n)
+    T, dim, block, window = 64, 64, 16, 200
+    table, pages = pool(r, 1, -(-n // block))
+    parts = list(random_cache(r, pages, 1, block, dim))
+    parts[1] = np.full((pages, 1), 0.01, np.float32)
+    for first in range(5, 12):
+        for apart in range(4, 10):
+            parts[3] = np.full((pages, 1), 0.01, np.float32)
+            parts[3][table[0, [first, first + apart]], 0] = 100.0
+            q = r.normal(size=(1, T, 1, dim)).astype(t)
+            out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=0.1, window=window)
+            check_cache(out[0], q[0], parts, table[0], n, 0.1, window, f"pages {first} and {first + apart}")
