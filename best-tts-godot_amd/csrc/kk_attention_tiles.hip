@@ -13,6 +13,7 @@ constexpr int kPutRows = 64;    // of them put out at a time
 constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
 constexpr int kSpread = 11;
 constexpr float kSlack = 7.0f;
+constexpr float kLeastSize = 100.0f;
 
 struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
@@ -85,8 +86,11 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // 8-bit codes and fp16 values are exact as halves; fp32 operands are the sum of
 // two, after a power of two for each row that brings its largest to 2^14, so
 // that 22 bits are kept whatever the rows' sizes, and the product of the two
-// low halves (2^-22) is left out.  Weights carry the rows' powers of two, or the
-// pages' scales, over that of the largest seen.  Weights of fp16 queries are rounded to fp16
+// low halves (2^-22) is left out.  fp32 weights carry the rows' powers of two, over
+// that of the largest seen.  Over pages, a weight carries its page's scale, over a
+// power of two of the largest such product that the query has met: by what it
+// weighs, not by what it sees, so that a page of large scale without weight takes
+// no bits from the others.  Weights of fp16 queries are rounded to fp16
 // (half a step of the output's type); that they are 2^8 times as large keeps 32
 // bits between the largest and fp16's smallest value.
 //
@@ -388,9 +392,11 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       }
   };
   float m = -3.4028235e38f, l = 0.0f, keep_r = 1.0f;
-  // values are scaled by 2^-(er - 127) (paged: of the lane's query), 2^-(er - 141)
-  // (fp32: of the block); least: the smallest row's exponent
-  int er = SRC == kPaged ? 27 : 0, least = 255;
+  // paged: log2 of the largest weight times page scale that the query has met (a
+  // whole number, as m is there; kLeastSize below m at the least), and 2^(m - mv + 8)
+  float mv = -3.4028235e38f, size = 256.0f;
+  // fp32: values are scaled by 2^-(er - 141) of the block; least: the smallest row's exponent
+  int er = 0, least = 255;
 
   auto stage = [&](int which) {
     if constexpr (SRC == kPaged) {
@@ -579,49 +585,19 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       for (int s = 0; s < 2 * NS; ++s) seen |= (static_cast<uint32_t>(w >> (16 * s)) & 0xffu) << (8 * s);
     }
 
-    float by[G], vw[G];
+    float by[G], vg[G], ev[G];  // of a group's tokens: score by, page scale, and its log2, rounded up
     if constexpr (SRC == kPaged) {
-      // the power of two above all scales that the lane's query has seen
       const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
-      int e1 = bits < 0x7f800000u ? static_cast<int>(bits >> 23) + 1 : 0;
-      e1 = e1 > 254 ? 254 : e1;
-      // (e1 is of group lane % G, er of query lane % 32: any group against any query)
-      int eg[G], most = 0;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        eg[g] = __builtin_amdgcn_readlane(e1, g);
-        most = eg[g] > most ? eg[g] : most;
-      }
-      if (__any(most > er)) {
-        int up = er;
-#pragma unroll
-        for (int g = 0; g < G; ++g) up = eg[g] > up && (!tested || groups >> g & 1) ? eg[g] : up;
-        keep_r = ldexpf(1.0f, er - up);
-        er = up;
-        if (__any(keep_r != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][e] *= keep_r;
-        }
-      }
-      const float r1 = __uint_as_float(static_cast<uint32_t>(254 - er) << 23);
+      const bool finite = bits < 0x7f800000u;
+      const float lane_v = finite ? vs : 0.0f;
+      const float lane_e = finite && bits ? static_cast<float>(static_cast<int>(bits >> 23) - 126) : -INFINITY;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         by[g] = cq * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), g));
-        vw[g] = r1 * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), g));
+        vg[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_v), g));
+        ev[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_e), g));
       }
-      if (tested) {  // a group that the query does not see (its scale may pass r), or one whose scale is not finite
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const bool sees = groups >> g & 1;
-          if (!sees) vw[g] = 0.0f;
-          if (!(__builtin_fabsf(vw[g]) < INFINITY)) {
-            vw[g] = 0.0f;
-            l = NAN;
-          }
-        }
-      }
+      if (poisoned && (groups & static_cast<uint32_t>(__ballot(!finite)))) l = NAN;  // (lane g is of group g)
     }
     {
       // fragments of keys or values are read a batch ahead of their products
@@ -684,13 +660,32 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[e] = seen >> (16 * j + e) & 1 ? s[e] : -INFINITY;
         }
-        float top = s[0];
+        float top = s[0], late = s[8];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        top = max_halves(top);
+        for (int e = 1; e < 8; ++e) {
+          top = fmaxf(top, s[e]);
+          late = fmaxf(late, s[8 + e]);
+        }
+        float sized = -INFINITY;
+        if constexpr (SRC == kPaged) sized = fmaxf(top + ev[2 * j % G], late + ev[(2 * j + 1) % G]);
+        top = max_halves(fmaxf(top, late));
         // m follows a row's maximum only where that is kSlack above it: weights are
-        // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again
-        if (__any(top > m + kSlack)) {
+        // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again; so does mv
+        if constexpr (SRC == kPaged) {
+          if (__any(top > m + kSlack || sized > mv + kSlack)) {
+            top = fmaxf(ceilf(top), m);
+            const float most = fmaxf(fmaxf(ceilf(max_halves(sized)), top - kLeastSize), mv);
+            const float keep = __builtin_amdgcn_exp2f(mv - most);
+            l *= __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            mv = most;
+            size = __builtin_amdgcn_exp2f(m - mv + 8.0f);
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
+          }
+        } else if (__any(top > m + kSlack)) {
           top = fmaxf(top, m);
           const float keep = __builtin_amdgcn_exp2f(m - top);
           m = top;
@@ -700,7 +695,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
         }
-        const float less = m - 8.0f;
+        const float less = SRC == kPaged ? m : m - 8.0f;
         h8 pf[2][PW];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -711,8 +706,9 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
             l += w[e];
           }
           if constexpr (SRC == kPaged) {
+            const float vw = fminf(vg[(2 * j + k) % G] * size, 3.4028235e38f);  // (past it: weights of zero)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] *= vw[(2 * j + k) % G];
+            for (int e = 0; e < 8; ++e) w[e] *= vw;
           }
           if constexpr (SRC == kFloat) {
 #pragma unroll
@@ -764,7 +760,9 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
   float* wm = sums + kPutRows * pitch;
   float* wl = wm + kPutRows;
   l = sum_halves(l);
-  const float scale = SRC == kHalf ? 1.0f : ldexpf(1.0f, er - (SRC == kPaged ? 127 : 141));
+  const float scale = SRC == kHalf    ? 1.0f
+                      : SRC == kPaged ? __builtin_amdgcn_exp2f(mv - m - 8.0f)
+                                      : ldexpf(1.0f, er - 141);
   const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile;
   if (cut.splits > 1 && chunk == 0 && tid == 0) cut.parts[pair] = chunks;
   if (chunks > 1) {

@@ -2,12 +2,12 @@
 beside the others, seen by some queries only, or seen and given no weight.
 
 The bounds go by what a query weighs, sum_j p_j |v_j| from the 64-bit oracle
-(|v_j| a row's largest), not by the largest value that it sees.  Per query:
-scores are D products and sums in fp32 of |q| |k| in size, and a weight is a power
-of two of them, so that each is off by twice the scores' share; sums over the
-tokens in parts of 16 at the least; powers and quotient 8 U; a weight in two
-halves keeps 2^-24 of itself and 2^-38 of the largest weight times size, in one
-half (fp16 operands) 2^-11 and 2^-31."""
+(|v_j| a row's largest), not by the largest value that it sees.  Score j is D
+products and sums in fp32 of |q| |k_j| in size, so that its power of two is off
+by e_j = 2 (D + 8) U |scale| |q| |k_j| of itself, and the quotient by their mean as
+well; sums over the tokens in parts of 16 at the least; powers and quotient 8 U; a
+weight in two halves keeps 2^-24 of itself and 2^-38 of the largest weight times
+size, in one half (fp16 operands) 2^-11 and 2^-31."""
 import numpy as np
 import pytest
 
@@ -35,12 +35,12 @@ def check(out, q, k, v, seen, scale, what=""):
             s = k64[at, g] @ q64[i, h] * scale
             p = np.exp(s - s.max())
             p /= p.sum()
-            size = p @ np.abs(v64[at, g]).max(-1)
-            share = 2 * (q.shape[-1] + 8) * U * (np.abs(k64[at, g]) @ np.abs(q64[i, h])).max() * abs(scale)
-            share += (at.size / 16 + 16) * U + at.size * 2.0 ** -38
+            top = np.abs(v64[at, g]).max(-1)
+            off = 2 * (q.shape[-1] + 8) * U * abs(scale) * (np.abs(k64[at, g]) @ np.abs(q64[i, h]))
+            share = p @ off + (at.size / 16 + 16) * U + at.size * 2.0 ** -38
             if t == np.float16:
                 share += half_step(t) + at.size * 2.0 ** -31
-            tol[i, h] = 2 * share * size
+            tol[i, h] = p @ (off * top) + 2 * share * (p @ top)
     tol += half_step(t) * np.abs(want) + 2.0 ** -25 * (t == np.float16)
     within(out, want, tol, what)
 
@@ -89,3 +89,30 @@ def test_one_large_page_behind_another_that_a_window_left(gpu, t, n):
             q = r.normal(size=(1, T, 1, dim)).astype(t)
             out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=0.1, window=window)
             check_cache(out[0], q[0], parts, table[0], n, 0.1, window, f"pages {first} and {first + apart}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,group,dim,block,n", [
+    (40, 1, 64, 16, 300), (40, 2, 128, 64, 300), (70, 1, 96, 32, 200), (33, 1, 240, 16, 150), (90, 1, 64, 256, 700)])
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9, 1e12, 1e30])
+def test_a_page_of_large_scale_without_weight_takes_no_bits(gpu, t, T, group, dim, block, n, ratio):
+    """Values `ratio` times the others', whose scores lie so far below that they weigh nothing, or (in a second head) as
+    much as all the others together."""
+    kk = gpu
+    r = rng(T + dim)
+    table, pages = pool(r, 1, -(-n // block))
+    parts = list(random_cache(r, pages, 2, block, dim))
+    parts[0] = r.integers(-12, 13, parts[0].shape).astype(np.int8)
+    sign = np.where(r.random(dim) < 0.5, 1, -1)
+    q = ((1 + 0.05 * r.random((1, T, 2 * group, dim))) * sign).astype(t)
+    parts[1] = np.full((pages, 2), 0.01, np.float32)
+    parts[3] = r.uniform(0.01, 0.02, (pages, 2)).astype(np.float32)
+    for page in table[0, [0, (n - T) // block // 2]] if block < 256 else table[0, 1:2]:
+        parts[0][page] = -127 * sign
+        parts[1][page] = np.float32((np.log(ratio) + np.array([60, 0])) / (127 * dim))
+        parts[3][page] *= np.float32(ratio)
+    out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=1.0)
+    at = np.unique([0, 1, T // 2, T - 2, T - 1])  # (of the queries the oracle forms, every one of these)
+    k, _ = D.cached(parts[0], parts[1], table[0], n)
+    v, _ = D.cached(parts[2], parts[3], table[0], n, tokens_last=True)
+    check(out[0][at], q[0][at], k, v, lambda i: np.arange(n - T + at[i] + 1), 1.0)
