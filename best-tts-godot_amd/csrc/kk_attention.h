@@ -7,6 +7,15 @@
 namespace kk {
 
 constexpr int kMaxHead = 256;
+// Weights over pages are kept beside 2^mv, mv = max log2(weight's power of two
+// times its page's scale), but not below 2^-kLeastSize of the largest power of two
+// (values whose scale is below that may lose bits).
+constexpr float kLeastSize = 100.0f;
+// The product of a page's scale and the power of two that its weights are kept
+// by; past the largest value those weights are zero, and stay so.
+__device__ __forceinline__ float sized_by(float scale, float by) {
+  return __builtin_amdgcn_fmed3f(scale * by, -3.4028235e38f, 3.4028235e38f);
+}
 
 // Queries and outputs: [B, T, heads, D], group query heads a key head.
 struct QueryArgs {

@@ -26,11 +26,12 @@ constexpr int kFewWaves = kFewThreads / 64;
 //
 // Codes are exact in fp16.  fp16 queries are taken as they are, fp32 ones as
 // the sum of two halves after a power of two that brings the row's largest to
-// 2^14 (22 bits; smaller values keep 2^-38 of the largest).  Weights, times
-// their page's scale over a power of two r >= all that the query has seen, are split into
-// two halves as well, also for fp16 queries (rounded to one, the output was 1.4
-// times as far off for the same time); 2^15 p <= 2^15 keeps 24 bits above fp16's
-// smallest value.
+// 2^14 (22 bits; smaller values keep 2^-38 of the largest).  Weights times
+// their page's scale, over a power of two of the largest such product that the
+// query has met (so that a page of large scale without weight takes no bits from
+// the others), are split into two halves as well, also for fp16 queries (rounded to
+// one, the output was 1.4 times as far off for the same time); 2^15 p <= 2^15 keeps
+// 24 bits above fp16's smallest value.
 template <typename T, int DT, int NT, bool EXACT>
 __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
     few_paged_kernel(QueryArgs a, PagedRows rows, Cut cut) {
@@ -167,12 +168,12 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
 
   f4 acc[NT][DT];
   float m[NT], l[NT];
-  int er[NT];  // r = 2^(er - 127), of what the lane's query has seen
+  float mv[NT];  // log2 of the largest weight times page scale that the lane's query has met, kLeastSize below m at the least
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt] = -3.4028235e38f;
     l[nt] = 0.0f;
-    er[nt] = 27;
+    mv[nt] = -3.4028235e38f;
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[nt][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -238,6 +239,8 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
 
     const uint32_t vbits = __float_as_uint(__builtin_fabsf(vs));
     const bool finite = vbits < 0x7f800000u;
+    // log2 of the scale, rounded up
+    const float ev = finite && vbits ? static_cast<float>(static_cast<int>(vbits >> 23) - 126) : -INFINITY;
 
     h8 pf[NT][2][PW];
 #pragma unroll
@@ -248,22 +251,6 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
       const int a0 = lo < 0 ? 0 : (lo > 16 ? 16 : static_cast<int>(lo));
       const int a1 = hi < 0 ? 0 : (hi > 16 ? 16 : static_cast<int>(hi));
       const bool whole = __all(a0 == 0 && a1 == 16 && finite);
-      // the power of two above all scales that the query has seen: the same in its lanes
-      int e1 = finite && a1 > a0 ? static_cast<int>(vbits >> 23) + 1 : 0;
-      e1 = e1 > 254 ? 254 : e1;
-      float keep_r = 1.0f;
-      if (__any(e1 > er[nt])) {
-#pragma unroll
-        for (int off = 16; off < 64; off <<= 1) {
-          const int o = __shfl_xor(e1, off, 64);
-          e1 = o > e1 ? o : e1;
-        }
-        const int up = e1 > er[nt] ? e1 : er[nt];
-        keep_r = ldexpf(1.0f, er[nt] - up);
-        er[nt] = up;
-      }
-      const float r15 = __uint_as_float(static_cast<uint32_t>(127 + 15 + 127 - er[nt]) << 23);  // 2^15 / r
-      const float vw = a1 > a0 ? vs * r15 : 0.0f;
       float x[16], top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
@@ -274,19 +261,25 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
+      float sized = top + ev;
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      top = fmaxf(top, m[nt]);
-      if (__any(top > m[nt] || keep_r != 1.0f)) {
-        const float keep = __builtin_amdgcn_exp2f(m[nt] - top);
+      // m and mv are whole numbers, so that the sums are scaled by powers of two
+      if (__any(top > m[nt] || sized > mv[nt])) {
+        top = fmaxf(ceilf(top), m[nt]);
+        sized = fmaxf(sized, __shfl_xor(sized, 16, 64));
+        sized = fmaxf(sized, __shfl_xor(sized, 32, 64));
+        const float most = fmaxf(fmaxf(ceilf(sized), top - kLeastSize), mv[nt]);
+        const float keep = __builtin_amdgcn_exp2f(mv[nt] - most);
+        l[nt] *= __builtin_amdgcn_exp2f(m[nt] - top);
         m[nt] = top;
-        l[nt] *= keep;
-        const float both = keep * keep_r;
+        mv[nt] = most;
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][i][e] *= both;
+          for (int e = 0; e < 4; ++e) acc[nt][i][e] *= keep;
       }
+      const float vw = a1 <= a0 ? 0.0f : finite ? sized_by(vs, __builtin_amdgcn_exp2f(m[nt] - mv[nt] + 15.0f)) : vs;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         x[j] = __builtin_amdgcn_exp2f(x[j] - m[nt]);
@@ -348,7 +341,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 && EXACT ? 2 : 1)
       wm[kFewWaves * R + r] = top;
       wl[kFewWaves * R + r] = sum;
     }
-    const float by = ldexpf(exp2f(m[nt] - top), er[nt] - 127 - 15);
+    const float by = exp2f(mv[nt] - top - 15.0f);
 #pragma unroll
     for (int i = 0; i < DT; ++i)
       if (16 * i < D) *reinterpret_cast<f4*>(sums + (wave * R + r) * pitch + 16 * i + 4 * g) = acc[nt][i] * by;

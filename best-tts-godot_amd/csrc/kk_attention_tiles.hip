@@ -13,7 +13,6 @@ constexpr int kPutRows = 64;    // of them put out at a time
 constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
 constexpr int kSpread = 11;
 constexpr float kSlack = 7.0f;
-constexpr float kLeastSize = 100.0f;
 
 struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
@@ -706,7 +705,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
             l += w[e];
           }
           if constexpr (SRC == kPaged) {
-            const float vw = fminf(vg[(2 * j + k) % G] * size, 3.4028235e38f);  // (past it: weights of zero)
+            const float vw = sized_by(vg[(2 * j + k) % G], size);
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] *= vw;
           }

@@ -93,7 +93,7 @@ def test_one_large_page_behind_another_that_a_window_left(gpu, t, n):
 
 @pytest.mark.parametrize("t", DTYPES)
 @pytest.mark.parametrize("T,group,dim,block,n", [
-    (40, 1, 64, 16, 300), (40, 2, 128, 64, 300), (70, 1, 96, 32, 200), (33, 1, 240, 16, 150), (90, 1, 64, 256, 700)])
+    (1, 1, 64, 16, 300), (1, 7, 128, 64, 900), (3, 2, 96, 32, 200), (20, 1, 48, 16, 150), (1, 4, 240, 128, 500), (40, 1, 64, 16, 300), (40, 2, 128, 64, 300), (70, 1, 96, 32, 200), (33, 1, 240, 16, 150), (90, 1, 64, 256, 700)])
 @pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9, 1e12, 1e30])
 def test_a_page_of_large_scale_without_weight_takes_no_bits(gpu, t, T, group, dim, block, n, ratio):
     """Values `ratio` times the others', whose scores lie so far below that they weigh nothing, or (in a second head) as
@@ -112,7 +112,7 @@ def test_a_page_of_large_scale_without_weight_takes_no_bits(gpu, t, T, group, di
         parts[1][page] = np.float32((np.log(ratio) + np.array([60, 0])) / (127 * dim))
         parts[3][page] *= np.float32(ratio)
     out = run_cache(kk, q, parts, table, np.array([n], np.int32), scale=1.0)
-    at = np.unique([0, 1, T // 2, T - 2, T - 1])  # (of the queries the oracle forms, every one of these)
+    at = np.unique(np.clip([0, 1, T // 2, T - 2, T - 1], 0, T - 1))  # (the queries that the oracle forms)
     k, _ = D.cached(parts[0], parts[1], table[0], n)
     v, _ = D.cached(parts[2], parts[3], table[0], n, tokens_last=True)
     check(out[0][at], q[0][at], k, v, lambda i: np.arange(n - T + at[i] + 1), 1.0)
