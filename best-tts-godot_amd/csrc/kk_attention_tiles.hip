@@ -11,7 +11,6 @@ constexpr int kTileThreads = 256;
 constexpr int kTileRows = 128;  // queries of a block: 32 a wave
 constexpr int kPutRows = 64;    // of them put out at a time
 constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
-constexpr int kSpread = 11;
 constexpr float kSlack = 7.0f;
 
 struct TileCut {
@@ -29,13 +28,12 @@ constexpr int64_t part_floats(int D) { return int64_t{kTileRows} * (D + 2); }
 enum Source { kPaged, kHalf, kFloat };
 
 // LDS of a block, in bytes: keys [TT][pitch], values [32 DT][pitch] (a copy for each
-// half of a split value), of dense rows what is added to their scores (0, or -inf
-// where none is seen), of fp32 ones their largest magnitudes and scales; later
-// the sums.
+// part of a split value), of dense rows what is added to their scores (0, or -inf
+// where none is seen); later the sums.
 constexpr int key_pitch(int DT) { return 64 * DT + 16; }
 constexpr int value_pitch(int TT) { return 2 * TT + 16; }
 constexpr int tile_bytes(int SRC, int DT, int TT) {
-  return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 2 : 1) + (SRC == kFloat ? 7 : SRC == kHalf ? 1 : 0) * TT * 4;
+  return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 3 : 1) + (SRC == kPaged ? 0 : TT * 4);
 }
 
 // The larger of, or the sum of, the values of lanes l and l ^ 32.
@@ -53,6 +51,59 @@ __device__ __forceinline__ void split2(float x, float y, h2* hi, h2* lo) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   *hi = __builtin_convertvector((f2{x, y}), h2);
   *lo = __builtin_convertvector((f2{x - static_cast<float>((*hi)[0]), y - static_cast<float>((*hi)[1])}), h2);
+}
+
+// Two values as the sums of three bf16 each, exactly (a part's rest is exact in
+// fp32): word p holds both values' parts p.  `rest` becomes NaN where a value is
+// not finite, or too large for bf16.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&word)[3], float* rest) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    const b2 v = __builtin_convertvector((f2{x, y}), b2);
+    word[p] = __builtin_bit_cast(uint32_t, v);
+    if (p == 2) break;
+    x -= __uint_as_float(word[p] << 16);
+    y -= __uint_as_float(word[p] & 0xffff0000u);
+    if (p == 0) *rest = __builtin_fmaf(x, 0.0f, __builtin_fmaf(y, 0.0f, *rest));
+  }
+}
+
+// c + a b of 32x32x16: of halves, or of bf16 parts.
+template <int SRC>
+__device__ __forceinline__ f16v product(h8 a, h8 b, f16v c) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  if constexpr (SRC == kFloat)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// c + the products of a's and b's parts, the small ones first; those below the
+// last part of a value (2^-24) are left out.
+template <int SRC, int PA, int PB>
+__device__ __forceinline__ f16v product_of_parts(const h8 (&a)[PA], const h8 (&b)[PB], f16v c) {
+  constexpr int kMost = (PA > PB ? PA : PB) - 1;
+#pragma unroll
+  for (int order = kMost; order >= 0; --order)
+#pragma unroll
+    for (int i = PA - 1; i >= 0; --i)
+      if (order - i >= 0 && order - i < PB) c = product<SRC>(a[i], b[order - i], c);
+  return c;
+}
+
+// Eight values as fragments of their three parts.
+__device__ __forceinline__ void split3(const float (&x)[8], h8 (&to)[3], float* rest) {
+  u4 part[3];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    uint32_t word[3];
+    split3(x[i], x[i + 1], word, rest);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) part[p][i / 2] = word[p];
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p) to[p] = __builtin_bit_cast(h8, part[p]);
 }
 
 // Whether a mask differs from query to query, and what it lets query t see of
@@ -82,44 +133,44 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // with lane l ^ 32, and with the tokens' order in the keys' rows (row_of) its
 // registers are, eight by eight, what the product O^T = V^T P^T takes.
 //
-// 8-bit codes and fp16 values are exact as halves; fp32 operands are the sum of
-// two, after a power of two for each row that brings its largest to 2^14, so
-// that 22 bits are kept whatever the rows' sizes, and the product of the two
-// low halves (2^-22) is left out.  fp32 weights carry the rows' powers of two, over
-// that of the largest seen.  Over pages, a weight carries its page's scale, over a
-// power of two of the largest such product that the query has met: by what it
-// weighs, not by what it sees, so that a page of large scale without weight takes
-// no bits from the others.  Weights of fp16 queries are rounded to fp16
-// (half a step of the output's type); that they are 2^8 times as large keeps 32
-// bits between the largest and fp16's smallest value.
+// 8-bit codes and fp16 values are exact as halves.  fp32 queries over pages are the
+// sum of two, after a power of two for each row that brings its largest to 2^14,
+// which keeps 22 bits.  fp32 queries over fp32 states, states and weights are sums of three
+// bf16 each, exactly, with fp32's exponents: no row shares a power of two with
+// another, or a value with its row, so that each keeps its own bits (values below
+// 2^-110 those that fp32's normal numbers hold); of nine products the three of
+// 2^-24 and less are left out.  Over pages, a weight carries
+// its page's scale, over a power of two of the largest such product that the query
+// has met: by what it weighs, not by what it sees, so that a page of large scale
+// without weight takes no bits from the others.  Weights of fp16 queries are rounded
+// to fp16 (half a step of the output's type); that they are 2^8 times as large keeps
+// 32 bits between the largest and fp16's smallest value.
 //
 // Bound by the vector units beside the products: 32 x 64 scores a wave take some
-// 300 vector instructions for their softmax against 32 (fp16, 128 values) or 48
-// (fp32, 64) products, bringing a tile 120 (codes), 30 (fp16) or 400 (fp32) a
+// 300 vector instructions for their softmax against 32 (fp16, 128 values) or 96
+// (fp32, 64) products, bringing a tile 120 (codes), 30 (fp16) or 220 (fp32) a
 // wave.  2 x 1531 queries of 32 heads of 128 over up to 4099 cached tokens: 257
 // us, 452 TFLOP/s; 2 x 3000 over 1500 fp16 states: 160 us, 690 TFLOP/s; 2 x 3380
-// of 12 heads of 64 over up to 509 fp32 states: 65 us.  64 tokens a tile: keys and
+// of 12 heads of 64 over up to 509 fp32 states: 71 us (67 in two halves beside the
+// block's largest row, which lost rows that a query weighs beside a large one that
+// it does not; heads of 80 and 96 take a tenth less than so, of 128 a twentieth).  64 tokens a tile: keys and
 // values of 128 take 36 KB, so that two blocks a CU overlap one's loads with the
 // other's products; 256 queries a block, for half the loads, gave 256 and 86 us.
 //
-// A state that is not finite (or, where queries see different ones, whose size
-// is too far from another's) poisons whole sums here (0 times it is NaN) where
+// A state that is not finite poisons whole sums here (0 times it is NaN) where
 // only queries that see it should be: a block that meets one marks its part, and
 // its queries are formed one by one.
 template <typename T, class Rows, int SRC, int DT, int TT, bool WIDE>
 __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2 : sizeof(T) == 4 ? 3 : 4) ? 2 : 1)
     attention_tile_kernel(QueryArgs a, Rows rows, TileCut cut) {
-  constexpr int PQ = sizeof(T) == 4 ? 2 : 1, PK = SRC == kFloat ? 2 : 1, PW = PQ;
+  constexpr int PQ = SRC == kFloat ? 3 : sizeof(T) == 4 ? 2 : 1, PK = SRC == kFloat ? 3 : 1, PW = PQ;  // parts
   constexpr int KS = 2 * DT, NS = TT / 32, G = TT / 16;
   constexpr int KP = key_pitch(DT), VP = value_pitch(TT);
   constexpr bool kAhead = SRC != kFloat || DT <= 4;  // (fp32 heads past 128 values leave no registers for it)
   extern __shared__ __attribute__((aligned(16))) char tile_lds[];
   char* lds_k = tile_lds;
   char* lds_v = lds_k + PK * TT * KP;
-  uint32_t* largest = reinterpret_cast<uint32_t*>(lds_v + PK * 32 * DT * VP);  // [2][keys, values][TT]
-  float* key_scale = reinterpret_cast<float*>(largest + 4 * TT);
-  float* value_scale = key_scale + TT;
-  float* key_bias = SRC == kFloat ? value_scale + TT : reinterpret_cast<float*>(largest);
+  float* key_bias = reinterpret_cast<float*>(lds_v + PK * 32 * DT * VP);
 
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int n = lane % 32, hf = lane / 32, D = a.D;
@@ -195,20 +246,26 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(x[s][i]));
       }
-      top = max_halves(top);
-      const int up = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
-      cq = ldexpf(a.scale, -up);
+      if constexpr (SRC == kFloat) {
+        float unused = 0.0f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s) split3(x[s], qf[s], &unused);
+      } else {
+        top = max_halves(top);
+        const int up = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
+        cq = ldexpf(a.scale, -up);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          h2 y0, y1;
-          split2(ldexpf(x[s][i], up), ldexpf(x[s][i + 1], up), &y0, &y1);
-          qf[s][0][i] = y0[0];
-          qf[s][0][i + 1] = y0[1];
-          qf[s][PQ - 1][i] = y1[0];
-          qf[s][PQ - 1][i + 1] = y1[1];
-        }
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            h2 y0, y1;
+            split2(ldexpf(x[s][i], up), ldexpf(x[s][i + 1], up), &y0, &y1);
+            qf[s][0][i] = y0[0];
+            qf[s][0][i + 1] = y0[1];
+            qf[s][PQ - 1][i] = y1[0];
+            qf[s][PQ - 1][i + 1] = y1[1];
+          }
+      }
     }
   }
 
@@ -367,37 +424,15 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       }
     }
   };
-  uint32_t bad = 0;  // half: bit 15 or 31 for a value that is not finite; fp32: the largest magnitude's bits
-  auto magnitudes = [&](int which) {
-    uint32_t* lk = largest + 2 * TT * which;
-    uint32_t* lv = lk + TT;
-#pragma unroll
-    for (int i = 0; i < UK; ++i) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, ck[(2 * i + e / 4) % (2 * UK)][e % 4] & 0x7fffffffu);
-      atomicMax(lk + key_unit(i) / (4 * DT), m);
-      bad = max(bad, m);
-    }
-#pragma unroll
-    for (int i = 0; i < UV; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, cv[(4 * i + j) % (4 * UV)][e] & 0x7fffffffu);
-        atomicMax(lv + value_tokens(value_unit(i)) + j, m);
-        bad = max(bad, m);
-      }
-  };
-  float m = -3.4028235e38f, l = 0.0f, keep_r = 1.0f;
+  // of values that are not finite: half: bit 15 or 31; fp32: NaN
+  uint32_t bad = 0;
+  float rest = 0.0f;
+  float m = -3.4028235e38f, l = 0.0f;
   // paged: log2 of the largest weight times page scale that the query has met (a
   // whole number, as m is there; kLeastSize below m at the least), and 2^(m - mv + 8)
   float mv = -3.4028235e38f, size = 256.0f;
-  // fp32: values are scaled by 2^-(er - 141) of the block; least: the smallest row's exponent
-  int er = 0, least = 255;
 
-  auto stage = [&](int which) {
+  auto stage = [&]() {
     if constexpr (SRC == kPaged) {
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
@@ -441,61 +476,37 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
           for (int e = 0; e < 4; ++e) bad |= (cv[(4 * i + j) % (4 * UV)][e] & 0x7c007c00u) + 0x04000400u;
       }
     } else {
-      const uint32_t* lk = largest + 2 * TT * which;
-      const uint32_t* lv = lk + TT;
-      // the values' power of two: of the largest so far
-      const int top = static_cast<int>(__float_as_uint(wave_max_dpp(__uint_as_float(lv[lane % TT]))) >> 23);
-      const int up = top > er ? top : er;
-      keep_r = ldexpf(1.0f, er - up);
-      er = up;
-      const float low = lv[lane % TT] ? __uint_as_float(lv[lane % TT]) : INFINITY;
-      const int bottom = static_cast<int>(__float_as_uint(-wave_max_dpp(-low)) >> 23);
-      least = bottom < least ? bottom : least;
 #pragma unroll
       for (int i = 0; i < UK; ++i) {
         const int u = key_unit(i), tk = u / (4 * DT), c = u % (4 * DT);
-        const int by = 141 - static_cast<int>(lk[tk] >> 23);
-        h8 y0, y1;
+        float x[8];
+        h8 part[3];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          h2 p0, p1;
-          split2(__builtin_amdgcn_ldexpf(__uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4]), by),
-                 __builtin_amdgcn_ldexpf(__uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4 + 1]), by), &p0, &p1);
-          y0[e] = p0[0];
-          y0[e + 1] = p0[1];
-          y1[e] = p1[0];
-          y1[e + 1] = p1[1];
-        }
-        *reinterpret_cast<h8*>(lds_k + row_of(tk) * KP + 16 * c) = y0;
-        *reinterpret_cast<h8*>(lds_k + (TT + row_of(tk)) * KP + 16 * c) = y1;
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4]);
+        split3(x, part, &rest);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          *reinterpret_cast<h8*>(lds_k + (p * TT + row_of(tk)) * KP + 16 * c) = part[p];
       }
 #pragma unroll
       for (int i = 0; i < UV; ++i) {
         const int u = value_unit(i), d = value_d(u), tk = value_tokens(u);
-        const u4 of = *reinterpret_cast<const u4*>(lv + tk);
-        int by[4];
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) by[j] = 141 - static_cast<int>(of[j] >> 23);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h4 y0, y1;
+        for (int e = 0; e < 4; ++e) {  // one value of four tokens
+          u2 part[3];
 #pragma unroll
           for (int j = 0; j < 4; j += 2) {
-            h2 p0, p1;
-            split2(__builtin_amdgcn_ldexpf(__uint_as_float(cv[(4 * i + j) % (4 * UV)][e]), by[j]),
-                   __builtin_amdgcn_ldexpf(__uint_as_float(cv[(4 * i + j + 1) % (4 * UV)][e]), by[j + 1]), &p0, &p1);
-            y0[j] = p0[0];
-            y0[j + 1] = p0[1];
-            y1[j] = p1[0];
-            y1[j + 1] = p1[1];
+            uint32_t word[3];
+            split3(__uint_as_float(cv[(4 * i + j) % (4 * UV)][e]),
+                   __uint_as_float(cv[(4 * i + j + 1) % (4 * UV)][e]), word, &rest);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) part[p][j / 2] = word[p];
           }
-          *reinterpret_cast<h4*>(lds_v + (d + e) * VP + 2 * tk) = y0;
-          *reinterpret_cast<h4*>(lds_v + (32 * DT + d + e) * VP + 2 * tk) = y1;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<u2*>(lds_v + (p * 32 * DT + d + e) * VP + 2 * tk) = part[p];
         }
       }
-      if (tid >= 64 && tid < 64 + TT) key_scale[tid - 64] = ldexpf(1.0f, static_cast<int>(lk[tid - 64] >> 23) - 141);
-      if (tid >= 128 && tid < 128 + TT) value_scale[tid - 128] = ldexpf(1.0f, static_cast<int>(lv[tid - 128] >> 23) - er);
-      if (tid < 2 * TT) largest[2 * TT * (which ^ 1) + tid] = 0;
     }
   };
 
@@ -521,25 +532,19 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
   const bool by_query = rows_masked_by_query(rows, a);
   if (wave * 32 >= count) upto = from = 0;  // (no queries: the wave only helps to bring tiles)
 
-  if constexpr (SRC == kFloat) {
-    if (tid < 2 * TT) largest[tid] = 0;
-    __syncthreads();
-  }
   if (kAhead && lo < hi) {
     find_entry(lo);
     fetch(lo);
     find_entry(lo + TT);
   }
-  int which = 0;
-  for (int64_t t0 = lo; t0 < hi; t0 += TT, which ^= 1) {
+  for (int64_t t0 = lo; t0 < hi; t0 += TT) {
     if (!kAhead) {
       find_entry(t0);
       fetch(t0);
     }
     const bool empty = SRC != kPaged && word == 0;  // the same in all waves
-    if (SRC == kFloat && !empty) magnitudes(which);
     __syncthreads();  // the tile before is read
-    if (!empty) stage(which);
+    if (!empty) stage();
     const int page = page1;
     const float ks = ks1, vs = page < 0 ? 0.0f : vs1;
     if (kAhead && t0 + TT < hi) {
@@ -547,14 +552,6 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       find_entry(t0 + 2 * TT);
     }
     __syncthreads();
-    if (empty) which ^= 1;  // (the magnitudes' other half is not cleared)
-    if (SRC == kFloat && keep_r != 1.0f) {
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] *= keep_r;
-      keep_r = 1.0f;
-    }
     if (empty || t0 >= upto || t0 + TT <= from) continue;
     // what the lane's query sees of its tokens 32 j + 16 k + 8 hf + e: bit 16 j + 8 k + e
     uint32_t seen = 0, groups = 0;  // (groups: bit g: some of tokens 16 g .. 16 g + 15)
@@ -600,7 +597,8 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
     }
     {
       // fragments of keys or values are read a batch ahead of their products
-      constexpr int KB = DT > 4 ? 1 : 2, BATCHES = KS / KB, VB = DT > 4 || DT % 2 ? 1 : 2, VBATCHES = DT / VB;
+      constexpr int KB = DT > 4 || PK > 1 ? 1 : 2, BATCHES = KS / KB;
+      constexpr int VB = DT > 4 || DT % 2 || PK > 1 ? 1 : 2, VBATCHES = DT / VB;
       h8 kf[2][KB][PK], vf[2][VB][PK];
       auto read_keys = [&](int j, int batch, h8 (&to)[KB][PK]) {
 #pragma unroll
@@ -630,12 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
           else
             read_values(2 * j, 0, vf[0]);
 #pragma unroll
-          for (int k = 0; k < KB; ++k) {
-            const int q = batch * KB + k;
-            if constexpr (PK == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][PK - 1], qf[q][0], s, 0, 0, 0);
-            if constexpr (PQ == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][0], qf[q][PQ - 1], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[now][k][0], qf[q][0], s, 0, 0, 0);
-          }
+          for (int k = 0; k < KB; ++k) s = product_of_parts<SRC>(kf[now][k], qf[batch * KB + k], s);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -645,14 +638,8 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
             for (int e = 0; e < 4; ++e) s[4 * c + e] *= by[(2 * j + c / 2) % G];
           } else {
             const f4 bias = *reinterpret_cast<const f4*>(key_bias + tk);
-            if constexpr (SRC == kHalf) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e], cq, bias[e]);
-            } else {
-              const f4 kc = *reinterpret_cast<const f4*>(key_scale + tk);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e] * cq, kc[e], bias[e]);
-            }
+            for (int e = 0; e < 4; ++e) s[4 * c + e] = __builtin_fmaf(s[4 * c + e], cq, bias[e]);
           }
         }
         if (tested) {
@@ -669,7 +656,8 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
         if constexpr (SRC == kPaged) sized = fmaxf(top + ev[2 * j % G], late + ev[(2 * j + 1) % G]);
         top = max_halves(fmaxf(top, late));
         // m follows a row's maximum only where that is kSlack above it: weights are
-        // 2^(x - m + 8) <= 2^15, and few tiles scale the sums again; so does mv
+        // 2^(x - m + 8) <= 2^15 (fp32: 2^(x - m - kSlack)), and few tiles scale the sums
+        // again; so does mv
         if constexpr (SRC == kPaged) {
           if (__any(top > m + kSlack || sized > mv + kSlack)) {
             top = fmaxf(ceilf(top), m);
@@ -694,7 +682,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][e] *= keep;
         }
-        const float less = SRC == kPaged ? m : m - 8.0f;
+        const float less = SRC == kPaged ? m : SRC == kHalf ? m - 8.0f : m + kSlack;
         h8 pf[2][PW];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -710,22 +698,19 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
             for (int e = 0; e < 8; ++e) w[e] *= vw;
           }
           if constexpr (SRC == kFloat) {
+            float unused = 0.0f;
+            split3(w, pf[k], &unused);
+          } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const f4 vc = *reinterpret_cast<const f4*>(value_scale + 32 * j + 16 * k + 8 * hf + 4 * c);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[4 * c + e] *= vc[e];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            h2 p0, p1;
-            split2(w[e], w[e + 1], &p0, &p1);
-            pf[k][0][e] = p0[0];
-            pf[k][0][e + 1] = p0[1];
-            if constexpr (PW == 2) {
-              pf[k][PW - 1][e] = p1[0];
-              pf[k][PW - 1][e + 1] = p1[1];
+            for (int e = 0; e < 8; e += 2) {
+              h2 p0, p1;
+              split2(w[e], w[e + 1], &p0, &p1);
+              pf[k][0][e] = p0[0];
+              pf[k][0][e + 1] = p0[1];
+              if constexpr (PW == 2) {
+                pf[k][PW - 1][e] = p1[0];
+                pf[k][PW - 1][e + 1] = p1[1];
+              }
             }
           }
         }
@@ -737,31 +722,21 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
           else if (j + 1 < NS)
             read_keys(j + 1, 0, kf[(j + 1) * BATCHES % 2]);
 #pragma unroll
-          for (int i = 0; i < VB; ++i) {
-            f16v& o = acc[batch * VB + i];
-            if constexpr (PK == 2) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][PK - 1], pf[k][0], o, 0, 0, 0);
-            if constexpr (PW == 2) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][0], pf[k][PW - 1], o, 0, 0, 0);
-            o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[step % 2][i][0], pf[k][0], o, 0, 0, 0);
-          }
+          for (int i = 0; i < VB; ++i)
+            acc[batch * VB + i] = product_of_parts<SRC>(vf[step % 2][i], pf[k], acc[batch * VB + i]);
         }
       }
     }
   }
 
   // the sums by rows, half of them at a time, in LDS
-  // (rows of values more than 2^kSpread apart keep their bits beside each other
-  // only if all queries see the same of them)
-  if (SRC == kFloat && by_query && er - least > kSpread) bad = 0x7f800000u;
-  const uint32_t none = SRC == kHalf ? bad & 0x80008000u : SRC == kFloat ? static_cast<uint32_t>(bad >= 0x7f800000u) : 0u;
-  const bool marked = __syncthreads_or(none != 0);
+  const bool marked = __syncthreads_or(SRC == kHalf ? (bad & 0x80008000u) != 0 : rest != rest);
   const int pitch = D + 4;
   float* sums = reinterpret_cast<float*>(tile_lds);
   float* wm = sums + kPutRows * pitch;
   float* wl = wm + kPutRows;
   l = sum_halves(l);
-  const float scale = SRC == kHalf    ? 1.0f
-                      : SRC == kPaged ? __builtin_amdgcn_exp2f(mv - m - 8.0f)
-                                      : ldexpf(1.0f, er - 141);
+  const float scale = SRC == kPaged ? __builtin_amdgcn_exp2f(mv - m - 8.0f) : 1.0f;
   const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile;
   if (cut.splits > 1 && chunk == 0 && tid == 0) cut.parts[pair] = chunks;
   if (chunks > 1) {

@@ -116,3 +116,54 @@ def test_a_page_of_large_scale_without_weight_takes_no_bits(gpu, t, T, group, di
     k, _ = D.cached(parts[0], parts[1], table[0], n)
     v, _ = D.cached(parts[2], parts[3], table[0], n, tokens_last=True)
     check(out[0][at], q[0][at], k, v, lambda i: np.arange(n - T + at[i] + 1), 1.0)
+
+
+def run_states(kk, q, k, v, mask=None, scale=1.0):
+    dev = kk.to_device
+    return kk.to_host(kk.ops.cross_attention(dev(q), dev(k), dev(v), mask=None if mask is None else dev(mask), scale=scale))
+
+
+@pytest.mark.parametrize("T,group,dim,S", [(1, 1, 64, 300), (8, 1, 128, 90), (40, 2, 64, 300), (33, 1, 128, 1000), (200, 1, 96, 130),
+                                           (40, 1, 200, 90), (50, 2, 33, 260)])
+@pytest.mark.parametrize("by_query", [False, True])
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9, 1e12, 1e30])
+def test_states_of_large_values_without_weight_take_no_bits(gpu, T, group, dim, S, by_query, ratio):
+    """As for pages: the rows that weigh nothing in one head weigh as much as all the others together in another."""
+    kk = gpu
+    r = rng(T + dim)
+    sign = np.where(r.random(dim) < 0.5, 1.0, -1.0)
+    q = ((1 + 0.05 * r.random((1, T, 2 * group, dim))) * sign).astype(np.float32)
+    k = (0.1 * r.normal(size=(1, S, 2, dim))).astype(np.float32)
+    v = r.normal(size=(1, S, 2, dim)).astype(np.float32)
+    for row in (3, S // 2, S - 1):
+        k[0, row] = -sign * (np.log(ratio) + np.array([[60], [0]])) / dim
+        v[0, row] *= np.float32(ratio)
+    mask = r.random((1, T, S)) < 0.8 if by_query else None
+    if by_query:
+        mask[:, :, [3, S // 2, S - 1]] = True
+    out = run_states(kk, q, k, v, mask)
+    at = np.unique(np.clip([0, 1, T // 2, T - 2, T - 1], 0, T - 1))
+    check(out[0][at], q[0][at], k[0], v[0], lambda i: np.flatnonzero(mask[0, at[i]]) if by_query else np.arange(S), 1.0)
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_channels_of_mixed_sizes_keep_their_own_bits(gpu, T):
+    """Channels of values 1e-9 to 1e9 in one row, queries' and keys' channels of opposite sizes: an output's bound goes
+    by its own channel's values."""
+    kk = gpu
+    r = rng(T)
+    dim, S = 64, 200
+    size = 10.0 ** r.permutation(np.linspace(-9, 9, dim))
+    q = (size * r.normal(size=(1, T, 1, dim))).astype(np.float32)
+    k = (0.2 / size * r.normal(size=(1, S, 1, dim))).astype(np.float32)
+    v = (r.permutation(size) * r.normal(size=(1, S, 1, dim))).astype(np.float32)
+    out = run_states(kk, q, k, v)
+    q64, k64, v64 = (np.asarray(x[0], np.float64) for x in (q, k, v))
+    for i in np.unique([0, T // 2, T - 1]):
+        s = k64[:, 0] @ q64[i, 0]
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        off = 2 * (dim + 8) * U * (np.abs(k64[:, 0]) @ np.abs(q64[i, 0]))
+        share = p @ off + (S / 16 + 16) * U
+        tol = (p * off) @ np.abs(v64[:, 0]) + 2 * share * (p @ np.abs(v64[:, 0]))
+        within(out[0, i, 0], p @ v64[:, 0], tol, f"query {i}")
