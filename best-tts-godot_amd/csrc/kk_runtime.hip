@@ -750,6 +750,7 @@ int kk_event_elapsed(int a, int b, float* ms) {
 // `after` waits for what `before` holds: an event that lives for the call (a
 // recorded event that is destroyed is released when it has completed).
 static int order_streams(hipStream_t before, hipStream_t after) {
+  if (before == after) return KK_OK;
   hipEvent_t ev;
   KK_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
   hipError_t e = hipEventRecord(ev, before);

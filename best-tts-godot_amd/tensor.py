@@ -10,6 +10,7 @@ the reference's Reshape/Transpose/Squeeze/Unsqueeze/Slice/Split branches do
 import ctypes
 import functools
 import math
+import sys
 
 import numpy as np
 
@@ -95,7 +96,9 @@ class Storage:
 
 
 class Borrowed:
-    """Device memory of another library's array, which is kept alive."""
+    """Device memory of another library's array, which is kept alive.  Where
+    it is torch's, torch's current stream waits for libkk's work before the
+    memory goes back to torch's allocator."""
 
     __slots__ = ("ptr", "nbytes", "owner")
 
@@ -103,6 +106,32 @@ class Borrowed:
         self.ptr = ptr
         self.nbytes = nbytes
         self.owner = owner
+
+    def __del__(self):
+        try:
+            if _is_torch(self.owner):
+                _order("kk_stream_signal")
+        except Exception:  # interpreter shutdown
+            pass
+
+
+def _is_torch(arr):
+    torch = sys.modules.get("torch")
+    return torch is not None and isinstance(arr, torch.Tensor)
+
+
+def _order(which):
+    """kk_stream_wait or kk_stream_signal with torch's current stream, where
+    torch has one.  Not while a graph is recorded: its replays are ordered by
+    whoever launches them."""
+    torch = sys.modules.get("torch")
+    if torch is None or _state["device"] is None or not torch.cuda.is_initialized():
+        return
+    try:
+        _lib.call(which, torch.cuda.current_stream(_state["device"]).cuda_stream)
+    except _lib.KKError as e:
+        if e.code != -4:  # KK_E_STATE
+            raise
 
 
 def wait_stream(stream=0):
@@ -191,11 +220,15 @@ class DeviceTensor:
     def from_array(cls, arr, stream=None):
         """A tensor over the memory of a device array of another library (one
         with `__cuda_array_interface__`, as torch's and cupy's have): no copy,
-        any strides, `arr` kept alive.  libkk has a stream of its own: with
-        `stream` (see wait_stream), or where the array names its stream,
-        libkk's later work waits for what that stream holds; otherwise the
-        values must be there already.  Memory that its owner may hand out
-        again must be kept until libkk has used it (sync or signal_stream)."""
+        any strides, `arr` kept alive.  libkk has a stream of its own: its
+        later work waits for what `stream` (see wait_stream) holds, or the
+        stream that the array names, or, for torch's arrays, torch's current
+        stream; the values of other libraries' arrays that name no stream must
+        be there already.  What is written to the array later needs
+        wait_stream again.  A torch array's memory goes back to torch when the
+        tensor and the array are dropped, in the order of torch's current
+        stream; other libraries' must be kept until libkk has used it (sync
+        or signal_stream)."""
         desc = arr.__cuda_array_interface__
         dtype = np.dtype(desc["typestr"])
         if dtype not in NP_TO_CODE:
@@ -213,6 +246,10 @@ class DeviceTensor:
             stream = 0 if desc["stream"] == 1 else desc["stream"]
         if stream is not None:
             wait_stream(stream)
+        elif _is_torch(arr):
+            if arr.device.index != init():
+                raise ValueError(f"an array on {arr.device}: libkk is on device {init()}")
+            _order("kk_stream_wait")
         t = cls(Borrowed(int(desc["data"][0] or 0), math.prod(shape) * dtype.itemsize, arr), shape, dtype, strides)
         return t
 
