@@ -128,6 +128,7 @@ PROTOTYPES = {
     "kk_process_logits": [_T] * 9,
     "kk_stream_wait": [_vp],
     "kk_stream_signal": [_vp],
+    "kk_stream": [ctypes.POINTER(_vp)],
     "kk_graph_begin": [],
     "kk_graph_begin_arena": [_sz],
     "kk_graph_abort": [],

@@ -771,6 +771,13 @@ int kk_stream_signal(void* stream) {
   return order_streams(ctx().stream, static_cast<hipStream_t>(stream));
 }
 
+int kk_stream(void** stream) {
+  KK_TRY(require_ready());
+  if (!stream) return set_error(KK_E_ARG, "kk_stream: NULL output");
+  *stream = ctx().stream;
+  return KK_OK;
+}
+
 int kk_graph_begin(void) {
   KK_TRY(require_ready());
   KK_TRY(not_capturing("kk_graph_begin"));

@@ -71,9 +71,11 @@ _fast = {}  # bound entry points of the allocation path
 
 
 class Storage:
-    """One pooled device buffer."""
+    """One pooled device buffer; `lent` once another library was told its
+    address: then libkk's stream waits for torch's current one before the
+    pool may hand the memory out again."""
 
-    __slots__ = ("ptr", "nbytes", "__weakref__")
+    __slots__ = ("ptr", "nbytes", "lent", "__weakref__")
 
     def __init__(self, nbytes):
         alloc = _fast.get("kk_alloc")
@@ -85,11 +87,14 @@ class Storage:
             _lib.raise_error("kk_alloc", rc)
         self.ptr = _alloc_out.value
         self.nbytes = nbytes
+        self.lent = False
 
     def __del__(self):
         ptr, self.ptr = getattr(self, "ptr", None), None
         if ptr and _lib._lib is not None:
             try:
+                if self.lent:
+                    _order("kk_stream_wait")
                 _lib._lib.kk_free(ptr)
             except Exception:  # interpreter shutdown: the process frees it
                 pass
@@ -145,6 +150,13 @@ def signal_stream(stream=0):
     """Work given to `stream` from here on starts after what libkk holds now."""
     init()
     _lib.call("kk_stream_signal", int(stream))
+
+
+def _stream_name():
+    """libkk's stream as the array interface names it: HIP's handle, but 1 the default stream."""
+    handle = ctypes.c_void_p(None)
+    _lib.call("kk_stream", ctypes.byref(handle))
+    return handle.value or 1
 
 
 _PROTOS = {}  # (shape, strides, dtype's letter) -> KKTensor with data unset
@@ -256,17 +268,26 @@ class DeviceTensor:
     @property
     def __cuda_array_interface__(self):
         """This tensor's memory for another library (torch.as_tensor(t,
-        device="cuda") makes a view that keeps it alive).  Not synchronised:
-        call sync(), or signal_stream() with the stream that reads it."""
+        device="cuda") makes a view that keeps it alive).  torch's current
+        stream waits for what libkk has been given so far; other libraries find
+        libkk's stream in the interface and wait for it themselves.  A reader
+        on any other stream needs signal_stream() before it reads, and
+        wait_stream() before the tensor is dropped."""
         key = (self.shape, self.strides, self.dtype.char)
         fixed = _INTERFACES.get(key)
         if fixed is None:
             item = self.dtype.itemsize
-            fixed = {"shape": self.shape, "typestr": self.dtype.str, "version": 2, "strides":
+            fixed = {"shape": self.shape, "typestr": self.dtype.str, "version": 3, "strides":
                      None if self.is_contiguous() else tuple(st * item for st in self.strides)}
             if len(_INTERFACES) < 4096:
                 _INTERFACES[key] = fixed
-        return dict(fixed, data=(self.storage.ptr + self.offset * self.dtype.itemsize if 0 not in self.shape else 0, False))
+        out = dict(fixed, data=(self.storage.ptr + self.offset * self.dtype.itemsize if 0 not in self.shape else 0, False))
+        if _state["device"] is not None:
+            if isinstance(self.storage, Storage):
+                self.storage.lent = True
+            _order("kk_stream_signal")
+            out["stream"] = _stream_name()
+        return out
 
     # ------------------------------------------------------------ queries
     @property

@@ -583,6 +583,8 @@ int kk_event_elapsed(int start_slot, int stop_slot, float* ms);
  * host.  Not while a graph is being recorded. */
 int kk_stream_wait(void* stream);
 int kk_stream_signal(void* stream);
+/* libkk's stream (a hipStream_t, NULL the default stream). */
+int kk_stream(void** stream);
 
 /* ---------------------------------------------------------- HIP graphs
  * Records the ops called between kk_graph_begin and kk_graph_end on the

@@ -83,3 +83,40 @@ def test_arrays_may_be_taken_and_dropped_while_recording(gpu):
         del t
     finally:
         kk._lib.call("kk_graph_abort")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [False, True])
+def test_what_libkk_has_still_to_write_is_waited_for(warm, side):
+    kk = warm
+    s = torch.cuda.Stream() if side else torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        z = torch.as_tensor(long_work_kk(kk), device="cuda") + 1
+        assert bool((z == 101).all())
+
+
+@pytest.mark.gpu
+def test_memory_lent_to_torch_is_read_before_it_is_written(warm):
+    kk = warm
+    x = torch.zeros(N, device="cuda")
+    t = kk.ops.fill((N,), 7)
+    view = torch.as_tensor(t, device="cuda")
+    torch.cuda.synchronize()
+    long_work(x)
+    z = view + x
+    ptr = t.ptr
+    del t, view
+    y = kk.ops.fill((N,), -1)
+    assert y.ptr == ptr  # (the pool hands the same memory out)
+    assert bool((z == 107).all()) and (kk.to_host(y) == -1).all()
+
+
+@pytest.mark.gpu
+def test_the_interface_names_libkks_stream(gpu):
+    kk = gpu
+    t = kk.to_device(np.arange(3, dtype=np.float32))
+    desc = t.__cuda_array_interface__
+    assert desc["version"] == 3 and desc["stream"] > 2
+    again = kk.DeviceTensor.from_array(t)  # (a stream does not wait for itself)
+    assert kk.to_host(again).tolist() == [0, 1, 2]
