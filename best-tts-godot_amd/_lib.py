@@ -129,6 +129,7 @@ PROTOTYPES = {
     "kk_stream_wait": [_vp],
     "kk_stream_signal": [_vp],
     "kk_stream": [ctypes.POINTER(_vp)],
+    "kk_stream_use": [_vp, _i],
     "kk_graph_begin": [],
     "kk_graph_begin_arena": [_sz],
     "kk_graph_abort": [],

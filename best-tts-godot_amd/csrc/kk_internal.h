@@ -17,7 +17,9 @@ namespace kk {
 struct Context {
   bool ready = false;
   int device = -1;
-  hipStream_t stream = nullptr;
+  hipStream_t stream = nullptr;  // all work's: `own`, or another library's (kk_stream_use)
+  hipStream_t own = nullptr;     // made by kk_init; graphs are recorded on it
+  hipStream_t resume = nullptr;  // `stream` after the recording under way
   int num_cus = 0;
   bool capturing = false;  // between kk_graph_begin and kk_graph_end
   // Per-row arrival counters of the multi-block row reductions, zero

@@ -461,6 +461,26 @@ static int not_capturing(const char* who) {
   return KK_OK;
 }
 
+// A recording takes place on libkk's own stream (the default stream cannot
+// record), whichever stream the graph will be launched on.
+static int begin_recording() {
+  Context& c = ctx();
+  // Thread-local mode: HIP itself refuses unsafe calls (hipMalloc) made by
+  // this thread while recording.
+  KK_HIP(hipStreamBeginCapture(c.own, hipStreamCaptureModeThreadLocal));
+  c.resume = c.stream;
+  c.stream = c.own;
+  c.capturing = true;
+  return KK_OK;
+}
+
+static hipError_t end_recording(hipGraph_t* g) {
+  Context& c = ctx();
+  c.capturing = false;
+  c.stream = c.resume;
+  return hipStreamEndCapture(c.own, g);
+}
+
 static void destroy_graphs() {
   for (auto& s : graphs()) {
     if (s.exec) (void)hipGraphExecDestroy(s.exec);
@@ -475,10 +495,9 @@ static void abandon_recording() {
   Context& c = ctx();
   if (!c.capturing) return;
   hipGraph_t g = nullptr;
-  (void)hipStreamEndCapture(c.stream, &g);
+  (void)end_recording(&g);
   if (g) (void)hipGraphDestroy(g);
   (void)hipGetLastError();
-  c.capturing = false;
   arena_release(g_rec_arena);  // nothing recorded into it has run
   g_rec_arena = nullptr;
 }
@@ -518,7 +537,8 @@ int kk_init(int device) {
   if (device < 0 || device >= n)
     return set_error(KK_E_ARG, "device %d not present (%d visible)", device, n);
   KK_HIP(hipSetDevice(device));
-  KK_HIP(hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking));
+  KK_HIP(hipStreamCreateWithFlags(&c.own, hipStreamNonBlocking));
+  c.stream = c.own;
   hipDeviceProp_t prop;
   KK_HIP(hipGetDeviceProperties(&prop, device));
   c.num_cus = prop.multiProcessorCount;
@@ -546,8 +566,8 @@ int kk_shutdown(void) {
   if (c.scratch) { (void)hipFree(c.scratch); c.scratch = nullptr; }
   for (int i = 0; i < KK_MAX_EVENTS; ++i)
     if (g_event_made[i]) { (void)hipEventDestroy(g_events[i]); g_event_made[i] = false; }
-  (void)hipStreamDestroy(c.stream);
-  c.stream = nullptr;
+  (void)hipStreamDestroy(c.own);
+  c.stream = c.own = nullptr;
   c.ready = false;
   c.device = -1;
   return KK_OK;
@@ -771,6 +791,16 @@ int kk_stream_signal(void* stream) {
   return order_streams(ctx().stream, static_cast<hipStream_t>(stream));
 }
 
+int kk_stream_use(void* stream, int own) {
+  KK_TRY(require_ready());
+  KK_TRY(not_capturing("kk_stream_use"));
+  Context& c = ctx();
+  const hipStream_t next = own ? c.own : static_cast<hipStream_t>(stream);
+  KK_TRY(order_streams(c.stream, next));
+  c.stream = next;
+  return KK_OK;
+}
+
 int kk_stream(void** stream) {
   KK_TRY(require_ready());
   if (!stream) return set_error(KK_E_ARG, "kk_stream: NULL output");
@@ -781,11 +811,7 @@ int kk_stream(void** stream) {
 int kk_graph_begin(void) {
   KK_TRY(require_ready());
   KK_TRY(not_capturing("kk_graph_begin"));
-  // Thread-local mode: HIP itself refuses unsafe calls (hipMalloc) made by
-  // this thread while recording.
-  KK_HIP(hipStreamBeginCapture(ctx().stream, hipStreamCaptureModeThreadLocal));
-  ctx().capturing = true;
-  return KK_OK;
+  return begin_recording();
 }
 
 int kk_graph_begin_arena(size_t arena_bytes) {
@@ -801,13 +827,12 @@ int kk_graph_begin_arena(size_t arena_bytes) {
     return set_error(KK_E_NOMEM, "kk_graph_begin_arena: hipMalloc(%zu) failed: %s", arena_bytes,
                      hipGetErrorString(e));
   }
-  e = hipStreamBeginCapture(ctx().stream, hipStreamCaptureModeThreadLocal);
-  if (e != hipSuccess) {
+  const int begun = begin_recording();
+  if (begun != KK_OK) {
     arena_release(a);
-    return check_hip(e, "hipStreamBeginCapture");
+    return begun;
   }
   g_rec_arena = a;
-  ctx().capturing = true;
   return KK_OK;
 }
 
@@ -831,11 +856,10 @@ int kk_graph_end(int* graph_id) {
     abandon_recording();
     return set_error(KK_E_ARG, "graph_id is NULL");
   }
-  ctx().capturing = false;
   GraphSlot s;
   s.arena = g_rec_arena;
   g_rec_arena = nullptr;
-  hipError_t e = hipStreamEndCapture(ctx().stream, &s.graph);
+  hipError_t e = end_recording(&s.graph);
   if (e != hipSuccess) {
     if (s.graph) (void)hipGraphDestroy(s.graph);
     keep_dead_arena(s.arena);

@@ -24,13 +24,15 @@ NP_TO_CODE = {
 }
 CODE_TO_NP = {v: k for k, v in NP_TO_CODE.items()}
 
-_state = {"device": None, "downloads": 0}  # downloads: DeviceTensor.numpy calls so far
+# downloads: DeviceTensor.numpy calls so far; stream: the handle of libkk's stream
+_state = {"device": None, "downloads": 0, "stream": None}
 
 
 def init(device=0):
     """Initialise libkk on `device` (idempotent)."""
     if _state["device"] is None:
         _lib.call("kk_init", int(device))
+        _state["stream"] = _stream()
         _state["device"] = int(device)
     return _state["device"]
 
@@ -91,11 +93,12 @@ class Storage:
 
     def __del__(self):
         ptr, self.ptr = getattr(self, "ptr", None), None
-        if ptr and _lib._lib is not None:
+        if ptr:
             try:
                 if self.lent:
                     _order("kk_stream_wait")
-                _lib._lib.kk_free(ptr)
+                if _lib._lib is not None:
+                    _lib._lib.kk_free(ptr)
             except Exception:  # interpreter shutdown: the process frees it
                 pass
 
@@ -105,7 +108,7 @@ class Borrowed:
     it is torch's, torch's current stream waits for libkk's work before the
     memory goes back to torch's allocator."""
 
-    __slots__ = ("ptr", "nbytes", "owner")
+    __slots__ = ("ptr", "nbytes", "owner", "lent")
 
     def __init__(self, ptr, nbytes, owner):
         self.ptr = ptr
@@ -125,15 +128,29 @@ def _is_torch(arr):
     return torch is not None and isinstance(arr, torch.Tensor)
 
 
+def _torch_stream(device):
+    """The handle of torch's current stream; libkk's own where torch has none yet."""
+    torch = sys.modules.get("torch")
+    if torch is None or device is None or not torch.cuda.is_initialized():
+        return _state["stream"]
+    # from here on by the shortest way (the first is the second without an object for it)
+    _fast["torch_stream"] = (getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+                             (lambda d: torch.cuda.current_stream(d).cuda_stream))
+    return _fast["torch_stream"](device)
+
+
+_fast["torch_stream"] = _torch_stream
+
+
 def _order(which):
     """kk_stream_wait or kk_stream_signal with torch's current stream, where
-    torch has one.  Not while a graph is recorded: its replays are ordered by
-    whoever launches them."""
-    torch = sys.modules.get("torch")
-    if torch is None or _state["device"] is None or not torch.cuda.is_initialized():
+    torch has one that is not libkk's.  Not while a graph is recorded: its
+    replays are ordered by whoever launches them."""
+    stream = _fast["torch_stream"](_state["device"])
+    if stream == _state["stream"]:
         return
     try:
-        _lib.call(which, torch.cuda.current_stream(_state["device"]).cuda_stream)
+        _lib.call(which, stream)
     except _lib.KKError as e:
         if e.code != -4:  # KK_E_STATE
             raise
@@ -152,11 +169,23 @@ def signal_stream(stream=0):
     _lib.call("kk_stream_signal", int(stream))
 
 
-def _stream_name():
-    """libkk's stream as the array interface names it: HIP's handle, but 1 the default stream."""
+def use_stream(stream=None):
+    """libkk's work from here on goes to `stream` (a handle, see wait_stream;
+    None: libkk's own stream), after what it has been given so far.  A program
+    whose torch and libkk work alternate gives libkk torch's stream
+    (`use_stream(torch.cuda.current_stream().cuda_stream)`): all of it is then
+    in the order of the calls, and nothing waits where arrays are handed over."""
+    init()
+    if stream is not None and stream == _state["stream"]:
+        return
+    _lib.call("kk_stream_use", stream, stream is None)
+    _state["stream"] = _stream()
+
+
+def _stream():
     handle = ctypes.c_void_p(None)
     _lib.call("kk_stream", ctypes.byref(handle))
-    return handle.value or 1
+    return handle.value or 0
 
 
 _PROTOS = {}  # (shape, strides, dtype's letter) -> KKTensor with data unset
@@ -281,13 +310,14 @@ class DeviceTensor:
                      None if self.is_contiguous() else tuple(st * item for st in self.strides)}
             if len(_INTERFACES) < 4096:
                 _INTERFACES[key] = fixed
-        out = dict(fixed, data=(self.storage.ptr + self.offset * self.dtype.itemsize if 0 not in self.shape else 0, False))
-        if _state["device"] is not None:
-            if isinstance(self.storage, Storage):
-                self.storage.lent = True
-            _order("kk_stream_signal")
-            out["stream"] = _stream_name()
-        return out
+        storage = self.storage
+        address = storage.ptr + self.offset * self.dtype.itemsize if 0 not in self.shape else 0
+        if _state["device"] is None:
+            return dict(fixed, data=(address, False))
+        storage.lent = True
+        _order("kk_stream_signal")
+        # (1 is the interface's name of the default stream)
+        return dict(fixed, data=(address, False), stream=_state["stream"] or 1)
 
     # ------------------------------------------------------------ queries
     @property

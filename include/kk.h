@@ -12,7 +12,8 @@
  *  - Every entry point returns 0 on success and a negative KK_E* code on
  *    failure; it never aborts.  kk_last_error() describes the last failure of
  *    the calling thread.
- *  - All work is enqueued on the library's one HIP stream, in call order.
+ *  - All work is enqueued on one HIP stream, in call order: the library's own,
+ *    or the one that kk_stream_use names.
  *    kk_download() and kk_sync() wait for it; nothing else blocks.
  *  - Tensors are described by kk_tensor: a device pointer to element
  *    [0,...,0], a dtype code and up to KK_MAX_RANK extents and element
@@ -583,8 +584,14 @@ int kk_event_elapsed(int start_slot, int stop_slot, float* ms);
  * host.  Not while a graph is being recorded. */
 int kk_stream_wait(void* stream);
 int kk_stream_signal(void* stream);
-/* libkk's stream (a hipStream_t, NULL the default stream). */
+/* The stream of libkk's work (a hipStream_t, NULL the default stream). */
 int kk_stream(void** stream);
+/* Gives libkk's work to `stream` from here on (or, where `own` is not 0, to
+ * libkk's own again), after what it holds: work of both libraries is then in
+ * the order of the calls, without the two above, whose order between streams
+ * takes the host and the GPU some 15 us a call.  The stream must live until
+ * another is named.  Graphs recorded before and after are launched on it. */
+int kk_stream_use(void* stream, int own);
 
 /* ---------------------------------------------------------- HIP graphs
  * Records the ops called between kk_graph_begin and kk_graph_end on the

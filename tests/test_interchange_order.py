@@ -120,3 +120,61 @@ def test_the_interface_names_libkks_stream(gpu):
     assert desc["version"] == 3 and desc["stream"] > 2
     again = kk.DeviceTensor.from_array(t)  # (a stream does not wait for itself)
     assert kk.to_host(again).tolist() == [0, 1, 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [False, True])
+def test_work_on_torchs_stream_is_in_the_order_of_the_calls(warm, side):
+    kk = warm
+    s = torch.cuda.Stream() if side else torch.cuda.default_stream()
+    own = kk.to_device(np.zeros(1, np.float32)).__cuda_array_interface__["stream"]
+    one = kk.to_device(np.float32(1))
+    x = torch.zeros(N, device="cuda")
+    t = kk.DeviceTensor.from_array(x)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(s):
+            kk.use_stream(s.cuda_stream)
+            kk.use_stream(s.cuda_stream)
+            for i in range(20):
+                x += 1
+                y = kk.ops.binary("Add", t, one)  # (the same handle: no order but the stream's)
+                x.copy_(torch.as_tensor(y, device="cuda"))
+            assert t.__cuda_array_interface__["stream"] == (s.cuda_stream or 1)
+            assert bool((x == 40).all())
+    finally:
+        kk.use_stream()
+    assert t.__cuda_array_interface__["stream"] == own
+    assert (kk.to_host(t) == 40).all()
+
+
+@pytest.mark.gpu
+def test_graphs_on_torchs_default_stream(gpu):
+    """Recorded while libkk works on the default stream, which cannot record, and launched there between torch's work."""
+    import ctypes
+    kk = gpu
+    x = torch.zeros(1000, device="cuda")
+    t = kk.DeviceTensor.from_array(x)
+    y, one = kk.DeviceTensor.empty((1000,)), kk.to_device(np.float32(1))
+    g = ctypes.c_int(-1)
+    kk.use_stream(torch.cuda.default_stream().cuda_stream)
+    try:
+        kk._lib.call("kk_graph_begin")
+        with pytest.raises(kk._lib.KKError, match="recorded"):
+            kk.use_stream()
+        kk._lib.call("kk_binary", kk._lib.OP["Add"], y.desc(), t.desc(), one.desc())
+        kk._lib.call("kk_graph_end", ctypes.byref(g))
+        view = torch.as_tensor(y, device="cuda")
+        for i in range(5):
+            x += 1
+            kk._lib.call("kk_graph_launch", g.value)
+            assert bool((view == i + 2).all()), f"replay {i}"
+            assert (kk.to_host(kk.ops.binary("Add", y, one)) == i + 3).all()
+        kk._lib.call("kk_graph_begin")
+        kk._lib.call("kk_graph_abort")
+        assert t.__cuda_array_interface__["stream"] == 1
+    finally:
+        kk.use_stream()
+    kk._lib.call("kk_graph_launch", g.value)
+    assert (kk.to_host(y) == 6).all()
+    kk._lib.call("kk_graph_destroy", g.value)
