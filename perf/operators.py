@@ -13,6 +13,7 @@ benchmarked utterance, 26 frames a token); the others are generic.  B
 sequences, T new tokens each, Hq query and Hk key/value heads of D values,
 S encoder states, V entries of the vocabulary, L tokens of history.
 """
+import functools
 import importlib
 import math
 
@@ -325,17 +326,21 @@ def _logits_plain(s):
 
 
 # ------------------------------------------------------- the framework's own
+@functools.lru_cache
 def _kk():
     return importlib.import_module("best-tts-godot_amd")
 
 
 def _handles(kk, s):
-    """The state's buffers as the framework's tensors (no copies), made once, as a program keeps them."""
-    if "handles" not in s:
-        kk.init(0)
-        s["handles"] = {n: kk.DeviceTensor.from_array(x) for n, x in s.items() if isinstance(x, torch.Tensor)}
+    """The state's buffers as the framework's tensors (no copies), made once, as a program keeps them, and again where
+    the state has got other buffers since."""
+    made = s.get("handles")
+    if made is None or not all(s[n] is x for n, x in made["of"]):
+        of = [(n, x) for n, x in s.items() if isinstance(x, torch.Tensor)]
+        made = {n: kk.DeviceTensor.from_array(x) for n, x in of}
         if "k_scale" in s:
-            s["handles"]["cache"] = kk.KVCache(*(s["handles"][n] for n in ("k", "k_scale", "v", "v_scale")))
+            made["cache"] = kk.KVCache(*(made[n] for n in ("k", "k_scale", "v", "v_scale")))
+        s["handles"] = dict(made, of=of)
     return s["handles"]
 
 
@@ -345,6 +350,9 @@ def _back(t):
 
 def _own(s):
     kk = _kk()
+    kk.init(0)
+    if hasattr(kk, "use_stream"):  # torch's stream, so that a pass is in order with what torch does before and after it
+        kk.use_stream(torch.cuda.current_stream().cuda_stream)
     h = _handles(kk, s)
     ops, kind = kk.ops, s["kind"]
     if kind == "rotary":
