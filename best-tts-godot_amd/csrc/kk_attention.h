@@ -303,8 +303,8 @@ struct Part {
 // counter is that of the row reductions: stores that write through to where
 // all XCDs read, a wait for them, then the count; no whole cache is written
 // back.  Called by all threads, after a barrier; `weights` holds
-// 2 * chunks * rows floats.  False, with nothing put out, where a row's maximum is NaN: a part
-// that the caller has marked as not to be used.
+// 2 * chunks * rows floats.  False, with nothing put out, where there is one part
+// and its first maximum is NaN: the caller has marked it as not to be used.
 template <typename T, int THREADS>
 __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, const float* acc, int pitch,
                                          const float* m, const float* l, float* weights) {
@@ -313,7 +313,7 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
     const int64_t row = u.first + r, t = row / a.group, head = u.h * a.group + row % a.group;
     from_f32(static_cast<T*>(a.y)[u.b * a.ys[0] + t * a.ys[1] + head * a.ys[2] + d], v);
   };
-  __shared__ int shared;  // last to arrive; then: parts marked
+  __shared__ int last;  // of a row's blocks to arrive
   if (u.chunks == 1) {
     if (m[0] != m[0]) return false;
     if (D % 4 == 0) {
@@ -354,16 +354,11 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __syncthreads();
   if (threadIdx.x == 0)
-    shared = __hip_atomic_fetch_add(u.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.chunks - 1;
+    last = __hip_atomic_fetch_add(u.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.chunks - 1;
   __syncthreads();
-  if (!shared) return true;
+  if (!last) return true;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    shared = 0;
-    __hip_atomic_store(u.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
+  if (threadIdx.x == 0) __hip_atomic_store(u.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // weights[i][r] = 2^(m_i - max) / sum_i l_i 2^(m_i - max), from all parts' m and
   // l at once (one after the other, each would wait its whole way)
   float* sums = weights + u.chunks * rows;
@@ -376,13 +371,11 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
   for (int r = threadIdx.x / 64; r < rows; r += THREADS / 64) {  // a wave a row, a lane a part
     const int i = threadIdx.x % 64;
     const float mi = i < u.chunks ? weights[i * rows + r] : -INFINITY;
-    if (mi != mi) shared = 1;
     const float w = exp2f(mi - wave_max_dpp(mi));
     const float sum = wave_sum_dpp(i < u.chunks ? w * sums[i * rows + r] : 0.0f);
     if (i < u.chunks) weights[i * rows + r] = sum != 0.0f ? w / sum : 0.0f;
   }
   __syncthreads();
-  if (shared) return false;
   for (int i = threadIdx.x; i < rows * D; i += THREADS) {
     const int r = i / D, d = i - r * D;
     float sum = 0.0f;

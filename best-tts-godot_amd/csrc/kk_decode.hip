@@ -381,7 +381,6 @@ __global__ void __launch_bounds__(256) cache_values_kernel(const int8_t* k, cons
 // ------------------------------------------------------------------- logits
 struct LogitArgs {
   const void* x;
-  int x_dt;
   int64_t xs;
   float* y;
   int64_t ys;
@@ -717,7 +716,6 @@ int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_te
     a.allowed = static_cast<const int32_t*>(allowed->data);
   }
   a.x = logits->data;
-  a.x_dt = logits->dtype;
   a.y = static_cast<float*>(out->data);
   a.V = V;
   KK_TRY(require_ready());
