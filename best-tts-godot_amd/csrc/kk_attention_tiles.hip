@@ -582,6 +582,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
     }
 
     float by[G], vg[G], ev[G];  // of a group's tokens: score by, page scale, and its log2, rounded up
+    float largest = -INFINITY;  // of the tile's ev
     if constexpr (SRC == kPaged) {
       const uint32_t bits = __float_as_uint(__builtin_fabsf(vs));
       const bool finite = bits < 0x7f800000u;
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
         by[g] = cq * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), g));
         vg[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_v), g));
         ev[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_e), g));
+        largest = fmaxf(largest, ev[g]);
       }
       if (poisoned && (groups & static_cast<uint32_t>(__ballot(!finite)))) l = NAN;  // (lane g is of group g)
     }
@@ -646,20 +648,22 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[e] = seen >> (16 * j + e) & 1 ? s[e] : -INFINITY;
         }
-        float top = s[0], late = s[8];
+        float top = s[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) {
-          top = fmaxf(top, s[e]);
-          late = fmaxf(late, s[8 + e]);
-        }
-        float sized = -INFINITY;
-        if constexpr (SRC == kPaged) sized = fmaxf(top + ev[2 * j % G], late + ev[(2 * j + 1) % G]);
-        top = max_halves(fmaxf(top, late));
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+        top = max_halves(top);
         // m follows a row's maximum only where that is kSlack above it: weights are
         // 2^(x - m + 8) <= 2^15 (fp32: 2^(x - m - kSlack)), and few tiles scale the sums
         // again; so does mv
         if constexpr (SRC == kPaged) {
-          if (__any(top > m + kSlack || sized > mv + kSlack)) {
+          if (__any(top > fminf(m, mv - largest) + kSlack)) {  // (as if the largest score had the largest scale)
+            float early = s[0], late = s[8];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) {
+              early = fmaxf(early, s[e]);
+              late = fmaxf(late, s[8 + e]);
+            }
+            const float sized = fmaxf(early + ev[2 * j % G], late + ev[(2 * j + 1) % G]);
             top = fmaxf(ceilf(top), m);
             const float most = fmaxf(fmaxf(ceilf(max_halves(sized)), top - kLeastSize), mv);
             const float keep = __builtin_amdgcn_exp2f(mv - most);
