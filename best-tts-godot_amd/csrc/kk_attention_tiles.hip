@@ -54,9 +54,9 @@ __device__ __forceinline__ void split2(float x, float y, h2* hi, h2* lo) {
 }
 
 // Two values as the sums of three bf16 each, exactly (a part's rest is exact in
-// fp32): word p holds both values' parts p.  `rest` becomes NaN where a value is
-// not finite, or too large for bf16.
-__device__ __forceinline__ void split3(float x, float y, uint32_t (&word)[3], float* rest) {
+// fp32): word p holds both values' parts p.  Of a value that is not finite, or
+// too large for bf16, the second part is NaN.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&word)[3]) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -66,7 +66,6 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t (&word)[3], fl
     if (p == 2) break;
     x -= __uint_as_float(word[p] << 16);
     y -= __uint_as_float(word[p] & 0xffff0000u);
-    if (p == 0) *rest = __builtin_fmaf(x, 0.0f, __builtin_fmaf(y, 0.0f, *rest));
   }
 }
 
@@ -93,12 +92,12 @@ __device__ __forceinline__ f16v product_of_parts(const h8 (&a)[PA], const h8 (&b
 }
 
 // Eight values as fragments of their three parts.
-__device__ __forceinline__ void split3(const float (&x)[8], h8 (&to)[3], float* rest) {
+__device__ __forceinline__ void split3(const float (&x)[8], h8 (&to)[3]) {
   u4 part[3];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     uint32_t word[3];
-    split3(x[i], x[i + 1], word, rest);
+    split3(x[i], x[i + 1], word);
 #pragma unroll
     for (int p = 0; p < 3; ++p) part[p][i / 2] = word[p];
   }
@@ -157,9 +156,9 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // values of 128 take 36 KB, so that two blocks a CU overlap one's loads with the
 // other's products; 256 queries a block, for half the loads, gave 256 and 86 us.
 //
-// A state that is not finite poisons whole sums here (0 times it is NaN) where
-// only queries that see it should be: a block that meets one marks its part, and
-// its queries are formed one by one.
+// A state that is not finite poisons the sums of all queries here (0 times it is
+// NaN) where only queries that see it should be: a block whose sums are not finite
+// marks its part, and its queries are formed one by one.
 template <typename T, class Rows, int SRC, int DT, int TT, bool WIDE>
 __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2 : sizeof(T) == 4 ? 3 : 4) ? 2 : 1)
     attention_tile_kernel(QueryArgs a, Rows rows, TileCut cut) {
@@ -247,9 +246,8 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
         for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(x[s][i]));
       }
       if constexpr (SRC == kFloat) {
-        float unused = 0.0f;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) split3(x[s], qf[s], &unused);
+        for (int s = 0; s < KS; ++s) split3(x[s], qf[s]);
       } else {
         top = max_halves(top);
         const int up = 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
@@ -424,9 +422,6 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       }
     }
   };
-  // of values that are not finite: half: bit 15 or 31; fp32: NaN
-  uint32_t bad = 0;
-  float rest = 0.0f;
   float m = -3.4028235e38f, l = 0.0f;
   // paged: log2 of the largest weight times page scale that the query has met (a
   // whole number, as m is there; kLeastSize below m at the least), and 2^(m - mv + 8)
@@ -456,8 +451,6 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
       for (int i = 0; i < UK; ++i) {
         const int u = key_unit(i), tk = u / (4 * DT), c = u % (4 * DT);
         *reinterpret_cast<u4*>(lds_k + row_of(tk) * KP + 16 * c) = ck[i];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= (ck[i][e] & 0x7c007c00u) + 0x04000400u;
       }
 #pragma unroll
       for (int i = 0; i < UV; ++i) {
@@ -470,10 +463,6 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
                         __builtin_amdgcn_perm(cv[(4 * i + 3) % (4 * UV)][e / 2], cv[(4 * i + 2) % (4 * UV)][e / 2], sel)};
           *reinterpret_cast<u2*>(lds_v + (d + e) * VP + 2 * tk) = w;
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bad |= (cv[(4 * i + j) % (4 * UV)][e] & 0x7c007c00u) + 0x04000400u;
       }
     } else {
 #pragma unroll
@@ -483,7 +472,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
         h8 part[3];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(ck[(2 * i + e / 4) % (2 * UK)][e % 4]);
-        split3(x, part, &rest);
+        split3(x, part);
 #pragma unroll
         for (int p = 0; p < 3; ++p)
           *reinterpret_cast<h8*>(lds_k + (p * TT + row_of(tk)) * KP + 16 * c) = part[p];
@@ -499,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
           for (int j = 0; j < 4; j += 2) {
             uint32_t word[3];
             split3(__uint_as_float(cv[(4 * i + j) % (4 * UV)][e]),
-                   __uint_as_float(cv[(4 * i + j + 1) % (4 * UV)][e]), word, &rest);
+                   __uint_as_float(cv[(4 * i + j + 1) % (4 * UV)][e]), word);
 #pragma unroll
             for (int p = 0; p < 3; ++p) part[p][j / 2] = word[p];
           }
@@ -702,8 +691,7 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
             for (int e = 0; e < 8; ++e) w[e] *= vw;
           }
           if constexpr (SRC == kFloat) {
-            float unused = 0.0f;
-            split3(w, pf[k], &unused);
+            split3(w, pf[k]);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -734,7 +722,16 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
   }
 
   // the sums by rows, half of them at a time, in LDS
-  const bool marked = __syncthreads_or(SRC == kHalf ? (bad & 0x80008000u) != 0 : rest != rest);
+  bool marked = false;
+  if constexpr (SRC != kPaged) {
+    float any = l * 0.0f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) any = __builtin_fmaf(acc[i][e], 0.0f, any);
+    marked = any != any;
+  }
+  marked = __syncthreads_or(marked);
   const int pitch = D + 4;
   float* sums = reinterpret_cast<float*>(tile_lds);
   float* wm = sums + kPutRows * pitch;
