@@ -563,9 +563,10 @@ int kk_qk_norm_rotary(const kk_tensor* out_q, const kk_tensor* out_k, const kk_t
   // sixteen-byte chunks where both chunks of a lane are whole and aligned
   const int vec = q->dtype == KK_F16 ? 8 : 4;
   wide = wide && D % (2 * vec) == 0 && (2 * a.half) % (2 * vec) == 0;
-  // outputs beyond what the caches hold go past them: 168 MB of fp16 82 us
-  // through them and 65 past them, 31 MB of fp32 15 and 22
-  const bool stream = B * T * (a.heads[0] + a.heads[1]) * D * dtype_size(q->dtype) > int64_t{128} << 20;
+  // outputs beyond what the caches hold go past them (32 + 8 heads of 128 in fp16,
+  // through the caches and past them: 112 MB 53 and 55 us, 144 MB 62 and 66, 168 MB
+  // 83 and 79, 256 MB 116 and 111; fp32 144 MB 56 and 61, 256 MB 110 and 107)
+  const bool stream = B * T * (a.heads[0] + a.heads[1]) * D * dtype_size(q->dtype) > int64_t{152} << 20;
   if (q->dtype == KK_F16)
     return !wide    ? launch_rotary<__half, 1, 2>(a, B * T)
            : stream ? launch_rotary<__half, 8, 1, true>(a, B * T)

@@ -269,7 +269,8 @@ class DeviceTensor:
         wait_stream again.  A torch array's memory goes back to torch when the
         tensor and the array are dropped, in the order of torch's current
         stream; other libraries' must be kept until libkk has used it (sync
-        or signal_stream)."""
+        or signal_stream).  Import torch before libkk is first used, so that
+        both run on the same HIP runtime."""
         desc = arr.__cuda_array_interface__
         dtype = np.dtype(desc["typestr"])
         if dtype not in NP_TO_CODE:
