@@ -142,15 +142,17 @@ __device__ __forceinline__ uint64_t query_mask(const Rows& rows, const QueryArgs
 // its page's scale, over a power of two of the largest such product that the query
 // has met: by what it weighs, not by what it sees, so that a page of large scale
 // without weight takes no bits from the others.  Weights of fp16 queries are rounded
-// to fp16 (half a step of the output's type); that they are 2^8 times as large keeps
-// 32 bits between the largest and fp16's smallest value.
+// to fp16 (half a step of the output's type; in two halves the chunk below takes 315
+// us).  They are 2^8 times as large, so that one below 2^-22 of the largest keeps
+// 2^-33 of that: over states, an error below half of fp16's smallest step for
+// values up to 256.
 //
 // Bound by the vector units beside the products: 32 x 64 scores a wave take some
 // 300 vector instructions for their softmax against 32 (fp16, 128 values) or 96
 // (fp32, 64) products, bringing a tile 120 (codes), 30 (fp16) or 220 (fp32) a
-// wave.  2 x 1531 queries of 32 heads of 128 over up to 4099 cached tokens: 257
-// us, 452 TFLOP/s; 2 x 3000 over 1500 fp16 states: 160 us, 690 TFLOP/s; 2 x 3380
-// of 12 heads of 64 over up to 509 fp32 states: 71 us (67 in two halves beside the
+// wave.  2 x 1531 queries of 32 heads of 128 over up to 4099 cached tokens: 255
+// us, 455 TFLOP/s; 2 x 3000 over 1500 fp16 states: 220 us, 669 TFLOP/s; 2 x 3380
+// of 12 heads of 64 over up to 509 fp32 states: 73 us (67 to 69 in two halves beside the
 // block's largest row, which lost rows that a query weighs beside a large one that
 // it does not; heads of 80 and 96 take a tenth less than so, of 128 a twentieth).  64 tokens a tile: keys and
 // values of 128 take 36 KB, so that two blocks a CU overlap one's loads with the

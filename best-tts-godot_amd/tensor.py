@@ -289,7 +289,7 @@ class DeviceTensor:
         if stream is not None:
             wait_stream(stream)
         elif _is_torch(arr):
-            if arr.device.index != init():
+            if arr.device.index != init(arr.device.index):
                 raise ValueError(f"an array on {arr.device}: libkk is on device {init()}")
             _order("kk_stream_wait")
         t = cls(Borrowed(int(desc["data"][0] or 0), math.prod(shape) * dtype.itemsize, arr), shape, dtype, strides)
