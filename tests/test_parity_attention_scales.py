@@ -167,3 +167,25 @@ def test_channels_of_mixed_sizes_keep_their_own_bits(gpu, T):
         share = p @ off + (S / 16 + 16) * U
         tol = (p * off) @ np.abs(v64[:, 0]) + 2 * share * (p @ np.abs(v64[:, 0]))
         within(out[0, i, 0], p @ v64[:, 0], tol, f"query {i}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,by_query", [(1, False), (5, False), (40, False), (40, True), (200, True)])
+def test_an_infinite_key_weighs_nothing_where_its_score_is_minus_infinity(gpu, t, T, by_query):
+    """One value of one key is infinite: queries whose own value there is negative do as if it were not there, the
+    others have no softmax."""
+    kk = gpu
+    r = rng(T)
+    S, dim = 150, 64
+    q = r.normal(size=(1, T, 1, dim)).astype(t)
+    q[0, ::2, 0, 7] = -np.abs(q[0, ::2, 0, 7]) - t(0.1)
+    q[0, 1::2, 0, 7] = np.abs(q[0, 1::2, 0, 7]) + t(0.1)
+    k, v = (r.normal(size=(1, S, 1, dim)).astype(t) for _ in range(2))
+    k[0, 100, 0, 7] = np.inf
+    mask = r.random((1, T, S)) < 0.8 if by_query else np.ones((1, T, S), bool)
+    mask[0, :, 100] = True
+    out = run_states(kk, q, k, v, mask if by_query else None, 0.3)
+    at = np.arange(0, T, 2)
+    k[0, 100] = 0
+    check(out[0][at], q[0][at], k[0], v[0], lambda i: [j for j in np.flatnonzero(mask[0, at[i]]) if j != 100], 0.3)
+    assert np.isnan(out[0, 1::2]).all()
