@@ -14,8 +14,8 @@ from .dispatch import dispatch, to_device, to_host  # noqa: F401
 from .tensor import (DeviceTensor, device_count, dispatch_count, init, pool_stats,  # noqa: F401
                      pool_trim, signal_stream, sync, use_stream, wait_stream)
 from . import ops  # noqa: F401
-from .cache import KVCache, allowed_bits, rotary_turns  # noqa: F401
+from .cache import KVCache, KVCache4, allowed_bits, rotary_turns  # noqa: F401
 
 __all__ = ["dispatch", "to_device", "to_host", "DeviceTensor", "init", "sync",
            "pool_stats", "pool_trim", "device_count", "dispatch_count", "ops", "wait_stream",
-           "signal_stream", "use_stream", "KVCache", "rotary_turns", "allowed_bits"]
+           "signal_stream", "use_stream", "KVCache", "KVCache4", "rotary_turns", "allowed_bits"]

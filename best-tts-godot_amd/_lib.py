@@ -126,6 +126,14 @@ PROTOTYPES = {
     "kk_cache_attention": [_T] * 9 + [_f, ctypes.c_int64],
     "kk_cross_attention": [_T] * 6 + [_f],
     "kk_process_logits": [_T] * 9,
+    "kk_rms_norm": [_T] * 5 + [_f],
+    "kk_rms_norm_quant": [_T] * 6 + [_f],
+    "kk_plan_pages": [_T] * 10 + [ctypes.c_int64],
+    "kk_release_pages": [_T] * 5 + [ctypes.c_int64],
+    "kk_cache4_append": [_T] * 7,
+    "kk_cache4_values": [_T] * 6,
+    "kk_cache4_attention": [_T] * 9 + [_f, ctypes.c_int64],
+    "kk_sample": [_T] * 8,
     "kk_stream_wait": [_vp],
     "kk_stream_signal": [_vp],
     "kk_stream": [ctypes.POINTER(_vp)],

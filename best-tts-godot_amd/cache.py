@@ -1,5 +1,5 @@
-"""What a token decoder's program keeps: the paged cache of 8-bit keys and
-values, the table of its rotation, a grammar's mask as bits."""
+"""What a token decoder's program keeps: the paged caches of 8-bit and 4-bit
+keys and values, the table of its rotation, a grammar's mask as bits."""
 import math
 
 import numpy as np
@@ -42,6 +42,43 @@ class KVCache:
         """What the codes stand for, as float32: keys [pages, heads, block, D]
         and values [pages, heads, D, block]."""
         return ops.cache_values(self)
+
+
+class KVCache4:
+    """Keys and values of one layer in 4 bits, two codes a byte, in pages of
+    `block` tokens with a step and a lowest value (fp16) for each token and head
+    (include/kk.h, kk_cache4_append): half the memory of a KVCache.  Which slots
+    a sequence's tokens have is the program's to keep (ops.plan_pages)."""
+
+    __slots__ = ("k", "k_scale", "v", "v_scale")
+
+    def __init__(self, k, k_scale, v, v_scale):
+        pages, heads, block, half = k.shape
+        if block not in BLOCKS:
+            raise ValueError(f"pages of {block} tokens (one of {BLOCKS})")
+        if half % 16 or not 16 <= half <= 128:
+            raise ValueError(f"heads of {2 * half} values (32 to 256 in steps of 32)")
+        if v.shape != (pages, heads, half, block):
+            raise ValueError(f"values {v.shape} do not fit keys {k.shape}")
+        if k_scale.shape != (pages, heads, block, 2) or v_scale.shape != (pages, heads, block, 2):
+            raise ValueError(f"scales {k_scale.shape}, {v_scale.shape} do not fit keys {k.shape}")
+        if k.dtype != np.uint8 or v.dtype != np.uint8 or k_scale.dtype != np.float16 or v_scale.dtype != np.float16:
+            raise TypeError("codes are uint8, scales float16")
+        self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
+
+    @classmethod
+    def zeros(cls, pages, heads, dim, block=64):
+        """An empty cache."""
+        pages, heads, half, block = int(pages), int(heads), int(dim) // 2, int(block)
+        if int(dim) % 32:
+            raise ValueError(f"heads of {int(dim)} values (32 to 256 in steps of 32)")
+        return cls(ops.fill((pages, heads, block, half), 0, np.uint8), ops.fill((pages, heads, block, 2), 0, np.float16),
+                   ops.fill((pages, heads, half, block), 0, np.uint8), ops.fill((pages, heads, block, 2), 0, np.float16))
+
+    def values(self):
+        """What the codes stand for, as float32: keys [pages, heads, block, D]
+        and values [pages, heads, D, block]."""
+        return ops.cache4_values(self)
 
 
 def rotary_turns(dim, base=10000.0, factor=1.0, old_length=None, low=1.0, high=4.0):

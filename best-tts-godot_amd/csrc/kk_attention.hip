@@ -1,6 +1,6 @@
 // Attention of a token decoder: over a paged cache of 8-bit codes, and over
 // an encoder's states.
-#include "kk_attention.h"
+#include "kk_attention4.h"
 
 namespace kk {
 
@@ -56,6 +56,31 @@ static int check_queries(const kk_tensor* out, const kk_tensor* q, int64_t key_h
   return KK_OK;
 }
 
+// What an attention over a paged cache takes of its table, lengths and counts.
+static int check_places(const kk_tensor* table, const kk_tensor* lengths, const kk_tensor* counts, int64_t window,
+                        const CacheShape& c, int64_t B, PagedArgs* p, const char* who) {
+  if (table->shape[0] != B) return set_error(KK_E_ARG, "%s: table must have a row a sequence", who);
+  KK_TRY(check_per_row(lengths, "lengths", B, true, who));
+  if (counts) KK_TRY(check_per_row(counts, "counts", B, true, who));
+  if (window < 0) return set_error(KK_E_ARG, "%s: window must not be negative", who);
+  p->table = static_cast<const int32_t*>(table->data);
+  p->table_stride = c.table_stride;
+  p->pages = c.pages;
+  p->columns = c.columns;
+  p->lengths = lengths->data;
+  p->lengths_dt = lengths->dtype;
+  p->lengths_st = row_stride(lengths);
+  if (counts) {
+    p->counts = counts->data;
+    p->counts_dt = counts->dtype;
+    p->counts_st = row_stride(counts);
+  }
+  p->window = window;
+  p->heads = static_cast<int>(c.heads);
+  p->block = static_cast<int>(c.block);
+  return KK_OK;
+}
+
 }  // namespace kk
 
 using namespace kk;
@@ -71,35 +96,40 @@ int kk_cache_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor
   KK_TRY(check_cache(k_codes, k_scales, v_codes, v_scales, table, &c, who));
   QueryArgs a{};
   KK_TRY(check_queries(out, q, c.heads, c.D, scale, &a, who));
-  if (table->shape[0] != a.B) return set_error(KK_E_ARG, "%s: table must have a row a sequence", who);
-  KK_TRY(check_per_row(lengths, "lengths", a.B, true, who));
-  if (counts) KK_TRY(check_per_row(counts, "counts", a.B, true, who));
-  if (window < 0) return set_error(KK_E_ARG, "%s: window must not be negative", who);
   PagedArgs p{};
+  KK_TRY(check_places(table, lengths, counts, window, c, a.B, &p, who));
   p.k = static_cast<const int8_t*>(k_codes->data);
   p.v = static_cast<const int8_t*>(v_codes->data);
   p.k_scale = static_cast<const float*>(k_scales->data);
   p.v_scale = static_cast<const float*>(v_scales->data);
-  p.table = static_cast<const int32_t*>(table->data);
-  p.table_stride = c.table_stride;
-  p.pages = c.pages;
-  p.columns = c.columns;
-  p.lengths = lengths->data;
-  p.lengths_dt = lengths->dtype;
-  p.lengths_st = row_stride(lengths);
-  if (counts) {
-    p.counts = counts->data;
-    p.counts_dt = counts->dtype;
-    p.counts_st = row_stride(counts);
-  }
-  p.window = window;
-  p.heads = static_cast<int>(c.heads);
-  p.block = static_cast<int>(c.block);
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
   int status = KK_OK;
   if (few_paged_try(a, p, q->dtype, &status) || tiles_paged_try(a, p, q->dtype, &status)) return status;
   const PagedRows rows{p, a.T, a.D};
+  return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
+}
+
+int kk_cache4_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k_codes,
+                        const kk_tensor* k_scales, const kk_tensor* v_codes, const kk_tensor* v_scales,
+                        const kk_tensor* table, const kk_tensor* lengths, const kk_tensor* counts, float scale,
+                        int64_t window) {
+  const char* who = "cache4_attention";
+  CacheShape c;
+  KK_TRY(check_codes4(k_codes, k_scales, v_codes, v_scales, &c, who));
+  KK_TRY(check_cache_table(table, &c, who));
+  QueryArgs a{};
+  KK_TRY(check_queries(out, q, c.heads, c.D, scale, &a, who));
+  Paged4Rows rows{};
+  KK_TRY(check_places(table, lengths, counts, window, c, a.B, &rows.a, who));
+  rows.T = a.T;
+  rows.D = a.D;
+  rows.k = static_cast<const uint8_t*>(k_codes->data);
+  rows.v = static_cast<const uint8_t*>(v_codes->data);
+  rows.k_scale = static_cast<const uint32_t*>(k_scales->data);
+  rows.v_scale = static_cast<const uint32_t*>(v_scales->data);
+  KK_TRY(require_ready());
+  if (a.B * a.T * a.heads == 0) return KK_OK;
   return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
 }
 

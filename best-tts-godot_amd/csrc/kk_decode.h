@@ -102,10 +102,8 @@ inline int check_codes(const kk_tensor* k_codes, const kk_tensor* k_scales, cons
   return KK_OK;
 }
 
-// The same with a table of its pages.
-inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
-                       const kk_tensor* v_scales, const kk_tensor* table, CacheShape* c, const char* who) {
-  KK_TRY(check_codes(k_codes, k_scales, v_codes, v_scales, c, who));
+// A table of a cache's pages.
+inline int check_cache_table(const kk_tensor* table, CacheShape* c, const char* who) {
   KK_TRY(check_tensor(table, "table"));
   if (table->dtype != KK_I32 || table->rank != 2)
     return set_error(KK_E_ARG, "%s: table must be int32 [sequences, pages]", who);
@@ -115,6 +113,53 @@ inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, cons
   if (c->columns > 1 && table->shape[0] > 0 && table->strides[1] != 1)
     return set_error(KK_E_ARG, "%s: a row of table must lie in one piece", who);
   c->table_stride = table->shape[0] > 1 ? table->strides[0] : 0;
+  return KK_OK;
+}
+
+// The same with a table of its pages.
+inline int check_cache(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                       const kk_tensor* v_scales, const kk_tensor* table, CacheShape* c, const char* who) {
+  KK_TRY(check_codes(k_codes, k_scales, v_codes, v_scales, c, who));
+  return check_cache_table(table, c, who);
+}
+
+// A paged cache of 4-bit codes, two a byte, with a step and a lowest value for
+// each token and head.
+inline int check_codes4(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                        const kk_tensor* v_scales, CacheShape* c, const char* who) {
+  const kk_tensor *codes[2] = {k_codes, v_codes}, *scales[2] = {k_scales, v_scales};
+  const char *names[2] = {"k_codes", "v_codes"}, *snames[2] = {"k_scales", "v_scales"};
+  for (int i = 0; i < 2; ++i) {
+    KK_TRY(check_tensor(codes[i], names[i]));
+    KK_TRY(check_tensor(scales[i], snames[i]));
+    if (codes[i]->dtype != KK_U8 || codes[i]->rank != 4 || !is_contiguous(codes[i]) ||
+        reinterpret_cast<uintptr_t>(codes[i]->data) % 16)
+      return set_error(KK_E_ARG, "%s: %s must be uint8 of four axes in one piece, 16-byte aligned", who, names[i]);
+  }
+  c->pages = k_codes->shape[0];
+  c->heads = k_codes->shape[1];
+  c->block = k_codes->shape[2];
+  c->D = 2 * k_codes->shape[3];
+  if (v_codes->shape[0] != c->pages || v_codes->shape[1] != c->heads || v_codes->shape[2] != c->D / 2 ||
+      v_codes->shape[3] != c->block)
+    return set_error(KK_E_ARG, "%s: v_codes must be [pages, heads, values / 2, rows] of k_codes' [pages, heads, rows, "
+                     "values / 2]", who);
+  for (int i = 0; i < 2; ++i)
+    if (scales[i]->dtype != KK_F16 || scales[i]->rank != 4 || !is_contiguous(scales[i]) ||
+        scales[i]->shape[0] != c->pages || scales[i]->shape[1] != c->heads || scales[i]->shape[2] != c->block ||
+        scales[i]->shape[3] != 2 || reinterpret_cast<uintptr_t>(scales[i]->data) % 16)
+      return set_error(KK_E_ARG, "%s: %s must be f16 [pages, heads, rows, 2] in one piece, 16-byte aligned", who,
+                       snames[i]);
+  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128 && c->block != 256)
+    return set_error(KK_E_UNSUPPORTED, "%s: pages of %lld rows (16, 32, 64, 128 or 256)", who,
+                     static_cast<long long>(c->block));
+  if (c->D < 32 || c->D > 256 || c->D % 32)
+    return set_error(KK_E_UNSUPPORTED, "%s: heads of %lld values (32 to 256 in steps of 32)", who,
+                     static_cast<long long>(c->D));
+  if (c->heads < 1 || c->heads > 65535) return set_error(KK_E_UNSUPPORTED, "%s: %lld heads", who,
+                                                         static_cast<long long>(c->heads));
+  if (c->pages > 0x7fffffff) return set_error(KK_E_UNSUPPORTED, "%s: too many pages", who);
+  c->columns = c->table_stride = 0;
   return KK_OK;
 }
 

@@ -572,7 +572,7 @@ def fir_pcm16(x, taps, center=-1, gain=1.0):
 
 
 # ------------------------------------------------------------ token decoder
-_F32 = np.dtype(np.float32)
+_F32, _I8, _I32, _I64 = (np.dtype(t) for t in (np.float32, np.int8, np.int32, np.int64))
 
 
 # (a copy that _inner or _flat makes must be held until the call: its buffer goes back to the pool with it)
@@ -583,6 +583,15 @@ def _inner(t):
 
 def _flat(t):
     return None if t is None else t.contiguous()
+
+
+def _rows(t):
+    """t as rows that are evenly spaced, each in one piece."""
+    if t is None or t.is_contiguous():
+        return t
+    step = [(n, st) for n, st in zip(t.shape[:-1], t.strides[:-1]) if n != 1]
+    even = all(a[1] == b[0] * b[1] for a, b in zip(step, step[1:]))
+    return t if even and (t.shape[-1] == 1 or t.strides[-1] == 1) else t.contiguous()
 
 
 def qk_norm_rotary(q, k, positions=None, turns=None, q_weight=None, k_weight=None, eps=1e-6,
@@ -654,3 +663,88 @@ def process_logits(logits, history=None, history_lengths=None, repetition=None, 
     _lib.call("kk_process_logits", out.desc(), logits.desc(), _d(history), _d(history_lengths), _d(repetition),
               _d(presence), _d(frequency), _d(bias), _d(allowed))
     return out
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """The root-mean-square norm of the rows of x [.., N] times weight [N], of
+    x's dtype; with a residual, (the norm of x + residual, x + residual)."""
+    x, residual, weight = _rows(x), _rows(residual), _flat(weight)
+    out = DeviceTensor._fresh(x.shape, x.dtype)
+    total = None if residual is None else DeviceTensor._fresh(residual.shape, residual.dtype)
+    _lib.call("kk_rms_norm", out.desc(), _d(total), x.desc(), _d(residual), _d(weight), float(eps))
+    return out if total is None else (out, total)
+
+
+def rms_norm_quant(x, weight=None, residual=None, eps=1e-6):
+    """(codes int8 [.., N], scales float32 [.., 1]) of rms_norm's rows, ahead of
+    an 8-bit product (`matmul_integer_scaled`, its rows times the scales); with a
+    residual, (codes, scales, x + residual)."""
+    x, residual, weight = _rows(x), _rows(residual), _flat(weight)
+    codes = DeviceTensor._fresh(x.shape, _I8)
+    scales = DeviceTensor._fresh(x.shape[:-1] + (1,), _F32)
+    total = None if residual is None else DeviceTensor._fresh(residual.shape, residual.dtype)
+    _lib.call("kk_rms_norm_quant", codes.desc(), scales.desc(), _d(total), x.desc(), _d(residual), _d(weight),
+              float(eps))
+    return (codes, scales) if total is None else (codes, scales, total)
+
+
+def plan_pages(table, starts, counts, free, used, tokens, block, used_out=None):
+    """Pages for the counts[b] (None: `tokens`) new tokens of sequences that
+    hold starts[b], from free[used[0]:], into table [B, columns] (in place), and
+    the tokens' places: (slots [B, tokens], positions [B, tokens], lengths [B],
+    granted [B], used [1]).  A sequence for whose tokens there are no pages is
+    granted none.  The new `used` is a tensor of its own, or used_out (which may
+    be `used`)."""
+    shape = (table.shape[0], int(tokens))
+    slots, positions = DeviceTensor._fresh(shape, _I64), DeviceTensor._fresh(shape, _I32)
+    lengths, granted = DeviceTensor._fresh(shape[:1], _I32), DeviceTensor._fresh(shape[:1], _I32)
+    used_out = DeviceTensor._fresh((1,), _I32) if used_out is None else used_out
+    _lib.call("kk_plan_pages", table.desc(), slots.desc(), positions.desc(), lengths.desc(), granted.desc(),
+              used_out.desc(), starts.desc(), _d(counts), free.desc(), used.desc(), int(block))
+    return slots, positions, lengths, granted, used_out
+
+
+def release_pages(table, lengths, ended, free, used, block):
+    """Takes the pages of the sequences with ended[b] (bool) back: table, free
+    and used in place."""
+    _lib.call("kk_release_pages", table.desc(), lengths.desc(), ended.desc(), free.desc(), used.desc(), int(block))
+
+
+def cache4_append(cache, k, v, slots):
+    """Keys and values [B, T, Hk, D] into the slots [B, T] (page * block + row,
+    -1: left out) of a KVCache4."""
+    k, v = _inner(k), _inner(v)
+    _lib.call("kk_cache4_append", cache.k.desc(), cache.k_scale.desc(), cache.v.desc(), cache.v_scale.desc(),
+              k.desc(), v.desc(), slots.desc())
+
+
+def cache4_values(cache):
+    """(keys [pages, Hk, block, D], values [pages, Hk, D, block]) of a KVCache4 as float32."""
+    pages, heads, block, half = cache.k.shape
+    k = DeviceTensor._fresh((pages, heads, block, 2 * half), _F32)
+    v = DeviceTensor._fresh((pages, heads, 2 * half, block), _F32)
+    _lib.call("kk_cache4_values", k.desc(), v.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
+              cache.v_scale.desc())
+    return k, v
+
+
+def cache4_attention(q, cache, table, lengths, counts=None, scale=None, window=0):
+    """cache_attention over a KVCache4."""
+    q, table = _inner(q), _inner(table)
+    out = DeviceTensor._fresh(q.shape, q.dtype)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _lib.call("kk_cache4_attention", out.desc(), q.desc(), cache.k.desc(), cache.k_scale.desc(), cache.v.desc(),
+              cache.v_scale.desc(), table.desc(), lengths.desc(), _d(counts), scale, int(window))
+    return out
+
+
+def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(tokens int32 [B], their log-probabilities float32 [B]) drawn from logits
+    [B, V] with the given numbers uniforms [B] in [0, 1) (include/kk.h,
+    kk_sample); a temperature of 0 takes the largest logit."""
+    logits = _inner(logits)
+    tokens = DeviceTensor._fresh(logits.shape[:1], _I32)
+    logs = DeviceTensor._fresh(logits.shape[:1], _F32)
+    _lib.call("kk_sample", tokens.desc(), logs.desc(), logits.desc(), uniforms.desc(), _d(temperature), _d(top_k),
+              _d(top_p), _d(min_p))
+    return tokens, logs

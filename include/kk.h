@@ -567,6 +567,97 @@ int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_te
                       const kk_tensor* presence, const kk_tensor* frequency, const kk_tensor* bias,
                       const kk_tensor* allowed);
 
+/* Root-mean-square norm of rows with the residual's addition in the same pass:
+ *   h = x + residual (residual NULL: h = x);   sum = h where sum is given
+ *   y = h / sqrt(mean(h^2) + eps) * weight     (weight [N]; NULL: 1)
+ * x, residual, out and sum [.., N], f32 or f16 each (sum of residual's dtype), rows
+ * evenly spaced, a row's values next to each other, 1 <= N <= 16384; the norm is
+ * that of h before it is rounded to sum's dtype.  out and sum may each be x or
+ * residual itself, but not both the same. */
+int kk_rms_norm(const kk_tensor* out, const kk_tensor* sum, const kk_tensor* x,
+                const kk_tensor* residual, const kk_tensor* weight, float eps);
+/* The same into 8 bits for kk_matmul_integer_scaled, with a scale for each row:
+ * scales f32 [rows], codes int8 like x,
+ *   scale = max |y| / 127,   code = rint(y / scale)  (a row of zeros: 0 and 0)
+ * of the exact quotient, ties to even.  A row that is not finite has the scale NaN. */
+int kk_rms_norm_quant(const kk_tensor* codes, const kk_tensor* scales, const kk_tensor* sum,
+                      const kk_tensor* x, const kk_tensor* residual, const kk_tensor* weight,
+                      float eps);
+
+/* Pages of `block` tokens (16, 32, 64, 128 or 256) for the new tokens of B
+ * sequences, and where the tokens go.  Sequence b holds starts[b] tokens in its row
+ * of `table` [B, columns] and gets counts[b] more (NULL: T each; at most T; starts
+ * and counts int32 or int64 [B] or [1]).  The pages that it lacks are taken in
+ * the sequences' order from free[*used ..] (int32 [F]) and put into the table behind
+ * those it has.  Where a sequence needs more than are left then, or where it would
+ * pass the table's columns, it gets none of its tokens; nor do, of the sequences
+ * behind one that lacked pages, those that need pages themselves.  Writes
+ *   granted [B]       counts[b], or 0             lengths [B]  starts[b] + granted[b]
+ *   slots [B, T]      page * block + row of each new token, -1 past granted[b] and
+ *                     where the page is negative
+ *   positions [B, T]  starts[b] + t, -1 past granted[b]
+ *   used_out [1]      *used and the pages taken (may be `used` itself)
+ * all int32 but slots (int64).  A start outside the table makes its sequence empty.
+ * lengths and granted must not be starts or counts. */
+int kk_plan_pages(const kk_tensor* table, const kk_tensor* slots, const kk_tensor* positions,
+                  const kk_tensor* lengths, const kk_tensor* granted, const kk_tensor* used_out,
+                  const kk_tensor* starts, const kk_tensor* counts, const kk_tensor* free,
+                  const kk_tensor* used, int64_t block);
+/* Takes back the pages of sequences b with ended[b] (bool [B]): the entries that are not
+ * negative of the columns that lengths[b] tokens reach, in the order of sequences and
+ * columns, come before the free ones: *used falls by their number n (not below 0:
+ * what passes that is dropped), free[*used ..] holds them.  Their entries become -1. */
+int kk_release_pages(const kk_tensor* table, const kk_tensor* lengths, const kk_tensor* ended,
+                     const kk_tensor* free, const kk_tensor* used, int64_t block);
+
+/* A cache of keys and values in 4 bits: pages of `block` tokens (16, 32, 64, 128
+ * or 256) with a step and a lowest value for each token and head, a value being
+ * low + step * code, code 0 to 15.
+ *   k_codes uint8 [pages, Hk, block, D / 2]   v_codes uint8 [pages, Hk, D / 2, block]
+ *   k_scales, v_scales f16 [pages, Hk, block, 2]: step, low
+ *   D 32 to 256 in steps of 32
+ * Byte i of a token holds the codes of its values i (low four bits) and i + D / 2.
+ * Slot s is row s % block of page s / block.
+ *
+ * kk_cache4_append puts the tokens of k and v [B, T, Hk, D] into slots [B, T] (int32
+ * or int64); slots outside the pool are left out, and no slot may come twice in a
+ * call.  With x taken as 0 where it is NaN and within +-65504,
+ *   low = min x in fp16,   step = (max x - low) / 15, to fp32 and then fp16,
+ *   code = rint((x - low) / step), of the exact quotient, ties to even, 0 to 15
+ * (a step of 0: all codes 0). */
+int kk_cache4_append(const kk_tensor* k_codes, const kk_tensor* k_scales, const kk_tensor* v_codes,
+                     const kk_tensor* v_scales, const kk_tensor* k, const kk_tensor* v,
+                     const kk_tensor* slots);
+/* What the codes of such a cache stand for: out_k f32 [pages, Hk, block, D] and out_v
+ * f32 [pages, Hk, D, block], in one piece and 16-byte aligned. */
+int kk_cache4_values(const kk_tensor* out_k, const kk_tensor* out_v, const kk_tensor* k_codes,
+                     const kk_tensor* k_scales, const kk_tensor* v_codes,
+                     const kk_tensor* v_scales);
+/* kk_cache_attention over such a cache. */
+int kk_cache4_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k_codes,
+                        const kk_tensor* k_scales, const kk_tensor* v_codes,
+                        const kk_tensor* v_scales, const kk_tensor* table,
+                        const kk_tensor* lengths, const kk_tensor* counts, float scale,
+                        int64_t window);
+
+/* A token from each row of logits [B, V] (f32 or f16, V <= 131072), with a
+ * given number uniforms[b] in [0, 1).  In order (larger logits first, equal ones
+ * by index) the tokens weigh w = exp((x - max) / temperature[b]); of them are kept
+ *   the first top_k[b]                                      (0 and less: all)
+ *   those before which less than top_p[b] of the weight kept so far comes
+ *                                                           (1 and more: all)
+ *   those with w >= min_p[b]                                (0 and less: all)
+ * and tokens[b] (int32) is the first whose running weight passes uniforms[b] times
+ * that of all kept; logs[b] (f32, may be NULL) the logarithm of its share of it.
+ * A temperature that is not above 0 takes the largest logit (the first of equal
+ * ones).  -inf and NaN are never drawn; a row without another logit gives the token
+ * -1 and the logarithm -inf; +inf outweighs all else.  uniforms, temperature, top_p
+ * and min_p f32, top_k int32 or int64, [B] or [1]; all but uniforms may be NULL (1,
+ * no limits). */
+int kk_sample(const kk_tensor* tokens, const kk_tensor* logs, const kk_tensor* logits,
+              const kk_tensor* uniforms, const kk_tensor* temperature, const kk_tensor* top_k,
+              const kk_tensor* top_p, const kk_tensor* min_p);
+
 /* -------------------------------------------------------------- timing
  * HIP events on the library stream, for measuring kernels where they run.
  * Slots 0..KK_MAX_EVENTS-1.  No counterpart in the reference, which has no
