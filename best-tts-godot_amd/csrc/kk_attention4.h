@@ -27,4 +27,7 @@ struct Paged4Rows : PagedRows {
   }
 };
 
+// Entry points of the kernels; false where a call is not theirs.
+bool few_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status);
+
 }  // namespace kk

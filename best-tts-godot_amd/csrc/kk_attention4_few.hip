@@ -1,0 +1,387 @@
+// Attention of few queries over a paged cache of 4-bit codes: a step of single
+// tokens, with the query heads that share a key head together.
+#include "kk_attention4.h"
+
+namespace kk {
+
+constexpr int kFew4Threads = 256;
+constexpr int kFew4Waves = kFew4Threads / 64;
+// Weights are kept beside 2^r, r a whole number near max (x + log2 step), but not
+// below 2^-kLeast4 of the largest (a step is 0 or 2^-24 at the least); it follows
+// where a product passes it by 2^kSlack4, or a weight by 2^kFar4.
+constexpr float kLeast4 = 25.0f, kSlack4 = 7.0f, kFar4 = 32.0f;
+
+// The value of lane J of each row of 16 lanes, in all of the row.
+template <int J>
+__device__ __forceinline__ float of_row(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + J, 0xF, 0xF, true));
+}
+// f(integral_constant<J>) for J = 0 .. N - 1.
+template <int J, int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (J < N) {
+    f(std::integral_constant<int, J>{});
+    each<J + 1, N>(f);
+  }
+}
+
+// The low four bits of each byte, and the high ones, of w as halves: a code in the
+// low bits of a half is the subnormal code 2^-24, in bits 4 to 7 code 2^-20, which
+// the matrix cores multiply exactly; bytes 0, 2, 1, 3.
+struct Codes4 {
+  uint32_t low[2], high[2];
+};
+__device__ __forceinline__ Codes4 codes4(uint32_t w) {
+  const uint32_t v = w >> 8;
+  return Codes4{{w & 0x000f000fu, v & 0x000f000fu}, {w & 0x00f000f0u, v & 0x00f000f0u}};
+}
+__device__ __forceinline__ h8 halves8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(h8, (u4{a, b, c, d}));
+}
+
+// out = sum_j 2^(x_j - r) (step_j code_j + low_j) / sum_j 2^(x_j - r), x_j = c (step_j q . code_j + low_j sum(q)):
+// a wave its own steps of 64 tokens, on the matrix cores (v_mfma_f32_16x16x32_f16),
+// codes straight from memory to the registers that multiply them, with two
+// operations for four codes (codes4).  Bound by the codes' way from memory and, near
+// it, by the vector units.
+//
+// Scores are formed transposed, S^T = K Q^T, 16 tokens by 16 queries: a lane
+// (n = l % 16, g = l / 16) holds a query's column, and with token 16 g + 4 i + e in row
+// 4 g + e of tile i it holds the tokens 16 g .. 16 g + 15 of the step: what the second
+// product O^T = V^T P^T takes from it as they are, next to 16 consecutive codes of
+// V's rows, and those whose scales the 16 lanes of its row have loaded, one each,
+// which a DPP move hands to all of them.  A group of 16 tokens lies in one page.
+//
+// A lane's word of keys is one fragment: values d and d + D / 2 of four d, the
+// latter 2^4 times too large, against queries 2^-4 as large.  Values' rows d and
+// d + D / 2 are fragments of their own, whose sums differ by 2^4.  Queries are
+// brought to 2^14 by a power of two for each row; fp32 ones are the sum of two
+// halves (22 bits).  Weights times their value's step, beside 2^r, are the sum of
+// two halves also for fp16 queries (in one, the output is 1.4 times as far off).
+template <typename T, int W, int NT>
+__global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kernel(QueryArgs a, Paged4Rows rows, Cut cut) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
+  constexpr int D = 32 * W, HALF = D / 2;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  Unit u;
+  if (!find_unit(rows, cut, &u)) return;
+  const PagedArgs& p = rows.a;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int n = lane % 16, g = lane / 16, R = static_cast<int>(cut.rows);
+
+  // the lane's queries n + 16 nt: of fragment j, values 4 (W g + j) + {0, 2, 1, 3}, and those + HALF
+  h8 qf[NT][W][P];
+  float cq[NT], sum[NT];
+  int64_t qlo[NT], qhi[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = n + 16 * nt < R ? n + 16 * nt : R - 1;
+    const int t = row / a.group, head = u.h * a.group + row % a.group;
+    const Seen w = rows.seen(u.b, t);
+    qlo[nt] = w.lo;
+    qhi[nt] = w.hi;
+    const T* q = static_cast<const T*>(a.q) + u.b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+      T v[4];
+    };
+    float x[W][8], top = 0.0f, all = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Four f = *reinterpret_cast<const Four*>(q + s * HALF + 4 * (W * g + j));
+        const int order[4] = {0, 2, 1, 3};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = a.scale < 0.0f ? -to_f32(f.v[order[e]]) : to_f32(f.v[order[e]]);
+          x[j][4 * s + e] = v;
+          top = fmaxf(top, __builtin_fabsf(v));
+        }
+      }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const int up = 13 + 127 - static_cast<int>(__float_as_uint(top) >> 23);
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = ldexpf(x[j][e], e < 4 ? up : up - 4);
+        all += e < 4 ? y : y * 16.0f;
+        const _Float16 hi = static_cast<_Float16>(y);
+        qf[nt][j][0][e] = hi;
+        if constexpr (P == 2) qf[nt][j][P - 1][e] = static_cast<_Float16>(y - static_cast<float>(hi));
+      }
+    all += __shfl_xor(all, 16, 64);
+    all += __shfl_xor(all, 32, 64);
+    // scores come out 2^(up - 24) too large
+    sum[nt] = all * 0x1p-24f;
+    cq[nt] = ldexpf(__builtin_fabsf(a.scale), 24 - up);
+  }
+
+  const int shift = __builtin_ctz(p.block);
+  const int32_t* table = p.table + u.b * p.table_stride;
+  const int64_t t_first = u.lo + wave * kStep, page_bytes = int64_t{p.block} * HALF;
+  constexpr int kStride = kFew4Waves * kStep;
+  // The table's entry for tokens t on, as it stands (past the table its last), and
+  // the page, -1 where there is none: apart, so that an entry is waited for where its
+  // page is needed, a step later.
+  auto entry_at = [&](int64_t t) -> int {
+    const int64_t column = t >> shift;
+    return table[column < p.columns ? column : p.columns - 1];
+  };
+  auto page_of = [&](int64_t t, int entry) -> int {
+    return t < u.hi && t >> shift < p.columns && entry < p.pages ? entry : -1;
+  };
+  // of keys the lane's group of tokens is n / 4, of values and scales g; where
+  // there is no page, page 0 is read, and its tokens get no weight
+  const int tk = 16 * (n / 4) + n % 4;
+  struct Words {
+    uint32_t w[W];
+  };
+  Words ck[4];
+  u4 cv[W];
+  uint32_t ks1 = 0, vs1 = 0;
+  auto load_k = [&](int64_t t0, int page_k, int page_g) {
+    const int64_t at = (int64_t{page_k < 0 ? 0 : page_k} * p.heads + u.h) * page_bytes;
+    const uint8_t* k = rows.k + at + static_cast<int>((t0 + tk) & (p.block - 1)) * HALF + 4 * W * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ck[i] = *reinterpret_cast<const Words*>(k + 4 * i * HALF);
+    ks1 = rows.k_scale[(int64_t{page_g < 0 ? 0 : page_g} * p.heads + u.h) * p.block + ((t0 + lane) & (p.block - 1))];
+  };
+  auto load_v = [&](int64_t t0, int page_g) {
+    const int64_t head = int64_t{page_g < 0 ? 0 : page_g} * p.heads + u.h;
+    const uint8_t* v = rows.v + head * page_bytes + n * p.block + static_cast<int>((t0 + 16 * g) & (p.block - 1));
+#pragma unroll
+    for (int i = 0; i < W; ++i) cv[i] = *reinterpret_cast<const u4*>(v + 16 * i * p.block);
+    vs1 = rows.v_scale[head * p.block + ((t0 + lane) & (p.block - 1))];
+  };
+
+  f4 acc[NT][2 * W];  // rows d of the first half (even) and the second (odd)
+  float r[NT], l[NT], lows[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    r[nt] = -3.4028235e38f;
+    l[nt] = lows[nt] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) acc[nt][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // Keys of the next step are asked for once this step's are multiplied, values
+  // likewise: each has the other's half of a step for its way.
+  int entry_k = entry_at(t_first + 16 * (n / 4)), entry_g = entry_at(t_first + 16 * g);
+  int page_g = page_of(t_first + 16 * g, entry_g);
+  if (t_first < u.hi) {
+    load_k(t_first, page_of(t_first + 16 * (n / 4), entry_k), page_g);
+    load_v(t_first, page_g);
+  }
+  entry_k = entry_at(t_first + kStride + 16 * (n / 4));
+  entry_g = entry_at(t_first + kStride + 16 * g);
+  for (int64_t t0 = t_first; t0 < u.hi; t0 += kStride) {
+    f4 s[NT][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const Codes4 c = codes4(ck[i].w[j]);
+        const h8 k = halves8(c.low[0], c.low[1], c.high[0], c.high[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = P - 1; e >= 0; --e) s[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[nt][j][e], s[nt][i], 0, 0, 0);
+      }
+    }
+    const bool there = page_g >= 0;  // of the lane's own token, too: it is of group g
+    const float kstep = there ? low_half(ks1) : 0.0f, klow = there ? high_half(ks1) : 0.0f;
+    const float vstep = there ? low_half(vs1) : 0.0f, vlow = there ? high_half(vs1) : 0.0f;
+    const int page1 = page_of(t0 + kStride + 16 * g, entry_g);
+    if (t0 + kStride < u.hi) load_k(t0 + kStride, page_of(t0 + kStride + 16 * (n / 4), entry_k), page1);
+    entry_k = entry_at(t0 + 2 * kStride + 16 * (n / 4));
+    entry_g = entry_at(t0 + 2 * kStride + 16 * g);
+
+    // log2 of the token's step, rounded up, and the largest of the wave's
+    const uint32_t bits = __float_as_uint(vstep) & 0x7fffffffu;
+    const float ev = bits ? static_cast<float>(static_cast<int>(bits >> 23) - 126) : -INFINITY;
+    const float limit = fminf(kSlack4 - wave_max_dpp(ev), kFar4);
+    const float vs = vstep * 256.0f;
+
+    h8 pf[NT][2][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int64_t lo = qlo[nt] - (t0 + 16 * g), hi = there ? qhi[nt] - (t0 + 16 * g) : 0;
+      const int a0 = lo < 0 ? 0 : (lo > 16 ? 16 : static_cast<int>(lo));
+      const int a1 = hi < 0 ? 0 : (hi > 16 ? 16 : static_cast<int>(hi));
+      const bool whole = __all(a0 == 0 && a1 == 16);
+      float x[16], top = -INFINITY;
+      each<0, 16>([&](auto c) {
+        constexpr int J = decltype(c)::value;
+        x[J] = __builtin_fmaf(of_row<J>(kstep), s[nt][J / 4][J % 4], of_row<J>(klow) * sum[nt]) * cq[nt];
+      });
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = j >= a0 && j < a1 ? x[j] : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
+      if (__any(top > r[nt] + limit)) {
+        float sized = -INFINITY;
+        each<0, 16>([&](auto c) {
+          constexpr int J = decltype(c)::value;
+          sized = fmaxf(sized, x[J] + of_row<J>(ev));
+        });
+        sized = fmaxf(ceilf(sized), ceilf(top) - kLeast4);
+        sized = fmaxf(sized, __shfl_xor(sized, 16, 64));
+        sized = fmaxf(fmaxf(sized, __shfl_xor(sized, 32, 64)), r[nt]);
+        const float keep = __builtin_amdgcn_exp2f(r[nt] - sized);
+        r[nt] = sized;
+        l[nt] *= keep;
+        lows[nt] *= keep;
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) acc[nt][i] *= keep;
+      }
+      each<0, 16>([&](auto c) {
+        constexpr int J = decltype(c)::value;
+        const float w = __builtin_amdgcn_exp2f(x[J] - r[nt]);
+        l[nt] += w;
+        x[J] = w;
+      });
+      if (whole) {
+        each<0, 16>([&](auto c) {
+          constexpr int J = decltype(c)::value;
+          lows[nt] = __builtin_fmaf(of_row<J>(vlow), x[J], lows[nt]);
+          x[J] *= of_row<J>(vs);
+        });
+      } else {  // (past scales that are not finite)
+        each<0, 16>([&](auto c) {
+          constexpr int J = decltype(c)::value;
+          const bool sees = J >= a0 && J < a1;
+          const float low = of_row<J>(vlow), by = of_row<J>(vs);
+          lows[nt] = __builtin_fmaf(sees ? low : 0.0f, x[J], lows[nt]);
+          x[J] = sees ? x[J] * by : 0.0f;
+        });
+      }
+      const int order[4] = {0, 2, 1, 3};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float w = x[j / 4 * 4 + order[j % 4]];
+        const _Float16 hi16 = static_cast<_Float16>(w);
+        pf[nt][j / 8][0][j % 8] = hi16;
+        pf[nt][j / 8][1][j % 8] = static_cast<_Float16>(w - static_cast<float>(hi16));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      Codes4 c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = codes4(cv[i][j]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // tokens 16 g + 8 h on
+        const h8 low = halves8(c[2 * h].low[0], c[2 * h].low[1], c[2 * h + 1].low[0], c[2 * h + 1].low[1]);
+        const h8 high = halves8(c[2 * h].high[0], c[2 * h].high[1], c[2 * h + 1].high[0], c[2 * h + 1].high[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 1; e >= 0; --e) {
+            acc[nt][2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, pf[nt][h][e], acc[nt][2 * i], 0, 0, 0);
+            acc[nt][2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, pf[nt][h][e], acc[nt][2 * i + 1], 0, 0, 0);
+          }
+      }
+    }
+    if (t0 + kStride < u.hi) load_v(t0 + kStride, page1);
+    page_g = page1;
+  }
+
+  // join the waves: r and l of a wave's queries, then the sums, in LDS
+  constexpr int pitch = D + 4;
+  float* wm = lds;  // [waves][R], then [R] the block's
+  float* wl = wm + (kFew4Waves + 1) * R;
+  const int tail = (2 * (kFew4Waves + 1) * R * 4 + 15) & ~15;
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<char*>(lds) + tail);  // [waves][R][pitch]
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] += __shfl_xor(l[nt], 16, 64);
+    l[nt] += __shfl_xor(l[nt], 32, 64);
+    lows[nt] += __shfl_xor(lows[nt], 16, 64);
+    lows[nt] += __shfl_xor(lows[nt], 32, 64);
+    const int row = n + 16 * nt;
+    if (g == 0 && row < R) {
+      wm[wave * R + row] = r[nt];
+      wl[wave * R + row] = l[nt];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = n + 16 * nt;
+    if (row >= R) continue;
+    float top = wm[row], all = 0.0f;
+    for (int w = 1; w < kFew4Waves; ++w) top = fmaxf(top, wm[w * R + row]);
+    for (int w = 0; w < kFew4Waves; ++w) all += wl[w * R + row] * exp2f(wm[w * R + row] - top);
+    if (wave == 0 && g == 0) {
+      wm[kFew4Waves * R + row] = top;
+      wl[kFew4Waves * R + row] = all;
+    }
+    // (codes were 2^-24 and 2^-20 as large, weights 2^8 times)
+    const float by = exp2f(r[nt] - top), low = lows[nt] * by;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f4*>(sums + (wave * R + row) * pitch + h * HALF + 16 * i + 4 * g) =
+            acc[nt][2 * i + h] * (by * (h ? 0x1p12f : 0x1p16f)) + low;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * D; i += kFew4Threads) {
+    float* at = sums + (i / D) * pitch + i % D;
+    float v = at[0];
+    for (int w = 1; w < kFew4Waves; ++w) v += at[w * R * pitch];
+    at[0] = v;
+  }
+  __syncthreads();
+  const int64_t slot = int64_t{R} * (D + 2);
+  const Part part{u.b,  u.h, R, u.chunk, u.chunks, 0, cut.part + u.slot * slot, slot * cut.heads,
+                  cut.arrived + u.b * cut.heads + u.h};
+  put_rows<T, kFew4Threads>(a, part, sums, pitch, wm + kFew4Waves * R, wl + kFew4Waves * R, sums + R * pitch);
+}
+
+template <typename T, int W, int NT>
+static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queries) {
+  const int64_t capacity = rows.a.columns * rows.a.block;
+  const int64_t seen = rows.a.window && rows.a.window < capacity ? rows.a.window + a.T - 1 : capacity;
+  Cut cut;
+  int64_t blocks;
+  KK_TRY(plan_cut(a.B, rows.a.heads, queries, a.D, seen < capacity ? seen : capacity, 16, int64_t{4} * ctx().num_cus,
+                  &cut, &blocks, "cache4_attention"));
+  // the waves' sums; then, beside the first's, the chunks' weights
+  const int R = static_cast<int>(queries);
+  const size_t sums = size_t{kFew4Waves} * R * (a.D + 4) * 4;
+  const size_t joined = static_cast<size_t>(R) * (a.D + 4 + 2 * kMaxChunks) * 4;
+  const size_t bytes = (2 * (kFew4Waves + 1) * R * 4 + 15) / 16 * 16 + (sums > joined ? sums : joined);
+  if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(few_paged4_kernel<T, W, NT>)));
+  KK_LAUNCH((few_paged4_kernel<T, W, NT>), dim3(static_cast<unsigned>(blocks)), dim3(kFew4Threads), bytes, ctx().stream, a,
+            rows, cut);
+  return check_launch("few_paged4_kernel");
+}
+
+template <typename T, int NT>
+static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queries) {
+  switch (a.D) {
+    case 32: return launch_few4<T, 1, NT>(a, rows, queries);
+    case 64: return launch_few4<T, 2, NT>(a, rows, queries);
+    case 96: return launch_few4<T, 3, NT>(a, rows, queries);
+  }
+  return launch_few4<T, 4, NT>(a, rows, queries);
+}
+
+bool few_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status) {
+  const int64_t queries = int64_t{a.T} * a.group;
+  if (rows.a.pages < 1 || rows.a.columns < 1 || a.D > 128 || queries > 32) return false;
+  if (dtype == KK_F16)
+    *status = queries > 16 ? launch_few4<__half, 2>(a, rows, queries) : launch_few4<__half, 1>(a, rows, queries);
+  else
+    *status = queries > 16 ? launch_few4<float, 2>(a, rows, queries) : launch_few4<float, 1>(a, rows, queries);
+  return true;
+}
+
+}  // namespace kk
