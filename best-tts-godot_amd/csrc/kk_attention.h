@@ -110,11 +110,11 @@ struct PagedRows {
 // Eight codes as halves, exactly: a byte with its sign turned over is the low
 // half of 1024 + 128 + code, from which a packed sum takes 1152.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ h8 codes_h8(uint32_t lo, uint32_t hi) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   const h2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
   uint32_t w[4];
   lo ^= 0x80808080u;
@@ -396,6 +396,85 @@ __device__ __forceinline__ bool put_rows(const QueryArgs& a, const Part& u, cons
     out(r, d, sum);
   }
   return true;
+}
+
+// ------------------------------------------------------- many queries
+constexpr int kTileThreads = 256;
+constexpr int kTileRows = 128;  // queries of a block: 32 a wave
+struct TileCut {
+  int splits;          // blocks that share the tokens of a tile of queries
+  int tiles;           // of kTileRows queries in a sequence and key head
+  int64_t rows;        // queries of a sequence and key head: T * group
+  // of each tile of queries, where splits > 1: the parts that it has, and those
+  // parts' sums [kTileRows][D], maxima and sums of powers [kTileRows]
+  int* parts;
+  float* part;
+};
+constexpr int64_t part_floats(int D) { return int64_t{kTileRows} * (D + 2); }
+
+// The larger of, or the sum of, the values of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// Joins the parts of queries whose tokens were shared by several blocks, a wave a
+// query: weights 2^(m_i - max) / sum_i l_i 2^(m_i - max), a lane a part.  A launch
+// of its own, so that parts go by ordinary stores and many CUs join them (2 x 100
+// queries of 28 heads over up to 2000 tokens: 35 us with it, 101 where the last
+// block of a tile joins its parts).
+template <typename T, class Rows>
+__global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, Rows rows, TileCut cut) {
+  __shared__ float qv[kTileThreads / 64][kMaxHead];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = a.D;
+  constexpr int kRows = kTileThreads / 64;
+  const int64_t unit = blockIdx.x / (kTileRows / kRows);
+  const int r = blockIdx.x % (kTileRows / kRows) * kRows + wave;
+  const int64_t row = unit % cut.tiles * kTileRows + r, pair = unit / cut.tiles;
+  const int parts = cut.parts[unit];
+  if (row >= cut.rows || parts <= 1) return;
+  const int heads = a.heads / a.group;
+  const int64_t b = pair / heads, t = row / a.group;
+  const int head = static_cast<int>(pair % heads) * a.group + static_cast<int>(row % a.group);
+  const float* from = cut.part + unit * cut.splits * part_floats(D);
+  const float* ml = from + kTileRows * D + r;
+  const float m = lane < parts ? ml[lane * part_floats(D)] : -INFINITY;
+  const float l = lane < parts ? ml[lane * part_floats(D) + kTileRows] : 0.0f;
+  if (!std::is_base_of<PagedRows, Rows>::value && __any(m != m)) {  // (no page marks a part)
+    one_query<T>(a, rows, b, t, head, qv[wave]);
+    return;
+  }
+  const float w = exp2f(m - wave_max_dpp(m)), sum = wave_sum_dpp(w * l);
+  const float by = sum != 0.0f ? w / sum : 0.0f;
+  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
+  for (int d = lane; d < D; d += 64) {
+    float v = 0.0f;
+    for (int i = 0; i < parts; ++i)
+      v = __builtin_fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(by), i)),
+                         from[i * part_floats(D) + r * D + d], v);
+    from_f32(y[d], v);
+  }
+}
+
+// How many blocks share the tokens of each of `blocks` tiles of queries that see
+// at most `tokens`, in parts of `least` tokens at the least: where there are fewer
+// blocks than two a CU (100 fp32 queries of 12 heads of 128 over 1400 states: 31 us; in
+// parts of four tiles 83).
+inline void plan_parts(int64_t blocks, int64_t tokens, int64_t least, int D, TileCut* cut) {
+  const int64_t head = (blocks * 4 + 15) / 16 * 16;
+  int64_t splits = ceil_div(2 * ctx().num_cus, blocks);
+  const int64_t room = (static_cast<int64_t>(kScratchBytes) - head) / 4 / part_floats(D) / blocks;
+  const int64_t parts = ceil_div(tokens, least);
+  splits = splits < parts ? splits : parts;
+  splits = splits < kMaxChunks ? splits : kMaxChunks;
+  splits = splits < room ? splits : room;
+  cut->splits = static_cast<int>(splits < 1 ? 1 : splits);
+  cut->parts = static_cast<int*>(ctx().scratch);
+  cut->part = reinterpret_cast<float*>(static_cast<char*>(ctx().scratch) + head);
 }
 
 // Whether rows of an operand start at multiples of 16 bytes.

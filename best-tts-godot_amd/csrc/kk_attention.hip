@@ -131,7 +131,7 @@ int kk_cache4_attention(const kk_tensor* out, const kk_tensor* q, const kk_tenso
   KK_TRY(require_ready());
   if (a.B * a.T * a.heads == 0) return KK_OK;
   int status = KK_OK;
-  if (few_paged4_try(a, rows, q->dtype, &status)) return status;
+  if (few_paged4_try(a, rows, q->dtype, &status) || tiles_paged4_try(a, rows, q->dtype, &status)) return status;
   return q->dtype == KK_F16 ? launch_rows<__half>(a, rows) : launch_rows<float>(a, rows);
 }
 

@@ -27,7 +27,66 @@ struct Paged4Rows : PagedRows {
   }
 };
 
+// Weights are kept beside 2^r, r a whole number near max (x + log2 step), but not
+// below 2^-kLeast4 of the largest (a step is 0 or 2^-24 at the least); it follows
+// where a product passes it by 2^kSlack4, or a weight by 2^kFar4.
+constexpr float kLeast4 = 25.0f, kSlack4 = 7.0f, kFar4 = 32.0f;
+
+// The value of lane J of each row of 16 lanes, in all of the row.
+template <int J>
+__device__ __forceinline__ float of_row(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + J, 0xF, 0xF, true));
+}
+// f(integral_constant<J>) for J = 0 .. N - 1.
+template <int J, int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (J < N) {
+    f(std::integral_constant<int, J>{});
+    each<J + 1, N>(f);
+  }
+}
+
+// A key's step, NaN where it or the lowest value is not finite (a key with an
+// infinite one is NaN in its codes of 0).
+__device__ __forceinline__ float key_step(uint32_t scale) {
+  const float step = low_half(scale), low = high_half(scale);
+  return step + ((step - step) + (low - low));
+}
+// The low four bits of each byte of w, and the high ones, as halves code 2^-18
+// (subnormal, code << 6), bytes 0, 2, 1, 3: two operations for two codes.  The
+// matrix cores add up a subnormal's products to what its exponent would leave a normal
+// number: further down in the half (a mask alone takes codes out where they lie) codes
+// would lose up to ten bits of their sums, here one to four.
+// CENTRE: less 8, for one operation more (sums of codes are then those of values
+// around their middle, and fp32 keeps more of them).
+struct Codes4 {
+  uint32_t low[2], high[2];
+};
+template <bool CENTRE>
+__device__ __forceinline__ Codes4 codes4(uint32_t w) {
+  constexpr uint32_t kAt = 0x03c003c0u;
+  Codes4 c{{w << 6 & kAt, w >> 2 & kAt}, {w << 2 & kAt, w >> 6 & kAt}};
+  if constexpr (CENTRE) {
+    const h2 middle = {static_cast<_Float16>(-0x1p-15f), static_cast<_Float16>(-0x1p-15f)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c.low[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, c.low[i]) + middle);
+      c.high[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, c.high[i]) + middle);
+    }
+  }
+  return c;
+}
+// What a token's values are beside: its lowest one, or step times 8 above it.
+template <bool CENTRE>
+__device__ __forceinline__ float base4(uint32_t scale) {
+  return CENTRE ? __builtin_fmaf(low_half(scale), 8.0f, high_half(scale)) : high_half(scale);
+}
+__device__ __forceinline__ h8 halves8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(h8, (u4{a, b, c, d}));
+}
+
 // Entry points of the kernels; false where a call is not theirs.
 bool few_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status);
+bool tiles_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status);
 
 }  // namespace kk

@@ -6,43 +6,10 @@ namespace kk {
 
 constexpr int kFew4Threads = 256;
 constexpr int kFew4Waves = kFew4Threads / 64;
-// Weights are kept beside 2^r, r a whole number near max (x + log2 step), but not
-// below 2^-kLeast4 of the largest (a step is 0 or 2^-24 at the least); it follows
-// where a product passes it by 2^kSlack4, or a weight by 2^kFar4.
-constexpr float kLeast4 = 25.0f, kSlack4 = 7.0f, kFar4 = 32.0f;
-
-// The value of lane J of each row of 16 lanes, in all of the row.
-template <int J>
-__device__ __forceinline__ float of_row(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + J, 0xF, 0xF, true));
-}
-// f(integral_constant<J>) for J = 0 .. N - 1.
-template <int J, int N, class F>
-__device__ __forceinline__ void each(F&& f) {
-  if constexpr (J < N) {
-    f(std::integral_constant<int, J>{});
-    each<J + 1, N>(f);
-  }
-}
-
-// The low four bits of each byte, and the high ones, of w as halves: a code in the
-// low bits of a half is the subnormal code 2^-24, in bits 4 to 7 code 2^-20, which
-// the matrix cores multiply exactly; bytes 0, 2, 1, 3.
-struct Codes4 {
-  uint32_t low[2], high[2];
-};
-__device__ __forceinline__ Codes4 codes4(uint32_t w) {
-  const uint32_t v = w >> 8;
-  return Codes4{{w & 0x000f000fu, v & 0x000f000fu}, {w & 0x00f000f0u, v & 0x00f000f0u}};
-}
-__device__ __forceinline__ h8 halves8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __builtin_bit_cast(h8, (u4{a, b, c, d}));
-}
 
 // out = sum_j 2^(x_j - r) (step_j code_j + low_j) / sum_j 2^(x_j - r), x_j = c (step_j q . code_j + low_j sum(q)):
 // a wave its own steps of 64 tokens, on the matrix cores (v_mfma_f32_16x16x32_f16),
-// codes straight from memory to the registers that multiply them, with two
-// operations for four codes (codes4).  Bound by the codes' way from memory and, near
+// codes straight from memory to the registers that multiply them (codes4).  Bound by the codes' way from memory and, near
 // it, by the vector units.
 //
 // Scores are formed transposed, S^T = K Q^T, 16 tokens by 16 queries: a lane
@@ -52,16 +19,15 @@ __device__ __forceinline__ h8 halves8(uint32_t a, uint32_t b, uint32_t c, uint32
 // V's rows, and those whose scales the 16 lanes of its row have loaded, one each,
 // which a DPP move hands to all of them.  A group of 16 tokens lies in one page.
 //
-// A lane's word of keys is one fragment: values d and d + D / 2 of four d, the
-// latter 2^4 times too large, against queries 2^-4 as large.  Values' rows d and
-// d + D / 2 are fragments of their own, whose sums differ by 2^4.  Queries are
-// brought to 2^14 by a power of two for each row; fp32 ones are the sum of two
-// halves (22 bits).  Weights times their value's step, beside 2^r, are the sum of
+// A lane's word of keys is one fragment: values d and d + D / 2 of four d.  Values'
+// rows d and d + D / 2 are fragments of their own.  Queries are brought to 2^14 by a
+// power of two for each row; fp32 ones are the sum of two halves (22 bits).  Weights times their value's step, beside 2^r, are the sum of
 // two halves also for fp16 queries (in one, the output is 1.4 times as far off).
 template <typename T, int W, int NT>
 __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kernel(QueryArgs a, Paged4Rows rows, Cut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr int D = 32 * W, HALF = D / 2;
+  constexpr bool CENTRE = P == 2;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   Unit u;
   if (!find_unit(rows, cut, &u)) return;
@@ -84,6 +50,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
     struct __attribute__((packed, aligned(sizeof(T)))) Four {
       T v[4];
     };
+    const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
     float x[W][8], top = 0.0f, all = 0.0f;
 #pragma unroll
     for (int j = 0; j < W; ++j)
@@ -93,7 +60,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
         const int order[4] = {0, 2, 1, 3};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = a.scale < 0.0f ? -to_f32(f.v[order[e]]) : to_f32(f.v[order[e]]);
+          const float v = to_f32(f.v[order[e]]) * sign;
           x[j][4 * s + e] = v;
           top = fmaxf(top, __builtin_fabsf(v));
         }
@@ -105,17 +72,17 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
     for (int j = 0; j < W; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = ldexpf(x[j][e], e < 4 ? up : up - 4);
-        all += e < 4 ? y : y * 16.0f;
+        const float y = ldexpf(x[j][e], up);
+        all += y;
         const _Float16 hi = static_cast<_Float16>(y);
         qf[nt][j][0][e] = hi;
         if constexpr (P == 2) qf[nt][j][P - 1][e] = static_cast<_Float16>(y - static_cast<float>(hi));
       }
     all += __shfl_xor(all, 16, 64);
     all += __shfl_xor(all, 32, 64);
-    // scores come out 2^(up - 24) too large
-    sum[nt] = all * 0x1p-24f;
-    cq[nt] = ldexpf(__builtin_fabsf(a.scale), 24 - up);
+    // scores come out 2^(up - 18) too large
+    sum[nt] = all * 0x1p-18f;
+    cq[nt] = a.scale == 0.0f ? 1.0f : ldexpf(__builtin_fabsf(a.scale), 18 - up);
   }
 
   const int shift = __builtin_ctz(p.block);
@@ -184,7 +151,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
       for (int nt = 0; nt < NT; ++nt) s[nt][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const Codes4 c = codes4(ck[i].w[j]);
+        const Codes4 c = codes4<CENTRE>(ck[i].w[j]);
         const h8 k = halves8(c.low[0], c.low[1], c.high[0], c.high[1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -193,8 +160,8 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
       }
     }
     const bool there = page_g >= 0;  // of the lane's own token, too: it is of group g
-    const float kstep = there ? low_half(ks1) : 0.0f, klow = there ? high_half(ks1) : 0.0f;
-    const float vstep = there ? low_half(vs1) : 0.0f, vlow = there ? high_half(vs1) : 0.0f;
+    const float kstep = there ? key_step(ks1) : 0.0f, klow = there ? base4<CENTRE>(ks1) : 0.0f;
+    const float vstep = there ? low_half(vs1) : 0.0f, vlow = there ? base4<CENTRE>(vs1) : 0.0f;
     const int page1 = page_of(t0 + kStride + 16 * g, entry_g);
     if (t0 + kStride < u.hi) load_k(t0 + kStride, page_of(t0 + kStride + 16 * (n / 4), entry_k), page1);
     entry_k = entry_at(t0 + 2 * kStride + 16 * (n / 4));
@@ -216,19 +183,21 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
       float x[16], top = -INFINITY;
       each<0, 16>([&](auto c) {
         constexpr int J = decltype(c)::value;
-        x[J] = __builtin_fmaf(of_row<J>(kstep), s[nt][J / 4][J % 4], of_row<J>(klow) * sum[nt]) * cq[nt];
+        x[J] = __builtin_fmaf(of_row<J>(kstep), s[nt][J / 4][J % 4], of_row<J>(klow) * sum[nt]);
       });
       if (!whole) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = j >= a0 && j < a1 ? x[j] : -INFINITY;
+        asm volatile("");  // (a branch: its tests are for few steps)
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
+      for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
+      top *= cq[nt];
       if (__any(top > r[nt] + limit)) {
         float sized = -INFINITY;
         each<0, 16>([&](auto c) {
           constexpr int J = decltype(c)::value;
-          sized = fmaxf(sized, x[J] + of_row<J>(ev));
+          sized = fmaxf(sized, __builtin_fmaf(x[J], cq[nt], of_row<J>(ev)));
         });
         sized = fmaxf(ceilf(sized), ceilf(top) - kLeast4);
         sized = fmaxf(sized, __shfl_xor(sized, 16, 64));
@@ -242,7 +211,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
       }
       each<0, 16>([&](auto c) {
         constexpr int J = decltype(c)::value;
-        const float w = __builtin_amdgcn_exp2f(x[J] - r[nt]);
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[J], cq[nt], -r[nt]));
         l[nt] += w;
         x[J] = w;
       });
@@ -260,21 +229,26 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
           lows[nt] = __builtin_fmaf(sees ? low : 0.0f, x[J], lows[nt]);
           x[J] = sees ? x[J] * by : 0.0f;
         });
+        asm volatile("");
       }
-      const int order[4] = {0, 2, 1, 3};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float w = x[j / 4 * 4 + order[j % 4]];
-        const _Float16 hi16 = static_cast<_Float16>(w);
-        pf[nt][j / 8][0][j % 8] = hi16;
-        pf[nt][j / 8][1][j % 8] = static_cast<_Float16>(w - static_cast<float>(hi16));
+      for (int j = 0; j < 16; j += 2) {  // tokens j / 4 * 4 + {0, 2} and {1, 3}
+        const int i = j / 4 * 4 + j % 4 / 2;
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const h2 w0 = __builtin_convertvector((f2{x[i], x[i + 2]}), h2);
+        const h2 w1 = __builtin_convertvector((f2{__builtin_fmaf(static_cast<float>(w0[0]), -1.0f, x[i]),
+                                                  __builtin_fmaf(static_cast<float>(w0[1]), -1.0f, x[i + 2])}), h2);
+        pf[nt][j / 8][0][j % 8] = w0[0];
+        pf[nt][j / 8][0][j % 8 + 1] = w0[1];
+        pf[nt][j / 8][1][j % 8] = w1[0];
+        pf[nt][j / 8][1][j % 8 + 1] = w1[1];
       }
     }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       Codes4 c[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = codes4(cv[i][j]);
+      for (int j = 0; j < 4; ++j) c[j] = codes4<CENTRE>(cv[i][j]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // tokens 16 g + 8 h on
         const h8 low = halves8(c[2 * h].low[0], c[2 * h].low[1], c[2 * h + 1].low[0], c[2 * h + 1].low[1]);
@@ -322,14 +296,14 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
       wm[kFew4Waves * R + row] = top;
       wl[kFew4Waves * R + row] = all;
     }
-    // (codes were 2^-24 and 2^-20 as large, weights 2^8 times)
+    // (codes were 2^-18 as large, weights 2^8 times)
     const float by = exp2f(r[nt] - top), low = lows[nt] * by;
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<f4*>(sums + (wave * R + row) * pitch + h * HALF + 16 * i + 4 * g) =
-            acc[nt][2 * i + h] * (by * (h ? 0x1p12f : 0x1p16f)) + low;
+            acc[nt][2 * i + h] * (by * 0x1p10f) + low;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * D; i += kFew4Threads) {

@@ -4,25 +4,9 @@
 
 namespace kk {
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f16v __attribute__((ext_vector_type(16)));
-
-constexpr int kTileThreads = 256;
-constexpr int kTileRows = 128;  // queries of a block: 32 a wave
 constexpr int kPutRows = 64;    // of them put out at a time
-constexpr int kLeastTiles = 2;    // of tokens, of a block that shares them
+constexpr int kLeastTiles = 2;  // of tokens, of a block that shares them
 constexpr float kSlack = 7.0f;
-
-struct TileCut {
-  int splits;          // blocks that share the tokens of a tile of queries
-  int tiles;           // of kTileRows queries in a sequence and key head
-  int64_t rows;        // queries of a sequence and key head: T * group
-  // of each tile of queries, where splits > 1: the parts that it has, and those
-  // parts' sums [kTileRows][D], maxima and sums of powers [kTileRows]
-  int* parts;
-  float* part;
-};
-constexpr int64_t part_floats(int D) { return int64_t{kTileRows} * (D + 2); }
 
 // Where the tile kernel's operands come from.
 enum Source { kPaged, kHalf, kFloat };
@@ -34,16 +18,6 @@ constexpr int key_pitch(int DT) { return 64 * DT + 16; }
 constexpr int value_pitch(int TT) { return 2 * TT + 16; }
 constexpr int tile_bytes(int SRC, int DT, int TT) {
   return (TT * key_pitch(DT) + 32 * DT * value_pitch(TT)) * (SRC == kFloat ? 3 : 1) + (SRC == kPaged ? 0 : TT * 4);
-}
-
-// The larger of, or the sum of, the values of lanes l and l ^ 32.
-__device__ __forceinline__ float max_halves(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float sum_halves(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
 // Two values as the sum of two halves each.
@@ -804,66 +778,16 @@ __global__ void __launch_bounds__(kTileThreads, WIDE && DT <= (SRC == kFloat ? 2
   }
 }
 
-// Joins the parts of queries whose tokens were shared by several blocks, a wave a
-// query: weights 2^(m_i - max) / sum_i l_i 2^(m_i - max), a lane a part.  A launch
-// of its own, so that parts go by ordinary stores and many CUs join them (2 x 100
-// queries of 28 heads over up to 2000 tokens: 35 us with it, 101 where the last
-// block of a tile joins its parts).
-template <typename T, class Rows>
-__global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, Rows rows, TileCut cut) {
-  __shared__ float qv[kTileThreads / 64][kMaxHead];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, D = a.D;
-  constexpr int kRows = kTileThreads / 64;
-  const int64_t unit = blockIdx.x / (kTileRows / kRows);
-  const int r = blockIdx.x % (kTileRows / kRows) * kRows + wave;
-  const int64_t row = unit % cut.tiles * kTileRows + r, pair = unit / cut.tiles;
-  const int parts = cut.parts[unit];
-  if (row >= cut.rows || parts <= 1) return;
-  const int heads = a.heads / a.group;
-  const int64_t b = pair / heads, t = row / a.group;
-  const int head = static_cast<int>(pair % heads) * a.group + static_cast<int>(row % a.group);
-  const float* from = cut.part + unit * cut.splits * part_floats(D);
-  const float* ml = from + kTileRows * D + r;
-  const float m = lane < parts ? ml[lane * part_floats(D)] : -INFINITY;
-  const float l = lane < parts ? ml[lane * part_floats(D) + kTileRows] : 0.0f;
-  if (!std::is_same<Rows, PagedRows>::value && __any(m != m)) {
-    one_query<T>(a, rows, b, t, head, qv[wave]);
-    return;
-  }
-  const float w = exp2f(m - wave_max_dpp(m)), sum = wave_sum_dpp(w * l);
-  const float by = sum != 0.0f ? w / sum : 0.0f;
-  T* y = static_cast<T*>(a.y) + b * a.ys[0] + t * a.ys[1] + head * a.ys[2];
-  for (int d = lane; d < D; d += 64) {
-    float v = 0.0f;
-    for (int i = 0; i < parts; ++i)
-      v = __builtin_fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(by), i)),
-                         from[i * part_floats(D) + r * D + d], v);
-    from_f32(y[d], v);
-  }
-}
-
 template <typename T, class Rows, int SRC, int DT, int TT, bool WIDE>
 static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, const char* who) {
   const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * (a.heads / a.group);
   const int64_t tiles = ceil_div(queries, kTileRows);
   TileCut cut{};
   cut.rows = queries;
-  // where there are fewer blocks than two a CU, the tokens are cut, into parts
-  // of two tiles at least (100 fp32 queries of 12 heads of 128 over 1400 states: 31
-  // us; in parts of four tiles 83)
-  const int64_t blocks = pairs * tiles, head = (blocks * 4 + 15) / 16 * 16;
-  int64_t splits = ceil_div(2 * ctx().num_cus, blocks);
-  const int64_t room = (static_cast<int64_t>(kScratchBytes) - head) / 4 / part_floats(a.D) / blocks;
-  const int64_t parts = ceil_div(tokens, kLeastTiles * TT);
-  splits = splits < parts ? splits : parts;
-  splits = splits < kMaxChunks ? splits : kMaxChunks;
-  splits = splits < room ? splits : room;
-  if (splits < 1) splits = 1;
-  cut.parts = static_cast<int*>(ctx().scratch);
-  cut.part = reinterpret_cast<float*>(static_cast<char*>(ctx().scratch) + head);
-  cut.splits = static_cast<int>(splits);
+  const int64_t blocks = pairs * tiles;
+  plan_parts(blocks, tokens, kLeastTiles * TT, a.D, &cut);
   cut.tiles = static_cast<int>(tiles);
-  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
+  const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
   int64_t bytes = (int64_t{kPutRows} * (a.D + 4) + 2 * kPutRows) * 4;
   if (bytes < tile_bytes(SRC, DT, TT)) bytes = tile_bytes(SRC, DT, TT);
@@ -872,7 +796,7 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, co
   KK_LAUNCH((attention_tile_kernel<T, Rows, SRC, DT, TT, WIDE>), grid, dim3(kTileThreads), static_cast<unsigned>(bytes),
             ctx().stream, a, rows, cut);
   KK_TRY(check_launch("attention_tile_kernel"));
-  if (splits == 1) return KK_OK;
+  if (cut.splits == 1) return KK_OK;
   KK_LAUNCH((join_parts_kernel<T, Rows>), dim3(static_cast<unsigned>(blocks * (kTileRows / (kTileThreads / 64)))),
             dim3(kTileThreads), 0, ctx().stream, a, rows, cut);
   return check_launch("join_parts_kernel");
