@@ -85,6 +85,37 @@ __device__ __forceinline__ h8 halves8(uint32_t a, uint32_t b, uint32_t c, uint32
   return __builtin_bit_cast(h8, (u4{a, b, c, d}));
 }
 
+// sum + the products of x[0 .. 15] with the values of lanes 0 .. 15 of each row: a
+// fused product with a DPP operand each, which the compiler makes two instructions
+// of.  (The first waits out what a DPP read needs behind a write of `of`, and what a
+// read needs behind an exponential.)
+__device__ __forceinline__ float dot_row(float sum, float of, const float (&x)[16]) {
+#define KK_DOT_ROW(J, X) "v_fmac_f32_dpp %0, %1, %" #X " row_newbcast:" #J " row_mask:0xf bank_mask:0xf\n"
+  asm("s_nop 1\n" KK_DOT_ROW(0, 2) KK_DOT_ROW(1, 3) KK_DOT_ROW(2, 4) KK_DOT_ROW(3, 5) KK_DOT_ROW(4, 6) KK_DOT_ROW(5, 7)
+          KK_DOT_ROW(6, 8) KK_DOT_ROW(7, 9) KK_DOT_ROW(8, 10) KK_DOT_ROW(9, 11) KK_DOT_ROW(10, 12) KK_DOT_ROW(11, 13)
+              KK_DOT_ROW(12, 14) KK_DOT_ROW(13, 15) KK_DOT_ROW(14, 16) KK_DOT_ROW(15, 17)
+      : "+v"(sum)
+      : "v"(of), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(x[8]),
+        "v"(x[9]), "v"(x[10]), "v"(x[11]), "v"(x[12]), "v"(x[13]), "v"(x[14]), "v"(x[15]));
+#undef KK_DOT_ROW
+  return sum;
+}
+
+// Two weights as the sum of two halves each; `less` holds -1, where the compiler
+// does not see it: the rest is then one mixed-precision fused product, not a
+// conversion and a difference.
+__device__ __forceinline__ float minus_one() {
+  float v = -1.0f;
+  asm("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ void split4(float x, float y, float less, h2* hi, h2* lo) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  *hi = __builtin_convertvector((f2{x, y}), h2);
+  *lo = __builtin_convertvector((f2{__builtin_fmaf(static_cast<float>((*hi)[0]), less, x),
+                                    __builtin_fmaf(static_cast<float>((*hi)[1]), less, y)}), h2);
+}
+
 // Entry points of the kernels; false where a call is not theirs.
 bool few_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status);
 bool tiles_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status);

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
     vs1 = rows.v_scale[head * p.block + ((t0 + lane) & (p.block - 1))];
   };
 
+  const float less = minus_one();
   f4 acc[NT][2 * W];  // rows d of the first half (even) and the second (odd)
   float r[NT], l[NT], lows[NT];
 #pragma unroll
@@ -209,16 +210,15 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) acc[nt][i] *= keep;
       }
-      each<0, 16>([&](auto c) {
-        constexpr int J = decltype(c)::value;
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[J], cq[nt], -r[nt]));
-        l[nt] += w;
-        x[J] = w;
-      });
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], cq[nt], -r[nt]));
+        l[nt] += x[j];
+      }
       if (whole) {
+        lows[nt] = dot_row(lows[nt], vlow, x);
         each<0, 16>([&](auto c) {
           constexpr int J = decltype(c)::value;
-          lows[nt] = __builtin_fmaf(of_row<J>(vlow), x[J], lows[nt]);
           x[J] *= of_row<J>(vs);
         });
       } else {  // (past scales that are not finite)
@@ -234,10 +234,8 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {  // tokens j / 4 * 4 + {0, 2} and {1, 3}
         const int i = j / 4 * 4 + j % 4 / 2;
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        const h2 w0 = __builtin_convertvector((f2{x[i], x[i + 2]}), h2);
-        const h2 w1 = __builtin_convertvector((f2{__builtin_fmaf(static_cast<float>(w0[0]), -1.0f, x[i]),
-                                                  __builtin_fmaf(static_cast<float>(w0[1]), -1.0f, x[i + 2])}), h2);
+        h2 w0, w1;
+        split4(x[i], x[i + 2], less, &w0, &w1);
         pf[nt][j / 8][0][j % 8] = w0[0];
         pf[nt][j / 8][0][j % 8 + 1] = w0[1];
         pf[nt][j / 8][1][j % 8] = w1[0];
