@@ -23,7 +23,7 @@ constexpr int kFew4Waves = kFew4Threads / 64;
 // rows d and d + D / 2 are fragments of their own.  Queries are brought to 2^14 by a
 // power of two for each row; fp32 ones are the sum of two halves (22 bits).  Weights times their value's step, beside 2^r, are the sum of
 // two halves also for fp16 queries (in one, the output is 1.4 times as far off).
-template <typename T, int W, int NT>
+template <typename T, int W, int NT, bool BIG>
 __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kernel(QueryArgs a, Paged4Rows rows, Cut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr int D = 32 * W, HALF = D / 2;
@@ -91,36 +91,43 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
   constexpr int kStride = kFew4Waves * kStep;
   // The table's entry for tokens t on, as it stands (past the table its last), and
   // the page, -1 where there is none: apart, so that an entry is waited for where its
-  // page is needed, a step later.
+  // page is needed, a step later.  BIG: a step's tokens lie in one page.
   auto entry_at = [&](int64_t t) -> int {
     const int64_t column = t >> shift;
     return table[column < p.columns ? column : p.columns - 1];
   };
   auto page_of = [&](int64_t t, int entry) -> int {
-    return t < u.hi && t >> shift < p.columns && entry < p.pages ? entry : -1;
+    const int page = t < u.hi && t >> shift < p.columns && entry < p.pages ? entry : -1;
+    return BIG ? __builtin_amdgcn_readfirstlane(page) : page;
   };
   // of keys the lane's group of tokens is n / 4, of values and scales g; where
   // there is no page, page 0 is read, and its tokens get no weight
-  const int tk = 16 * (n / 4) + n % 4;
+  const int tk = 16 * (n / 4) + n % 4, group_k = BIG ? 0 : 16 * (n / 4), group_g = BIG ? 0 : 16 * g;
   struct Words {
     uint32_t w[W];
   };
   Words ck[4];
   u4 cv[W];
   uint32_t ks1 = 0, vs1 = 0;
+  // (of tokens t0 + i, within a page: all of them where BIG)
+  auto in_page = [&](int64_t t0, int i) -> int {
+    const int first = static_cast<int>(t0) & (p.block - 1);
+    return BIG ? first + i : (first + i) & (p.block - 1);
+  };
   auto load_k = [&](int64_t t0, int page_k, int page_g) {
-    const int64_t at = (int64_t{page_k < 0 ? 0 : page_k} * p.heads + u.h) * page_bytes;
-    const uint8_t* k = rows.k + at + static_cast<int>((t0 + tk) & (p.block - 1)) * HALF + 4 * W * g;
+    const int64_t head_k = int64_t{page_k < 0 ? 0 : page_k} * p.heads + u.h;
+    const int64_t head_g = BIG ? head_k : int64_t{page_g < 0 ? 0 : page_g} * p.heads + u.h;
+    const uint8_t* k = rows.k + head_k * page_bytes + static_cast<uint32_t>(in_page(t0, tk) * HALF + 4 * W * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) ck[i] = *reinterpret_cast<const Words*>(k + 4 * i * HALF);
-    ks1 = rows.k_scale[(int64_t{page_g < 0 ? 0 : page_g} * p.heads + u.h) * p.block + ((t0 + lane) & (p.block - 1))];
+    ks1 = rows.k_scale[head_g * p.block + static_cast<uint32_t>(in_page(t0, lane))];
   };
   auto load_v = [&](int64_t t0, int page_g) {
     const int64_t head = int64_t{page_g < 0 ? 0 : page_g} * p.heads + u.h;
-    const uint8_t* v = rows.v + head * page_bytes + n * p.block + static_cast<int>((t0 + 16 * g) & (p.block - 1));
+    const uint8_t* v = rows.v + head * page_bytes + static_cast<uint32_t>(n * p.block + in_page(t0, 16 * g));
 #pragma unroll
     for (int i = 0; i < W; ++i) cv[i] = *reinterpret_cast<const u4*>(v + 16 * i * p.block);
-    vs1 = rows.v_scale[head * p.block + ((t0 + lane) & (p.block - 1))];
+    vs1 = rows.v_scale[head * p.block + static_cast<uint32_t>(in_page(t0, lane))];
   };
 
   const float less = minus_one();
@@ -136,14 +143,17 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
 
   // Keys of the next step are asked for once this step's are multiplied, values
   // likewise: each has the other's half of a step for its way.
-  int entry_k = entry_at(t_first + 16 * (n / 4)), entry_g = entry_at(t_first + 16 * g);
-  int page_g = page_of(t_first + 16 * g, entry_g);
+  int entry_k = entry_at(t_first + group_k), entry_g = BIG ? entry_k : entry_at(t_first + group_g);
+  int page_g = page_of(t_first + group_g, entry_g);
   if (t_first < u.hi) {
-    load_k(t_first, page_of(t_first + 16 * (n / 4), entry_k), page_g);
+    load_k(t_first, BIG ? page_g : page_of(t_first + group_k, entry_k), page_g);
     load_v(t_first, page_g);
   }
-  entry_k = entry_at(t_first + kStride + 16 * (n / 4));
-  entry_g = entry_at(t_first + kStride + 16 * g);
+  auto next_entries = [&](int64_t t) {
+    entry_g = entry_at(t + group_g);
+    entry_k = BIG ? entry_g : entry_at(t + group_k);
+  };
+  next_entries(t_first + kStride);
   for (int64_t t0 = t_first; t0 < u.hi; t0 += kStride) {
     f4 s[NT][4];
 #pragma unroll
@@ -163,10 +173,9 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
     const bool there = page_g >= 0;  // of the lane's own token, too: it is of group g
     const float kstep = there ? key_step(ks1) : 0.0f, klow = there ? base4<CENTRE>(ks1) : 0.0f;
     const float vstep = there ? low_half(vs1) : 0.0f, vlow = there ? base4<CENTRE>(vs1) : 0.0f;
-    const int page1 = page_of(t0 + kStride + 16 * g, entry_g);
-    if (t0 + kStride < u.hi) load_k(t0 + kStride, page_of(t0 + kStride + 16 * (n / 4), entry_k), page1);
-    entry_k = entry_at(t0 + 2 * kStride + 16 * (n / 4));
-    entry_g = entry_at(t0 + 2 * kStride + 16 * g);
+    const int page1 = page_of(t0 + kStride + group_g, entry_g);
+    if (t0 + kStride < u.hi) load_k(t0 + kStride, BIG ? page1 : page_of(t0 + kStride + group_k, entry_k), page1);
+    next_entries(t0 + 2 * kStride);
 
     // log2 of the token's step, rounded up, and the largest of the wave's
     const uint32_t bits = __float_as_uint(vstep) & 0x7fffffffu;
@@ -187,9 +196,10 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
         x[J] = __builtin_fmaf(of_row<J>(kstep), s[nt][J / 4][J % 4], of_row<J>(klow) * sum[nt]);
       });
       if (!whole) {
+        int first = a0, past = a1;
+        asm volatile("" : "+v"(first), "+v"(past));  // (a branch: its tests are for few steps)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = j >= a0 && j < a1 ? x[j] : -INFINITY;
-        asm volatile("");  // (a branch: its tests are for few steps)
+        for (int j = 0; j < 16; ++j) x[j] = j >= first && j < past ? x[j] : -INFINITY;
       }
 #pragma unroll
       for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
@@ -222,14 +232,15 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
           x[J] *= of_row<J>(vs);
         });
       } else {  // (past scales that are not finite)
+        int first = a0, past = a1;
+        asm volatile("" : "+v"(first), "+v"(past));
         each<0, 16>([&](auto c) {
           constexpr int J = decltype(c)::value;
-          const bool sees = J >= a0 && J < a1;
+          const bool sees = J >= first && J < past;
           const float low = of_row<J>(vlow), by = of_row<J>(vs);
           lows[nt] = __builtin_fmaf(sees ? low : 0.0f, x[J], lows[nt]);
           x[J] = sees ? x[J] * by : 0.0f;
         });
-        asm volatile("");
       }
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {  // tokens j / 4 * 4 + {0, 2} and {1, 3}
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kern
   put_rows<T, kFew4Threads>(a, part, sums, pitch, wm + kFew4Waves * R, wl + kFew4Waves * R, sums + R * pitch);
 }
 
-template <typename T, int W, int NT>
+template <typename T, int W, int NT, bool BIG>
 static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queries) {
   const int64_t capacity = rows.a.columns * rows.a.block;
   const int64_t seen = rows.a.window && rows.a.window < capacity ? rows.a.window + a.T - 1 : capacity;
@@ -330,10 +341,16 @@ static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queri
   const size_t sums = size_t{kFew4Waves} * R * (a.D + 4) * 4;
   const size_t joined = static_cast<size_t>(R) * (a.D + 4 + 2 * kMaxChunks) * 4;
   const size_t bytes = (2 * (kFew4Waves + 1) * R * 4 + 15) / 16 * 16 + (sums > joined ? sums : joined);
-  if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(few_paged4_kernel<T, W, NT>)));
-  KK_LAUNCH((few_paged4_kernel<T, W, NT>), dim3(static_cast<unsigned>(blocks)), dim3(kFew4Threads), bytes, ctx().stream, a,
+  if (bytes > 65536) KK_TRY(allow_large_lds(reinterpret_cast<const void*>(few_paged4_kernel<T, W, NT, BIG>)));
+  KK_LAUNCH((few_paged4_kernel<T, W, NT, BIG>), dim3(static_cast<unsigned>(blocks)), dim3(kFew4Threads), bytes, ctx().stream, a,
             rows, cut);
   return check_launch("few_paged4_kernel");
+}
+
+template <typename T, int W, int NT>
+static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queries) {
+  return rows.a.block >= kStep ? launch_few4<T, W, NT, true>(a, rows, queries)
+                               : launch_few4<T, W, NT, false>(a, rows, queries);
 }
 
 template <typename T, int NT>

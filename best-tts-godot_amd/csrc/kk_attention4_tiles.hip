@@ -263,11 +263,11 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
         const uint32_t w = a1 > a0 ? (0xffffu >> (16 - (a1 - a0))) << a0 : 0u;
         seen = k ? (seen & 0xffffu) | w << 16 : (seen & 0xffff0000u) | w;
       }
+      asm volatile("" : "+v"(seen));  // (a branch: its tests are for few steps)
 #pragma unroll
       for (int k = 0; k < SUB; ++k)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[k][e] = seen >> (16 * k + e) & 1 ? s[k][e] : -INFINITY;
-      asm volatile("");  // (a branch: its tests are for few steps)
     }
     float top = -INFINITY;
 #pragma unroll
@@ -313,14 +313,15 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
           x[J] *= of_row<J>(vs[k]);
         });
       } else {  // (past scales that are not finite)
+        uint32_t bits = seen >> (16 * k);
+        asm volatile("" : "+v"(bits));
         each<0, 16>([&](auto c) {
           constexpr int J = decltype(c)::value;
-          const bool sees = seen >> (16 * k + J) & 1;
+          const bool sees = bits >> J & 1;
           const float m = of_row<J>(low[k]), by = of_row<J>(vs[k]);
           lows = __builtin_fmaf(sees ? m : 0.0f, x[J], lows);
           x[J] = sees ? x[J] * by : 0.0f;
         });
-        asm volatile("");
       }
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
