@@ -126,6 +126,28 @@ def test_rms_norm_views_in_place_and_misaligned(gpu, t):
     assert kk.to_host(kk.ops.rms_norm(kk.to_device(np.zeros((0, 5), t)))).shape == (0, 5)
 
 
+@pytest.mark.parametrize("shape,scale", [
+    ((1, 256), (1, 1)), ((3, 260), (3, 1)), ((5, 4096), (5, 1)), ((2, 3, 1028), (2, 3, 1)), ((2, 3, 1028), (1, 3, 1)),
+    ((7, 8196), ()), ((70000, 256), (70000, 1)), ((3, 255), (3, 1)), ((4, 12), (4, 1))])
+def test_dequantize_rows(gpu, shape, scale):
+    """Codes of tokens with their scales: products of fp32, equal to the last bit."""
+    kk = gpu
+    r = rng(shape[-1])
+    q = r.integers(-127, 128, shape).astype(np.int8)
+    s = np.asarray(r.uniform(-1e-2, 1e-2, scale), np.float32)
+    s[(0,) * s.ndim] = 3e38
+    with np.errstate(over="ignore"):
+        want = q.astype(np.float32) * s
+    dev = kk.to_device
+    assert_bitexact(kk.to_host(kk.ops.dequantize(dev(q), dev(s))), want, "rows")
+    if q.ndim == 2:  # views of rows of another length, and codes at an odd address
+        wide = np.zeros((shape[0], shape[1] + 8), np.int8)
+        for at in (4, 3):
+            wide[:, at:at + shape[1]] = q
+            view = dev(wide).slice_axis(1, at, at + shape[1])
+            assert_bitexact(kk.to_host(kk.ops.dequantize(view, dev(s))), want, "views")
+
+
 def test_rms_norm_quant_feeds_the_8_bit_product(gpu):
     """Codes and scales as matmul_integer_scaled takes them: its rows times the scales."""
     kk = gpu
