@@ -285,6 +285,8 @@ static int rms_norm(const kk_tensor* out, const kk_tensor* scales, const kk_tens
   if (!(eps >= 0.0f) || eps == INFINITY) return set_error(KK_E_ARG, "%s: eps must be finite and not negative", who);
   if (N < 1 || N > kMostNorm)
     return set_error(KK_E_UNSUPPORTED, "%s: rows of %lld values (1 to %d)", who, static_cast<long long>(N), kMostNorm);
+  if (sum && numel(x) > 0 && sum->data == out->data)
+    return set_error(KK_E_ARG, "%s: out and sum must not be the same", who);
   KK_TRY(require_ready());
   if (a.rows == 0) return KK_OK;
   a.x = x->data;

@@ -172,30 +172,44 @@ struct ReleaseArgs {
 constexpr int kReleaseThreads = 1024;
 
 // One block: first how many pages come back, then they, in the order of
-// sequences and columns, in front of those that are free.
+// sequences and columns, in front of those that are free.  Of 1024 sequences at a
+// time it lists the ended ones, and takes the columns of each 1024 at a time.
 __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(ReleaseArgs a) {
   __shared__ int64_t part[kReleaseThreads / 64];
+  __shared__ int s_row[kReleaseThreads], s_pages[kReleaseThreads];
+  const int tid = threadIdx.x;
   const int64_t given = *a.used < 0 ? 0 : *a.used < a.F ? *a.used : a.F;
   int64_t all = 0, back = 0;
   for (int pass = 0; pass < 2; ++pass) {
     int64_t mine = 0, at = given - back;  // (pass 1)
-    for (int64_t b = 0; b < a.B; ++b) {
-      if (!a.ended[b * a.ended_st]) continue;
-      int64_t n = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
-      n = n < 0 ? 0 : n;
-      n = n > a.columns << a.shift ? a.columns : (n + (int64_t{1} << a.shift) - 1) >> a.shift;
-      int32_t* row = a.table + b * a.table_stride;
-      for (int64_t c0 = 0; c0 < n; c0 += kReleaseThreads) {
-        const int64_t c = c0 + threadIdx.x;
-        const int32_t page = c < n ? row[c] : -1;
-        if (pass == 0) {
-          mine += page >= 0;
-          continue;
+    for (int64_t b0 = 0; b0 < a.B; b0 += kReleaseThreads) {
+      const int64_t b = b0 + tid;
+      int64_t n = 0;
+      if (b < a.B && a.ended[b * a.ended_st]) {
+        n = load_index(a.lengths, a.lengths_dt, b * a.lengths_st);
+        n = n < 0 ? 0 : n;
+        n = n > a.columns << a.shift ? a.columns : (n + (int64_t{1} << a.shift) - 1) >> a.shift;
+      }
+      const int place = static_cast<int>(scan_block(n > 0, &all, part)) - 1, listed = static_cast<int>(all);
+      if (n > 0) {
+        s_row[place] = tid;
+        s_pages[place] = static_cast<int>(n);
+      }
+      __syncthreads();
+      for (int e = 0; e < listed; ++e) {
+        int32_t* row = a.table + (b0 + s_row[e]) * a.table_stride;
+        for (int c0 = 0; c0 < s_pages[e]; c0 += kReleaseThreads) {
+          const int c = c0 + tid;
+          const int32_t page = c < s_pages[e] ? row[c] : -1;
+          if (pass == 0) {
+            mine += page >= 0;
+            continue;
+          }
+          const int64_t to = at + scan_block(page >= 0, &all, part) - 1;
+          if (page >= 0 && to < given) a.free[to] = page;
+          if (c < s_pages[e]) row[c] = -1;
+          at += all;
         }
-        const int64_t to = at + scan_block(page >= 0, &all, part) - 1;
-        if (page >= 0 && to < given) a.free[to] = page;
-        if (c < n) row[c] = -1;
-        at += all;
       }
     }
     if (pass == 0) {
@@ -203,7 +217,7 @@ __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(ReleaseA
       back = all < given ? all : given;
     }
   }
-  if (threadIdx.x == 0) *a.used = static_cast<int32_t>(given - back);
+  if (tid == 0) *a.used = static_cast<int32_t>(given - back);
 }
 
 static int check_ints(const kk_tensor* t, const char* name, int dtype, int64_t n, const char* who) {

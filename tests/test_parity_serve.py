@@ -224,7 +224,7 @@ def test_plan_pages_odd_lists(gpu):
     assert (s[:, 0] == 77).all() and np.array_equal(s[:, 1:], np.arange(3)[:, None] * 16 + np.arange(10))
 
 
-@pytest.mark.parametrize("B,columns,block", [(1, 1, 16), (7, 5, 32), (3, 2500, 16), (90, 40, 64)])
+@pytest.mark.parametrize("B,columns,block", [(1, 1, 16), (7, 5, 32), (3, 2500, 16), (90, 40, 64), (1024, 3, 16), (2500, 7, 32)])
 def test_release_pages(gpu, B, columns, block):
     kk = gpu
     r = rng(B * columns)
@@ -430,7 +430,55 @@ def test_sample_repeats_itself(gpu):
             assert_bitexact(kk.to_host(g), w)
 
 
+@pytest.mark.parametrize("B,V", [(150, 60000), (330, 33000)])
+def test_sample_many_long_rows(gpu, B, V):
+    """More rows than there is room to cut as often as one, or at all."""
+    r = rng(V)
+    x = (2 * r.normal(size=(B, V))).astype(np.float16)
+    check_sample(gpu, x, r.random(B).astype(np.float32), top_k=r.choice([0, 1, 50, 1000], B).astype(np.int32),
+                 top_p=r.choice([1.0, 0.9, 0.5], B).astype(np.float32))
+
+
 # ------------------------------------------------------------------- graphs
+def test_recorded_draws_of_long_rows_replay(gpu):
+    """Two recorded calls over rows cut into blocks, with rows of nothing, of equal logits and without a temperature
+    among them, replayed by turns between eager calls, share no state."""
+    kk = gpu
+    r = rng(24)
+    f = np.float32
+    graphs = []
+    for B, V, t in ((5, 50257, np.float32), (7, 20001, np.float16)):
+        x, u, temperature, top_p = (kk.to_device(np.ones(s, d)) for s, d in (((B, V), t), ((B,), f), ((B,), f), ((B,), f)))
+        tokens, logs = kk.DeviceTensor.empty((B,), np.int32), kk.DeviceTensor.empty((B,))
+        args = [z.desc() for z in (tokens, logs, x, u, temperature)] + [None, top_p.desc(), None]
+        kk._lib.call("kk_sample", *args)
+        kk.sync()
+        kk._lib.call("kk_graph_begin")
+        kk._lib.call("kk_sample", *args)
+        g = ctypes.c_int(-1)
+        kk._lib.call("kk_graph_end", ctypes.byref(g))
+        graphs.append((g.value, B, V, t, x, u, temperature, top_p, tokens, logs))
+    for i in range(4):
+        want = []
+        for g, B, V, t, x, u, temperature, top_p, tokens, logs in graphs:
+            host = (3 * r.normal(size=(B, V))).astype(t)
+            host[1], host[2] = -np.inf, 0.25
+            hu, ht, hp = r.random(B).astype(f), r.choice([0.5, 1.0], B).astype(f), r.choice([0.9, 1.0], B).astype(f)
+            ht[0] = 0
+            for to, of in ((x, host), (u, hu), (temperature, ht), (top_p, hp), (tokens, np.full(B, -7, np.int32))):
+                kk.ops.copy_into(to, kk.to_device(of))
+            want.append([kk.to_host(z) for z in kk.ops.sample(x, u, temperature, top_p=top_p)])
+            check_sample(kk, host, hu, ht, top_p=hp)
+        kk.sync()
+        for g, *_ in graphs:
+            kk._lib.call("kk_graph_launch", g)
+        for (*_, tokens, logs), w in zip(graphs, want):
+            assert_bitexact(kk.to_host(tokens), w[0], f"replay {i}")
+            assert_bitexact(kk.to_host(logs), w[1], f"replay {i}")
+    for g, *_ in graphs:
+        kk._lib.call("kk_graph_destroy", g)
+
+
 def test_a_recorded_serving_step_replays(gpu):
     """Pages, norm, append, attention and a token, recorded with resident buffers and replayed between eager work, each
     replay as the eager call."""

@@ -36,7 +36,8 @@ def norm_args(quant=False, **over):
     (dict(weight=T((64,), I8)), ARG, "weight"),
     (dict(weight=T((64,), F32, (2,))), ARG, "weight"),
     (dict(eps=-1e-6), ARG, "eps"),
-    (dict(eps=float("nan")), ARG, "eps")])
+    (dict(eps=float("nan")), ARG, "eps"),
+    (dict(), ARG, "must not be the same")])
 def test_rms_norm_refuses(quant, over, code, match):
     refused("kk_rms_norm_quant" if quant else "kk_rms_norm", norm_args(quant, **over), code, match)
 
