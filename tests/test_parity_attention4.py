@@ -155,6 +155,25 @@ def test_a_batch_past_a_waves_lanes(gpu, t, window):
 
 
 @pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T", [1, 33])
+def test_more_sequences_than_a_grids_axis(gpu, t, T):
+    """33000 sequences of two heads that share their pages."""
+    kk = gpu
+    r = rng(33000)
+    B, block, dim, at = 33000, 16, 32, [0, 1, 255, 32767, 32768, 32999]
+    lengths = r.integers(0, 33, B).astype(np.int32)
+    lengths[at] = [32, 1, 0, 17, 16, 31]
+    table = np.broadcast_to(np.array([4, 1], np.int32), (B, 2))
+    parts = filled(r, 5, 2, dim, block)
+    q = np.broadcast_to(r.normal(size=(1, T, 2, dim)).astype(t), (B, T, 2, dim))
+    out = run(kk, q, parts, table, lengths, scale=0.2)
+    assert not out[lengths == 0].any()
+    for b in at:
+        if lengths[b]:
+            check(out[b], q[b], parts, table[b], int(lengths[b]), 0.2, what=f"sequence {b}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
 @pytest.mark.parametrize("T,Hq,Hk,dim,block,longest,window", [
     (1, 2, 1, 128, 64, 20011, 0), (1, 7, 1, 96, 32, 9000, 0), (1, 24, 1, 64, 16, 7001, 5000), (3, 8, 1, 64, 256, 6000, 0),
     (2, 12, 1, 96, 64, 4100, 130), (1, 16, 2, 192, 64, 5003, 0)])
