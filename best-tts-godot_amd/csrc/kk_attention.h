@@ -462,11 +462,11 @@ __global__ void __launch_bounds__(kTileThreads) join_parts_kernel(QueryArgs a, R
 
 // How many blocks share the tokens of each of `blocks` tiles of queries that see
 // at most `tokens`, in parts of `least` tokens at the least: where there are fewer
-// blocks than two a CU (100 fp32 queries of 12 heads of 128 over 1400 states: 31 us; in
+// blocks than `wanted` (two a CU: 100 fp32 queries of 12 heads of 128 over 1400 states: 31 us; in
 // parts of four tiles 83).
-inline void plan_parts(int64_t blocks, int64_t tokens, int64_t least, int D, TileCut* cut) {
+inline void plan_parts(int64_t blocks, int64_t tokens, int64_t least, int D, int64_t wanted, TileCut* cut) {
   const int64_t head = (blocks * 4 + 15) / 16 * 16;
-  int64_t splits = ceil_div(2 * ctx().num_cus, blocks);
+  int64_t splits = ceil_div(wanted, blocks);
   const int64_t room = (static_cast<int64_t>(kScratchBytes) - head) / 4 / part_floats(D) / blocks;
   const int64_t parts = ceil_div(tokens, least);
   splits = splits < parts ? splits : parts;

@@ -13,20 +13,27 @@ constexpr int kLeastTokens4 = 256;  // of a block that shares them
 // 4 h + c it holds 16 tokens next to each other, whose scales the lanes of its rows
 // of 16 have loaded, one each.  A wave reads codes from the caches straight into
 // the registers that multiply them (its three neighbours read the same ones):
-// nothing goes through LDS, and no wave waits for another.
+// nothing goes through LDS, and no wave waits for another.  Bound by the vector units
+// (codes, exponentials, weights to halves) beside the products: 2 x 1531 queries of 32
+// heads of 128 over up to 4099 tokens in 246 us, 470 TFLOP/s of fp16.
 //
 // Keys' lowest values (beside fp32 queries: their middles, in two halves) times the
 // query's sum, in three halves, are added by a product of their own.  Queries,
 // weights and codes as there; PW 1: weights are rounded to one half, values count as
 // step (code - 8) + middle, and 8 times the rounded weights' sum is taken off in the
 // end, so that a weight's rounding acts on what a value differs from its middle by.
-template <typename T, int W, int SUB, bool BIG, int PW>
-__global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
+//
+// WAVES 8: two waves have the same queries and one half of the tokens each, and the
+// first adds up both through LDS.
+template <typename T, int W, int SUB, bool BIG, int PW, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
     tile_paged4_kernel(QueryArgs a, Paged4Rows rows, TileCut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr bool CENTRE = P == 2;
   constexpr int D = 32 * W, HALF = D / 2, KF = 2 * W, RT = (W + 1) / 2, kTokens4 = 32 * SUB;
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  constexpr int PAIRS = WAVES / (kTileRows / 32);  // waves of the same queries
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % (kTileRows / 32);
+  const int which = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / (kTileRows / 32);
   const int n = lane % 32, hf = lane / 32;
   const PagedArgs& p = rows.a;
   // neighbouring blocks of an XCD share keys and values; the longest rows first
@@ -53,6 +60,11 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
   if (chunk >= chunks) return;
   lo = uniform(lo + chunk * share * kTokens4);
   hi = uniform(chunk + 1 < chunks ? lo + share * kTokens4 : hi);
+  if constexpr (PAIRS == 2) {
+    const int64_t middle = lo + (ceil_div(hi - lo, kTokens4) + 1) / 2 * kTokens4;
+    lo = which ? middle : lo;
+    hi = which ? hi : middle < hi ? middle : hi;
+  }
 
   // the lane's query: of fragment j, values 8 W hf + 4 j + {0, 2, 1, 3}, and those + HALF
   const int row = wave * 32 + n < count ? wave * 32 + n : count - 1;
@@ -359,7 +371,44 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
 
   // codes were 2^-18 as large, weights 2^8 times
   l = sum_halves(l);
-  const float base = sum_halves(lows) - (PW == 1 ? sum_halves(sumw) * 0x1p-5f : 0.0f);
+  float base = sum_halves(lows) - (PW == 1 ? sum_halves(sumw) * 0x1p-5f : 0.0f), unit = 0x1p10f;
+  if constexpr (PAIRS == 2) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // [waves][D + 2][32]
+    float* const its = lds + wave * ((D + 2) * 32) + n;
+    auto place = [&](int i, int h, int e) { return (32 * i + 8 * (e / 4) + 4 * hf + e % 4 + h * HALF) * 32; };
+    auto there = [&](int i, int e) { return 32 * i + 8 * (e / 4) + 4 * hf < HALF; };
+    if (which) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (there(i, e)) its[place(i, h, e)] = __builtin_fmaf(acc[i][h][e], unit, base);
+      if (hf == 0) {
+        its[D * 32] = r;
+        its[D * 32 + 32] = l;
+      }
+    }
+    __syncthreads();
+    if (which) return;
+    const float r1 = its[D * 32], l1 = its[D * 32 + 32], top = fmaxf(r, r1);
+    const float by0 = __builtin_amdgcn_exp2f(r - top), by1 = __builtin_amdgcn_exp2f(r1 - top);
+    r = top;
+    l = l * by0 + l1 * by1;
+    unit *= by0;
+    base *= by0;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (there(i, e))
+            acc[i][h][e] = __builtin_fmaf(its[place(i, h, e)], by1, __builtin_fmaf(acc[i][h][e], unit, base));
+    unit = 1.0f;
+    base = 0.0f;
+  }
   const int64_t pair = at.z * static_cast<int64_t>(cut.tiles) + tile;
   if (cut.splits > 1 && chunk == 0 && threadIdx.x == 0) cut.parts[pair] = chunks;
   if (wave * 32 + n >= count) return;
@@ -373,7 +422,7 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
         for (int c = 0; c < 4; ++c) {
           const int d = 32 * i + 8 * c + 4 * hf;
           if (d >= HALF) continue;
-          const f4 v = f4{acc[i][h][4 * c], acc[i][h][4 * c + 1], acc[i][h][4 * c + 2], acc[i][h][4 * c + 3]} * 0x1p10f + base;
+          const f4 v = f4{acc[i][h][4 * c], acc[i][h][4 * c + 1], acc[i][h][4 * c + 2], acc[i][h][4 * c + 3]} * unit + base;
           *reinterpret_cast<f4*>(to + row * D + h * HALF + d) = v;
         }
     if (hf == 0) {
@@ -398,33 +447,50 @@ __global__ void __launch_bounds__(kTileThreads, W <= 4 ? 2 : 1)
         } o;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          from_f32(o.v[e], l != 0.0f ? __builtin_fmaf(acc[i][h][4 * c + e], 0x1p10f, base) * by : 0.0f);
+          from_f32(o.v[e], l != 0.0f ? __builtin_fmaf(acc[i][h][4 * c + e], unit, base) * by : 0.0f);
         *reinterpret_cast<Four*>(y + h * HALF + d) = o;
       }
 }
 
-template <typename T, int W, bool BIG, int PW>
-static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
+template <typename T, int W, bool BIG, int PW, int WAVES>
+static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileCut& cut, int64_t pairs) {
   const char* who = "cache4_attention";
-  const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * rows.a.heads, tiles = ceil_div(queries, kTileRows);
-  TileCut cut{};
-  cut.rows = queries;
-  cut.tiles = static_cast<int>(tiles);
-  plan_parts(pairs * tiles, tokens, kLeastTokens4, a.D, &cut);
-  const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
+  const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cut.tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
   constexpr int SUB = W <= (sizeof(T) == 4 ? 2 : 4) ? 2 : 1;
-  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, PW>), grid, dim3(kTileThreads), 0, ctx().stream, a, rows, cut);
+  constexpr unsigned bytes = WAVES * 32 == kTileRows ? 0 : kTileRows * (32 * W + 2) * 4;
+  if (bytes > 65536)
+    KK_TRY(allow_large_lds(reinterpret_cast<const void*>(tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES>)));
+  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES>), grid, dim3(64 * WAVES), bytes, ctx().stream, a, rows, cut);
   KK_TRY(check_launch("tile_paged4_kernel"));
   if (cut.splits == 1) return KK_OK;
-  KK_LAUNCH((join_parts_kernel<T, Paged4Rows>), dim3(static_cast<unsigned>(pairs * tiles * (kTileRows / (kTileThreads / 64)))),
+  KK_LAUNCH((join_parts_kernel<T, Paged4Rows>), dim3(static_cast<unsigned>(pairs * cut.tiles * (kTileRows / (kTileThreads / 64)))),
             dim3(kTileThreads), 0, ctx().stream, a, rows, cut);
   return check_launch("join_parts_kernel");
 }
 
+// Eight waves a block, of which one fits a CU, where whole rounds of a tile's blocks
+// take five eighths of the CUs or more (heads of 128, 128 blocks: 127 us with four waves,
+// 105 with eight; 176: 67 and 56; heads of 64 in fp32, 144 blocks: 47 and 50); else four,
+// and as many blocks as fit two a CU.
+template <typename T, int W, bool BIG, int PW>
+static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
+  const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * rows.a.heads, tiles = ceil_div(queries, kTileRows);
+  TileCut cut{};
+  cut.rows = queries;
+  cut.tiles = static_cast<int>(tiles);
+  if constexpr (W <= 4)
+    if (const int64_t cus = ctx().num_cus, blocks = pairs * tiles; cus / blocks * blocks * 8 >= cus * 5) {
+      plan_parts(blocks, tokens, kLeastTokens4, a.D, cus - blocks + 1, &cut);
+      return launch_tiles4<T, W, BIG, PW, 8>(a, rows, cut, pairs);
+    }
+  plan_parts(pairs * tiles, tokens, kLeastTokens4, a.D, 2 * ctx().num_cus, &cut);
+  return launch_tiles4<T, W, BIG, PW, 4>(a, rows, cut, pairs);
+}
+
 // Weights of fp16 queries in one half, where many queries keep the matrix cores
-// busy, or in two (2 x 1531 queries of 32 heads of 128 over up to 4099 tokens: 267
-// and 310 us, outputs 1.4 times and as far off as their own rounding to fp16).
+// busy, or in two (2 x 1531 queries of 32 heads of 128 over up to 4099 tokens: 246
+// and 305 us, outputs 1.4 times and as far off as their own rounding to fp16).
 template <typename T, int W, bool BIG>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
   if constexpr (sizeof(T) == 2 && W <= 4)

@@ -785,7 +785,7 @@ static int launch_tiles(const QueryArgs& a, const Rows& rows, int64_t tokens, co
   TileCut cut{};
   cut.rows = queries;
   const int64_t blocks = pairs * tiles;
-  plan_parts(blocks, tokens, kLeastTiles * TT, a.D, &cut);
+  plan_parts(blocks, tokens, kLeastTiles * TT, a.D, 2 * ctx().num_cus, &cut);
   cut.tiles = static_cast<int>(tiles);
   const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));

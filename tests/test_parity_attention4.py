@@ -155,6 +155,30 @@ def test_a_batch_past_a_waves_lanes(gpu, t, window):
 
 
 @pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("B,T,Hq,Hk,dim,block,longest,window", [
+    (35, 70, 4, 4, 64, 16, 700, 0), (70, 40, 8, 4, 128, 64, 300, 40), (50, 130, 3, 3, 96, 32, 530, 0),
+    (9, 600, 16, 8, 32, 128, 900, 0), (33, 520, 2, 2, 128, 16, 521, 0)])
+def test_many_tiles_of_queries(gpu, t, B, T, Hq, Hk, dim, block, longest, window):
+    """Batches whose tiles of queries fill the GPU once, nearly, or several times over."""
+    kk = gpu
+    r = rng(B * T)
+    table, pages = pool(r, B, -(-longest // block))
+    lengths = r.integers(1, longest + 1, B).astype(np.int32)
+    lengths[[0, B - 1]] = longest, longest - 1
+    counts = np.minimum(r.integers(0, T + 1, B), lengths).astype(np.int32)
+    counts[0] = min(T, longest)
+    parts = filled(r, pages, Hk, dim, block)
+    q = (1.5 * r.normal(size=(B, T, Hq, dim))).astype(t)
+    scale = 1.3 / dim ** 0.5
+    out = run(kk, q, parts, table, lengths, counts, scale, window)
+    for b in range(B):
+        assert not out[b, counts[b]:].any()
+    for b in (0, 1, B // 2, B - 1):
+        some = np.unique(r.integers(0, T, 24))
+        check(out[b], q[b], parts, table[b], int(lengths[b]), scale, window, int(counts[b]), some, f"sequence {b}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
 @pytest.mark.parametrize("T", [1, 33])
 def test_more_sequences_than_a_grids_axis(gpu, t, T):
     """33000 sequences of two heads that share their pages."""
