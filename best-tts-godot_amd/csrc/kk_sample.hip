@@ -127,22 +127,22 @@ __device__ __forceinline__ int bin_of(const RowRule& r, double y) {
   const double b = y * r.inv;
   return b < BINS - 1 ? static_cast<int>(b) : BINS - 1;
 }
-// 2^34 (1 - 2^-(y - lower edge)): 1 - e^-z by its series, z <= 64 ln 2 / BINS, to
-// the term below 2^-36.
+// 2^34 (1 - 2^-t), t = y - lower edge, by its series, t <= 64 / BINS, to the term
+// below 2^-36.
 template <int BINS>
 __device__ __forceinline__ uint32_t deficit(const RowRule& r, double y, int bin) {
-  double z = fma(-static_cast<double>(bin), r.width, y) * 0.69314718055994530942;
-  z = z > 0.0 ? z : 0.0;
-  double d = 1.0;
-  if constexpr (BINS < kWide) {
-    d = fma(-z * (1.0 / 7.0), d, 1.0);
-    d = fma(-z * (1.0 / 6.0), d, 1.0);
-  }
-  d = fma(-z * (1.0 / 5.0), d, 1.0);
-  d = fma(-z * (1.0 / 4.0), d, 1.0);
-  d = fma(-z * (1.0 / 3.0), d, 1.0);
-  d = fma(-z * (1.0 / 2.0), d, 1.0);
-  return static_cast<uint32_t>(fma(z * d, static_cast<double>(int64_t{1} << kOnes), 0.5));
+  constexpr double kLn2 = 0.69314718055994530942, kUnit = static_cast<double>(int64_t{1} << kOnes);
+  constexpr double k1 = kUnit * kLn2, k2 = -k1 * kLn2 / 2, k3 = -k2 * kLn2 / 3, k4 = -k3 * kLn2 / 4, k5 = -k4 * kLn2 / 5,
+                   k6 = -k5 * kLn2 / 6, k7 = -k6 * kLn2 / 7;
+  double t = fma(-static_cast<double>(bin), r.width, y);
+  t = t > 0.0 ? t : 0.0;
+  double d = k5;
+  if constexpr (BINS < kWide) d = fma(fma(k7, t, k6), t, k5);
+  d = fma(d, t, k4);
+  d = fma(d, t, k3);
+  d = fma(d, t, k2);
+  d = fma(d, t, k1);
+  return static_cast<uint32_t>(fma(d, t, 0.5));
 }
 __device__ __forceinline__ double edge_weight(const RowRule& r, int bin) { return exp2(-static_cast<double>(bin) * r.width); }
 

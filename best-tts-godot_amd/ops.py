@@ -696,9 +696,9 @@ def plan_pages(table, starts, counts, free, used, tokens, block, used_out=None):
     granted none.  The new `used` is a tensor of its own, or used_out (which may
     be `used`)."""
     shape = (table.shape[0], int(tokens))
-    slots, positions = DeviceTensor._fresh(shape, _I64), DeviceTensor._fresh(shape, _I32)
-    lengths, granted = DeviceTensor._fresh(shape[:1], _I32), DeviceTensor._fresh(shape[:1], _I32)
-    used_out = DeviceTensor._fresh((1,), _I32) if used_out is None else used_out
+    slots, positions, lengths, granted, own = DeviceTensor._together(
+        (shape, _I64), (shape, _I32), (shape[:1], _I32), (shape[:1], _I32), ((1,), _I32))
+    used_out = own if used_out is None else used_out
     _lib.call("kk_plan_pages", table.desc(), slots.desc(), positions.desc(), lengths.desc(), granted.desc(),
               used_out.desc(), starts.desc(), _d(counts), free.desc(), used.desc(), int(block))
     return slots, positions, lengths, granted, used_out
@@ -743,8 +743,7 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
     [B, V] with the given numbers uniforms [B] in [0, 1) (include/kk.h,
     kk_sample); a temperature of 0 takes the largest logit."""
     logits = _inner(logits)
-    tokens = DeviceTensor._fresh(logits.shape[:1], _I32)
-    logs = DeviceTensor._fresh(logits.shape[:1], _F32)
+    tokens, logs = DeviceTensor._together((logits.shape[:1], _I32), (logits.shape[:1], _F32))
     _lib.call("kk_sample", tokens.desc(), logs.desc(), logits.desc(), uniforms.desc(), _d(temperature), _d(top_k),
               _d(top_p), _d(min_p))
     return tokens, logs

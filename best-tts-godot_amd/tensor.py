@@ -245,6 +245,27 @@ class DeviceTensor:
         return t
 
     @classmethod
+    def _together(cls, *parts):
+        """_fresh() of each (shape, dtype), in one buffer: for small results of
+        one call, which cost an allocation each otherwise (and its release)."""
+        starts, end = [], 0
+        for shape, dtype in parts:
+            starts.append(end)
+            end += (math.prod(shape) * dtype.itemsize + 63) // 64 * 64
+        storage, made = Storage(end), []
+        for (shape, dtype), start in zip(parts, starts):
+            t = object.__new__(cls)
+            t.storage = storage
+            t.shape = shape
+            t.dtype = dtype
+            t.strides = _contig_strides(shape)
+            t.offset = start // dtype.itemsize
+            t.host = None
+            t._desc = None
+            made.append(t)
+        return made
+
+    @classmethod
     def from_numpy(cls, arr):
         arr = np.asarray(arr)
         if not arr.flags.c_contiguous:  # (np.ascontiguousarray would make 0-d arrays 1-d)
