@@ -7,6 +7,69 @@ namespace kk {
 constexpr int kFew4Threads = 256;
 constexpr int kFew4Waves = kFew4Threads / 64;
 
+// find_unit for more sequences than a wave has lanes, by all threads: each a run of
+// sequences (512 sequences of up to 500 tokens, 8 key heads of 128: 139 us where each
+// wave goes through them 64 at a time, 101 here).
+__device__ __forceinline__ bool find_unit_by_block(const Paged4Rows& rows, const Cut& cut, Unit* u, float* lds) {
+  int64_t* const sums = reinterpret_cast<int64_t*>(lds);  // [2][waves]
+  Unit* const found = reinterpret_cast<Unit*>(sums + 2 * kFew4Waves);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t id = blockIdx.x / cut.heads, each = ceil_div(cut.B, kFew4Threads);
+  const int64_t b0 = threadIdx.x * each, b1 = b0 + each < cut.B ? b0 + each : cut.B;
+  auto steps_of = [&](int64_t b) -> int64_t {
+    const Seen s = rows.span(b);
+    return ceil_div(s.hi - (s.lo / kStep) * kStep, kStep);
+  };
+  int64_t total = 0;
+  for (int64_t b = b0; b < b1; ++b) total += steps_of(b);
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+  if (lane == 0) sums[wave] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kFew4Waves; ++w) total += sums[w];
+  const int64_t c = chunk_size(total, cut.units, cut.most, cut.least);
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += chunk_count(steps_of(b), c);
+  int64_t upto = mine;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t o = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += o;
+  }
+  if (lane == 63) sums[kFew4Waves + wave] = upto;
+  __syncthreads();
+  int64_t all = 0;
+  for (int w = 0; w < kFew4Waves; ++w) {
+    if (w < wave) upto += sums[kFew4Waves + w];
+    all += sums[kFew4Waves + w];
+  }
+  if (id >= all) return false;
+  if (id < upto && id >= upto - mine) {
+    int64_t first = upto - mine, b = b0, n = steps_of(b);
+    for (; id >= first + chunk_count(n, c); n = steps_of(b)) {
+      first += chunk_count(n, c);
+      ++b;
+    }
+    const Seen s = rows.span(b);
+    const int64_t size = chunk_steps(n, c) * kStep, lo = (s.lo / kStep) * kStep + (id - first) * size;
+    found->b = b;
+    found->chunks = static_cast<int>(chunk_count(n, c));
+    found->chunk = static_cast<int>(id - first);
+    found->slot = first * cut.heads;
+    found->lo = lo;
+    found->hi = lo + size < s.hi ? lo + size : s.hi;
+  }
+  __syncthreads();
+  u->h = static_cast<int>(blockIdx.x % cut.heads);
+  u->b = uniform(found->b);
+  u->chunks = static_cast<int>(uniform(found->chunks));
+  u->chunk = static_cast<int>(uniform(found->chunk));
+  u->slot = uniform(found->slot) + u->h;
+  u->lo = uniform(found->lo);
+  u->hi = uniform(found->hi);
+  __syncthreads();
+  return true;
+}
+
 // out = sum_j 2^(x_j - r) (step_j code_j + low_j) / sum_j 2^(x_j - r), x_j = c (step_j q . code_j + low_j sum(q)):
 // a wave its own steps of 64 tokens, on the matrix cores (v_mfma_f32_16x16x32_f16),
 // codes straight from memory to the registers that multiply them (codes4).  Bound by the
@@ -26,13 +89,13 @@ constexpr int kFew4Waves = kFew4Threads / 64;
 // their value's step, beside 2^r, are the sum of two halves also for fp16 queries (in
 // one, the output is 1.4 times as far off).
 template <typename T, int W, int NT, bool BIG>
-__global__ void __launch_bounds__(kFew4Threads, NT == 1 ? 2 : 1) few_paged4_kernel(QueryArgs a, Paged4Rows rows, Cut cut) {
+__global__ void __launch_bounds__(kFew4Threads, NT * W * sizeof(T) <= 28 ? 2 : 1) few_paged4_kernel(QueryArgs a, Paged4Rows rows, Cut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr int D = 32 * W, HALF = D / 2;
   constexpr bool CENTRE = P == 2;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   Unit u;
-  if (!find_unit(rows, cut, &u)) return;
+  if (cut.B > 64 ? !find_unit_by_block(rows, cut, &u, lds) : !find_unit(rows, cut, &u)) return;
   const PagedArgs& p = rows.a;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int n = lane % 16, g = lane / 16, R = static_cast<int>(cut.rows);
@@ -360,13 +423,20 @@ static int launch_few4(const QueryArgs& a, const Paged4Rows& rows, int64_t queri
     case 32: return launch_few4<T, 1, NT>(a, rows, queries);
     case 64: return launch_few4<T, 2, NT>(a, rows, queries);
     case 96: return launch_few4<T, 3, NT>(a, rows, queries);
+    case 128: return launch_few4<T, 4, NT>(a, rows, queries);
   }
-  return launch_few4<T, 4, NT>(a, rows, queries);
+  if constexpr (NT == 1) switch (a.D) {
+    case 160: return launch_few4<T, 5, NT>(a, rows, queries);
+    case 192: return launch_few4<T, 6, NT>(a, rows, queries);
+    case 224: return launch_few4<T, 7, NT>(a, rows, queries);
+    case 256: return launch_few4<T, 8, NT>(a, rows, queries);
+  }
+  return set_error(KK_E_UNSUPPORTED, "cache4_attention: heads of %d values", a.D);
 }
 
 bool few_paged4_try(const QueryArgs& a, const Paged4Rows& rows, int dtype, int* status) {
   const int64_t queries = int64_t{a.T} * a.group;
-  if (rows.a.pages < 1 || rows.a.columns < 1 || a.D > 128 || queries > 32) return false;
+  if (rows.a.pages < 1 || rows.a.columns < 1 || queries > (a.D > 128 ? 16 : 32)) return false;
   if (dtype == KK_F16)
     *status = queries > 16 ? launch_few4<__half, 2>(a, rows, queries) : launch_few4<__half, 1>(a, rows, queries);
   else
