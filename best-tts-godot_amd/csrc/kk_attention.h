@@ -405,6 +405,7 @@ struct TileCut {
   int splits;          // blocks that share the tokens of a tile of queries
   int tiles;           // of kTileRows queries in a sequence and key head
   int64_t rows;        // queries of a sequence and key head: T * group
+  int row_waves;       // waves of a block that have queries of their own (over 4-bit codes)
   // of each tile of queries, where splits > 1: the parts that it has, and those
   // parts' sums [kTileRows][D], maxima and sums of powers [kTileRows]
   int* parts;

@@ -23,17 +23,17 @@ constexpr int kLeastTokens4 = 256;  // of a block that shares them
 // step (code - 8) + middle, and 8 times the rounded weights' sum is taken off in the
 // end, so that a weight's rounding acts on what a value differs from its middle by.
 //
-// WAVES 8: two waves have the same queries and one half of the tokens each, and the
-// first adds up both through LDS.
-template <typename T, int W, int SUB, bool BIG, int PW, int WAVES>
+// SHARE: cut.row_waves waves (4, 2 or 1: as many as have queries) share the tokens
+// with the others, which have the same queries; the first of them add all up in LDS.
+template <typename T, int W, int SUB, bool BIG, int PW, int WAVES, bool SHARE>
 __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
     tile_paged4_kernel(QueryArgs a, Paged4Rows rows, TileCut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr bool CENTRE = P == 2;
   constexpr int D = 32 * W, HALF = D / 2, KF = 2 * W, RT = (W + 1) / 2, kTokens4 = 32 * SUB;
-  constexpr int PAIRS = WAVES / (kTileRows / 32);  // waves of the same queries
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % (kTileRows / 32);
-  const int which = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / (kTileRows / 32);
+  const int lane = threadIdx.x % 64, row_waves = SHARE ? cut.row_waves : WAVES, sharers = WAVES / row_waves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % row_waves;
+  const int which = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / row_waves;
   const int n = lane % 32, hf = lane / 32;
   const PagedArgs& p = rows.a;
   // neighbouring blocks of an XCD share keys and values; the longest rows first
@@ -60,10 +60,10 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
   if (chunk >= chunks) return;
   lo = uniform(lo + chunk * share * kTokens4);
   hi = uniform(chunk + 1 < chunks ? lo + share * kTokens4 : hi);
-  if constexpr (PAIRS == 2) {
-    const int64_t middle = lo + (ceil_div(hi - lo, kTokens4) + 1) / 2 * kTokens4;
-    lo = which ? middle : lo;
-    hi = which ? hi : middle < hi ? middle : hi;
+  if constexpr (SHARE) {
+    const int64_t each = ceil_div(ceil_div(hi - lo, kTokens4), sharers) * kTokens4;
+    lo += which * each;
+    hi = lo + each < hi ? lo + each : hi;
   }
 
   // the lane's query: of fragment j, values 8 W hf + 4 j + {0, 2, 1, 3}, and those + HALF
@@ -372,40 +372,53 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
   // codes were 2^-18 as large, weights 2^8 times
   l = sum_halves(l);
   float base = sum_halves(lows) - (PW == 1 ? sum_halves(sumw) * 0x1p-5f : 0.0f), unit = 0x1p10f;
-  if constexpr (PAIRS == 2) {
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // [waves][D + 2][32]
-    float* const its = lds + wave * ((D + 2) * 32) + n;
+  if constexpr (SHARE) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // [sharers - 1][row_waves][D + 2][32]
+    const int size = (D + 2) * 32;
+    float* const theirs = lds + wave * size + n;  // of the second; the others' are row_waves * size on
     auto place = [&](int i, int h, int e) { return (32 * i + 8 * (e / 4) + 4 * hf + e % 4 + h * HALF) * 32; };
     auto there = [&](int i, int e) { return 32 * i + 8 * (e / 4) + 4 * hf < HALF; };
     if (which) {
+      float* const to = theirs + (which - 1) * row_waves * size;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (there(i, e)) its[place(i, h, e)] = __builtin_fmaf(acc[i][h][e], unit, base);
+            if (there(i, e)) to[place(i, h, e)] = __builtin_fmaf(acc[i][h][e], unit, base);
       if (hf == 0) {
-        its[D * 32] = r;
-        its[D * 32 + 32] = l;
+        to[D * 32] = r;
+        to[D * 32 + 32] = l;
       }
     }
     __syncthreads();
     if (which) return;
-    const float r1 = its[D * 32], l1 = its[D * 32 + 32], top = fmaxf(r, r1);
-    const float by0 = __builtin_amdgcn_exp2f(r - top), by1 = __builtin_amdgcn_exp2f(r1 - top);
+    float top = r;
+    for (int k = 0; k < sharers - 1; ++k) top = fmaxf(top, theirs[k * row_waves * size + D * 32]);
+    float by = __builtin_amdgcn_exp2f(r - top);
     r = top;
-    l = l * by0 + l1 * by1;
-    unit *= by0;
-    base *= by0;
+    l *= by;
+    unit *= by;
+    base *= by;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (there(i, e))
-            acc[i][h][e] = __builtin_fmaf(its[place(i, h, e)], by1, __builtin_fmaf(acc[i][h][e], unit, base));
+        for (int e = 0; e < 16; ++e) acc[i][h][e] = __builtin_fmaf(acc[i][h][e], unit, base);
+    for (int k = 0; k < sharers - 1; ++k) {
+      const float* from = theirs + k * row_waves * size;
+      by = __builtin_amdgcn_exp2f(from[D * 32] - top);
+      l += from[D * 32 + 32] * by;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (there(i, e)) acc[i][h][e] = __builtin_fmaf(from[place(i, h, e)], by, acc[i][h][e]);
+    }
     unit = 1.0f;
     base = 0.0f;
   }
@@ -452,16 +465,16 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
       }
 }
 
-template <typename T, int W, bool BIG, int PW, int WAVES>
+template <typename T, int W, bool BIG, int PW, int WAVES, bool SHARE>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileCut& cut, int64_t pairs) {
   const char* who = "cache4_attention";
   const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cut.tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
-  constexpr int SUB = W <= (sizeof(T) == 4 ? 2 : 4) ? 2 : 1;
-  constexpr unsigned bytes = WAVES * 32 == kTileRows ? 0 : kTileRows * (32 * W + 2) * 4;
+  constexpr int SUB = W <= (sizeof(T) == 4 ? 2 : SHARE && !BIG && PW == 2 ? 3 : 4) ? 2 : 1;  // (what spills nothing)
+  const unsigned bytes = SHARE ? (WAVES - cut.row_waves) * (32 * W + 2) * 32 * 4 : 0;
   if (bytes > 65536)
-    KK_TRY(allow_large_lds(reinterpret_cast<const void*>(tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES>)));
-  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES>), grid, dim3(64 * WAVES), bytes, ctx().stream, a, rows, cut);
+    KK_TRY(allow_large_lds(reinterpret_cast<const void*>(tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES, SHARE>)));
+  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES, SHARE>), grid, dim3(64 * WAVES), bytes, ctx().stream, a, rows, cut);
   KK_TRY(check_launch("tile_paged4_kernel"));
   if (cut.splits == 1) return KK_OK;
   KK_LAUNCH((join_parts_kernel<T, Paged4Rows>), dim3(static_cast<unsigned>(pairs * cut.tiles * (kTileRows / (kTileThreads / 64)))),
@@ -469,23 +482,29 @@ static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileC
   return check_launch("join_parts_kernel");
 }
 
-// Eight waves a block, of which one fits a CU, where whole rounds of a tile's blocks
-// take five eighths of the CUs or more (heads of 128, 128 blocks: 127 us with four waves,
-// 105 with eight; 176: 67 and 56; heads of 64 in fp32, 144 blocks: 47 and 50); else four,
-// and as many blocks as fit two a CU.
+// Tokens shared by the waves of a block where it has 64 queries at most (16 sequences of
+// 64 queries a key head over up to 4000 tokens: 115 us where the other waves idle,
+// 65 here), and by eight waves, of which one block fits a CU, where whole rounds of a
+// tile's blocks take five eighths of the CUs or more (heads of 128, 128 blocks: 127 us
+// with four waves, 105 with eight; 176: 67 and 56; heads of 64 in fp32, 144 blocks: 47
+// and 50); else four waves, and as many blocks as fit two a CU.
 template <typename T, int W, bool BIG, int PW>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
   const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * rows.a.heads, tiles = ceil_div(queries, kTileRows);
+  const int64_t cus = ctx().num_cus, blocks = pairs * tiles;
   TileCut cut{};
   cut.rows = queries;
   cut.tiles = static_cast<int>(tiles);
+  cut.row_waves = queries <= 32 ? 1 : queries <= 64 ? 2 : 4;
   if constexpr (W <= 4)
-    if (const int64_t cus = ctx().num_cus, blocks = pairs * tiles; cus / blocks * blocks * 8 >= cus * 5) {
-      plan_parts(blocks, tokens, kLeastTokens4, a.D, cus - blocks + 1, &cut);
-      return launch_tiles4<T, W, BIG, PW, 8>(a, rows, cut, pairs);
+    if (cut.row_waves < 4 || cus / blocks * blocks * 8 >= cus * 5) {
+      plan_parts(blocks, tokens, kLeastTokens4, a.D, blocks < cus ? cus - blocks + 1 : 1, &cut);
+      return launch_tiles4<T, W, BIG, PW, 8, true>(a, rows, cut, pairs);
     }
-  plan_parts(pairs * tiles, tokens, kLeastTokens4, a.D, 2 * ctx().num_cus, &cut);
-  return launch_tiles4<T, W, BIG, PW, 4>(a, rows, cut, pairs);
+  plan_parts(blocks, tokens, kLeastTokens4, a.D, 2 * cus, &cut);
+  if constexpr (W > 4)
+    if (cut.row_waves < 4) return launch_tiles4<T, W, BIG, PW, 4, true>(a, rows, cut, pairs);
+  return launch_tiles4<T, W, BIG, PW, 4, false>(a, rows, cut, pairs);
 }
 
 // Weights of fp16 queries in one half, where many queries keep the matrix cores
