@@ -5,6 +5,7 @@ returns a new DeviceTensor.  Shapes are computed here with numpy's rules;
 the kernels re-validate them before launching.
 """
 import ctypes
+import math
 
 import numpy as np
 
@@ -594,6 +595,14 @@ def _rows(t):
     return t if even and (t.shape[-1] == 1 or t.strides[-1] == 1) else t.contiguous()
 
 
+def _results(*parts):
+    """Fresh tensors of (shape, dtype) each: in one buffer where they are small; large ones apart, so that
+    one that is kept keeps no other's memory."""
+    if math.prod(parts[0][0]) <= 16384:
+        return DeviceTensor._together(*parts)
+    return [DeviceTensor._fresh(*part) for part in parts]
+
+
 def qk_norm_rotary(q, k, positions=None, turns=None, q_weight=None, k_weight=None, eps=1e-6,
                    interleaved=False, amplitude=1.0):
     """(q, k) with each head's norm (where a weight [D] is given) and the
@@ -669,8 +678,10 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     """The root-mean-square norm of the rows of x [.., N] times weight [N], of
     x's dtype; with a residual, (the norm of x + residual, x + residual)."""
     x, residual, weight = _rows(x), _rows(residual), _flat(weight)
-    out = DeviceTensor._fresh(x.shape, x.dtype)
-    total = None if residual is None else DeviceTensor._fresh(residual.shape, residual.dtype)
+    if residual is None:
+        out, total = DeviceTensor._fresh(x.shape, x.dtype), None
+    else:
+        out, total = _results((x.shape, x.dtype), (residual.shape, residual.dtype))
     _lib.call("kk_rms_norm", out.desc(), _d(total), x.desc(), _d(residual), _d(weight), float(eps))
     return out if total is None else (out, total)
 
@@ -680,9 +691,9 @@ def rms_norm_quant(x, weight=None, residual=None, eps=1e-6):
     an 8-bit product (`matmul_integer_scaled`, its rows times the scales); with a
     residual, (codes, scales, x + residual)."""
     x, residual, weight = _rows(x), _rows(residual), _flat(weight)
-    codes = DeviceTensor._fresh(x.shape, _I8)
-    scales = DeviceTensor._fresh(x.shape[:-1] + (1,), _F32)
-    total = None if residual is None else DeviceTensor._fresh(residual.shape, residual.dtype)
+    own = (x.shape, _I8), (x.shape[:-1] + (1,), _F32)
+    codes, scales, total = (*_results(*own), None) if residual is None else \
+        _results(*own, (residual.shape, residual.dtype))
     _lib.call("kk_rms_norm_quant", codes.desc(), scales.desc(), _d(total), x.desc(), _d(residual), _d(weight),
               float(eps))
     return (codes, scales) if total is None else (codes, scales, total)
@@ -696,7 +707,7 @@ def plan_pages(table, starts, counts, free, used, tokens, block, used_out=None):
     granted none.  The new `used` is a tensor of its own, or used_out (which may
     be `used`)."""
     shape = (table.shape[0], int(tokens))
-    slots, positions, lengths, granted, own = DeviceTensor._together(
+    slots, positions, lengths, granted, own = _results(
         (shape, _I64), (shape, _I32), (shape[:1], _I32), (shape[:1], _I32), ((1,), _I32))
     used_out = own if used_out is None else used_out
     _lib.call("kk_plan_pages", table.desc(), slots.desc(), positions.desc(), lengths.desc(), granted.desc(),
@@ -743,7 +754,7 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
     [B, V] with the given numbers uniforms [B] in [0, 1) (include/kk.h,
     kk_sample); a temperature of 0 takes the largest logit."""
     logits = _inner(logits)
-    tokens, logs = DeviceTensor._together((logits.shape[:1], _I32), (logits.shape[:1], _F32))
+    tokens, logs = _results((logits.shape[:1], _I32), (logits.shape[:1], _F32))
     _lib.call("kk_sample", tokens.desc(), logs.desc(), logits.desc(), uniforms.desc(), _d(temperature), _d(top_k),
               _d(top_p), _d(min_p))
     return tokens, logs
