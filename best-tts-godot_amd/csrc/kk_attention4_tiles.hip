@@ -15,17 +15,16 @@ constexpr int kLeastTokens4 = 256;  // of a block that shares them
 // the registers that multiply them (its three neighbours read the same ones):
 // nothing goes through LDS, and no wave waits for another.  Bound by the vector units
 // (codes, exponentials, weights to halves) beside the products: 2 x 1531 queries of 32
-// heads of 128 over up to 4099 tokens in 246 us, 470 TFLOP/s of fp16.
+// heads of 128 over up to 4099 tokens in 279 us, 415 TFLOP/s of fp16.
 //
 // Keys' lowest values (beside fp32 queries: their middles, in two halves) times the
-// query's sum, in three halves, are added by a product of their own.  Queries,
-// weights and codes as there; PW 1: weights are rounded to one half, values count as
-// step (code - 8) + middle, and 8 times the rounded weights' sum is taken off in the
-// end, so that a weight's rounding acts on what a value differs from its middle by.
+// query's sum, in three halves, are added by a product of their own.  Queries, codes and
+// weights as there: in one half a weight (246 us for the queries above) outputs are up
+// to 13 times as far off as their own rounding to fp16.
 //
 // SHARE: cut.row_waves waves (4, 2 or 1: as many as have queries) share the tokens
 // with the others, which have the same queries; the first of them add all up in LDS.
-template <typename T, int W, int SUB, bool BIG, int PW, int WAVES, bool SHARE>
+template <typename T, int W, int SUB, bool BIG, int WAVES, bool SHARE>
 __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
     tile_paged4_kernel(QueryArgs a, Paged4Rows rows, TileCut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
@@ -196,9 +195,8 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
   };
 
   f16v acc[RT][2];
-  float r = -3.4028235e38f, l = 0.0f, lows = 0.0f, sumw = 0.0f;
+  float r = -3.4028235e38f, l = 0.0f, lows = 0.0f;
   const float less = minus_one();
-  const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -250,7 +248,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
     for (int k = 0; k < SUB; ++k) {
       there[k] = pg[k] >= 0;
       none = none || !there[k];
-      const float vstep = there[k] ? low_half(vs1[k]) : 0.0f, vlow = there[k] ? base4<CENTRE || PW == 1>(vs1[k]) : 0.0f;
+      const float vstep = there[k] ? low_half(vs1[k]) : 0.0f, vlow = there[k] ? base4<CENTRE>(vs1[k]) : 0.0f;
       const uint32_t bits = __float_as_uint(vstep) & 0x7fffffffu;
       ev[k] = bits ? static_cast<float>(static_cast<int>(bits >> 23) - 126) : -INFINITY;
       most = fmaxf(most, ev[k]);
@@ -300,7 +298,6 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
       r = sized;
       l *= keep;
       lows *= keep;
-      sumw *= keep;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -309,7 +306,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
           acc[i][1][e] *= keep;
         }
     }
-    h8 pf[SUB][2][PW];
+    h8 pf[SUB][2][2];
 #pragma unroll
     for (int k = 0; k < SUB; ++k) {
       float x[16];
@@ -341,11 +338,10 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
         const int i = j / 4 * 4 + j % 4 / 2;
         h2 w0, w1;
         split4(x[i], x[i + 2], less, &w0, &w1);
-        if constexpr (PW == 1) sumw = __builtin_amdgcn_fdot2(w0, ones, sumw, false);
         pf[k][j / 8][0][j % 8] = w0[0];
         pf[k][j / 8][0][j % 8 + 1] = w0[1];
-        pf[k][j / 8][PW - 1][j % 8] = PW == 2 ? w1[0] : w0[0];
-        pf[k][j / 8][PW - 1][j % 8 + 1] = PW == 2 ? w1[1] : w0[1];
+        pf[k][j / 8][1][j % 8] = w1[0];
+        pf[k][j / 8][1][j % 8 + 1] = w1[1];
       }
     }
 #pragma unroll
@@ -360,7 +356,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
           const h8 low = halves8(c[2 * u].low[0], c[2 * u].low[1], c[2 * u + 1].low[0], c[2 * u + 1].low[1]);
           const h8 high = halves8(c[2 * u].high[0], c[2 * u].high[1], c[2 * u + 1].high[0], c[2 * u + 1].high[1]);
 #pragma unroll
-          for (int e = PW - 1; e >= 0; --e) {
+          for (int e = 1; e >= 0; --e) {
             acc[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(low, pf[k][u][e], acc[i][0], 0, 0, 0);
             acc[i][1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(high, pf[k][u][e], acc[i][1], 0, 0, 0);
           }
@@ -371,7 +367,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
 
   // codes were 2^-18 as large, weights 2^8 times
   l = sum_halves(l);
-  float base = sum_halves(lows) - (PW == 1 ? sum_halves(sumw) * 0x1p-5f : 0.0f), unit = 0x1p10f;
+  float base = sum_halves(lows), unit = 0x1p10f;
   if constexpr (SHARE) {
     extern __shared__ __attribute__((aligned(16))) float lds[];  // [sharers - 1][row_waves][D + 2][32]
     const int size = (D + 2) * 32;
@@ -465,16 +461,16 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
       }
 }
 
-template <typename T, int W, bool BIG, int PW, int WAVES, bool SHARE>
+template <typename T, int W, bool BIG, int WAVES, bool SHARE>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileCut& cut, int64_t pairs) {
   const char* who = "cache4_attention";
   const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cut.tiles), static_cast<unsigned>(pairs));
   KK_TRY(check_xcd_grid(grid, who));
-  constexpr int SUB = W <= (sizeof(T) == 4 ? 2 : SHARE && !BIG && PW == 2 ? 3 : 4) ? 2 : 1;  // (what spills nothing)
+  constexpr int SUB = W <= (sizeof(T) == 4 ? 2 : SHARE && !BIG ? 3 : 4) ? 2 : 1;  // (what spills nothing)
   const unsigned bytes = SHARE ? (WAVES - cut.row_waves) * (32 * W + 2) * 32 * 4 : 0;
   if (bytes > 65536)
-    KK_TRY(allow_large_lds(reinterpret_cast<const void*>(tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES, SHARE>)));
-  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, PW, WAVES, SHARE>), grid, dim3(64 * WAVES), bytes, ctx().stream, a, rows, cut);
+    KK_TRY(allow_large_lds(reinterpret_cast<const void*>(tile_paged4_kernel<T, W, SUB, BIG, WAVES, SHARE>)));
+  KK_LAUNCH((tile_paged4_kernel<T, W, SUB, BIG, WAVES, SHARE>), grid, dim3(64 * WAVES), bytes, ctx().stream, a, rows, cut);
   KK_TRY(check_launch("tile_paged4_kernel"));
   if (cut.splits == 1) return KK_OK;
   KK_LAUNCH((join_parts_kernel<T, Paged4Rows>), dim3(static_cast<unsigned>(pairs * cut.tiles * (kTileRows / (kTileThreads / 64)))),
@@ -488,7 +484,7 @@ static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileC
 // tile's blocks take five eighths of the CUs or more (heads of 128, 128 blocks: 127 us
 // with four waves, 105 with eight; 176: 67 and 56; heads of 64 in fp32, 144 blocks: 47
 // and 50); else four waves, and as many blocks as fit two a CU.
-template <typename T, int W, bool BIG, int PW>
+template <typename T, int W, bool BIG>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
   const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * rows.a.heads, tiles = ceil_div(queries, kTileRows);
   const int64_t cus = ctx().num_cus, blocks = pairs * tiles;
@@ -499,22 +495,12 @@ static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tok
   if constexpr (W <= 4)
     if (cut.row_waves < 4 || cus / blocks * blocks * 8 >= cus * 5) {
       plan_parts(blocks, tokens, kLeastTokens4, a.D, blocks < cus ? cus - blocks + 1 : 1, &cut);
-      return launch_tiles4<T, W, BIG, PW, 8, true>(a, rows, cut, pairs);
+      return launch_tiles4<T, W, BIG, 8, true>(a, rows, cut, pairs);
     }
   plan_parts(blocks, tokens, kLeastTokens4, a.D, 2 * cus, &cut);
   if constexpr (W > 4)
-    if (cut.row_waves < 4) return launch_tiles4<T, W, BIG, PW, 4, true>(a, rows, cut, pairs);
-  return launch_tiles4<T, W, BIG, PW, 4, false>(a, rows, cut, pairs);
-}
-
-// Weights of fp16 queries in one half, where many queries keep the matrix cores
-// busy, or in two (2 x 1531 queries of 32 heads of 128 over up to 4099 tokens: 246
-// and 305 us, outputs 1.4 times and as far off as their own rounding to fp16).
-template <typename T, int W, bool BIG>
-static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
-  if constexpr (sizeof(T) == 2 && W <= 4)
-    if (int64_t{a.T} * a.group > 512) return launch_tiles4<T, W, BIG, 1>(a, rows, tokens);
-  return launch_tiles4<T, W, BIG, 2>(a, rows, tokens);
+    if (cut.row_waves < 4) return launch_tiles4<T, W, BIG, 4, true>(a, rows, cut, pairs);
+  return launch_tiles4<T, W, BIG, 4, false>(a, rows, cut, pairs);
 }
 
 template <typename T, bool BIG>

@@ -634,7 +634,9 @@ int kk_cache4_append(const kk_tensor* k_codes, const kk_tensor* k_scales, const 
 int kk_cache4_values(const kk_tensor* out_k, const kk_tensor* out_v, const kk_tensor* k_codes,
                      const kk_tensor* k_scales, const kk_tensor* v_codes,
                      const kk_tensor* v_scales);
-/* kk_cache_attention over such a cache. */
+/* kk_cache_attention over such a cache.  Products are those of fp16 with sums in fp32:
+ * fp16 queries as they are, fp32 ones and the weights (each times its value's step) as
+ * the sums of two halves, 22 bits, however many queries a call has. */
 int kk_cache4_attention(const kk_tensor* out, const kk_tensor* q, const kk_tensor* k_codes,
                         const kk_tensor* k_scales, const kk_tensor* v_codes,
                         const kk_tensor* v_scales, const kk_tensor* table,
