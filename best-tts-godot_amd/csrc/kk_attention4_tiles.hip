@@ -17,8 +17,9 @@ constexpr int kLeastTokens4 = 256;  // of a block that shares them
 // (codes, exponentials, weights to halves) beside the products: 2 x 1531 queries of 32
 // heads of 128 over up to 4099 tokens in 279 us, 415 TFLOP/s of fp16.
 //
-// Keys' lowest values (beside fp32 queries: their middles, in two halves) times the
-// query's sum, in three halves, are added by a product of their own.  Queries, codes and
+// Keys' lowest values (beside fp32 queries: their middles, in two halves and, past
+// 2^15, 16 times a third, since a step times 8 passes fp16's range) times the query's
+// sum, in three halves, are added by a product of their own.  Queries, codes and
 // weights as there: in one half a weight (246 us for the queries above) outputs are up
 // to 13 times as far off as their own rounding to fp16.
 //
@@ -29,6 +30,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
     tile_paged4_kernel(QueryArgs a, Paged4Rows rows, TileCut cut) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // halves of a query
   constexpr bool CENTRE = P == 2;
+  constexpr int DOWN = CENTRE ? 11 : 8;  // (16 times a sum of 256 values below 2^14 stays a half)
   constexpr int D = 32 * W, HALF = D / 2, KF = 2 * W, RT = (W + 1) / 2, kTokens4 = 32 * SUB;
   const int lane = threadIdx.x % 64, row_waves = SHARE ? cut.row_waves : WAVES, sharers = WAVES / row_waves;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % row_waves;
@@ -103,14 +105,15 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
         qf[j][0][e] = top16;
         if constexpr (P == 2) qf[j][P - 1][e] = static_cast<_Float16>(y - static_cast<float>(top16));
       }
-    // scores come out 2^(up - 8) too large (codes are 2^-18 as large, steps 2^10 times)
-    all = sum_halves(all) * 0x1p-8f;
-    cq = a.scale == 0.0f ? 1.0f : ldexpf(__builtin_fabsf(a.scale), 8 - up);
+    // scores come out 2^(up - DOWN) too large (codes are 2^-18 as large, steps 2^(18 - DOWN) times)
+    all = sum_halves(all) * (CENTRE ? 0x1p-11f : 0x1p-8f);
+    cq = a.scale == 0.0f ? 1.0f : ldexpf(__builtin_fabsf(a.scale), DOWN - up);
 #pragma unroll
     for (int e = 0; e < 3; ++e) {
       const _Float16 part = static_cast<_Float16>(all);
       sum_f[e] = hf ? static_cast<_Float16>(0.0f) : part;
       if (CENTRE && e < 2) sum_f[3 + e] = sum_f[e];
+      if (CENTRE) sum_f[5 + e] = sum_f[e] * static_cast<_Float16>(16.0f);
       all -= static_cast<float>(part);
     }
   }
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
 #pragma unroll
         for (int e = P - 1; e >= 0; --e) s[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[j][e], s[k], 0, 0, 0);
       }
-      const float kstep = key_step(ks1[k]) * 0x1p10f;
+      const float kstep = key_step(ks1[k]) * (CENTRE ? 0x1p7f : 0x1p10f);
       each<0, 16>([&](auto c) {
         constexpr int J = decltype(c)::value;
         s[k][J] *= of_row<J>(kstep);
@@ -235,9 +238,12 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
       h8 base = {};
       if constexpr (CENTRE) {
         const float all = hf ? 0.0f : base4<true>(kl1[k]);
-        const _Float16 most16 = static_cast<_Float16>(all);
+        const _Float16 far16 = static_cast<_Float16>(__builtin_fabsf(all) >= 0x1p15f ? all * 0x1p-4f : 0.0f);
+        const float near = __builtin_fmaf(static_cast<float>(far16), -16.0f, all);
+        const _Float16 most16 = static_cast<_Float16>(near);
         base[0] = base[1] = base[2] = most16;
-        base[3] = base[4] = static_cast<_Float16>(all - static_cast<float>(most16));
+        base[3] = base[4] = static_cast<_Float16>(near - static_cast<float>(most16));
+        base[5] = base[6] = base[7] = far16;
       } else {
         const uint32_t low = hf ? 0u : (kl1[k] >> 16) * 0x10001u;
         base = halves8(low, low & 0xffffu, 0u, 0u);

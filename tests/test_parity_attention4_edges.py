@@ -1,0 +1,28 @@
+"""Attention over the 4-bit cache at the ends of its types: scales near fp16's
+largest, queries of nothing, batches that a block's threads go through."""
+import numpy as np
+import pytest
+
+from conftest import rng
+from test_parity_attention4 import check, filled, pool, run
+from test_parity_serve import DTYPES
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T", [1, 60, 200])
+@pytest.mark.parametrize("step,low", [(9000, 0), (8200, -30), (65000, 65504), (7000, 60000), (9000, -65504), (4094, 0)])
+def test_keys_of_fp16s_largest_sizes(gpu, t, T, step, low):
+    """Some keys' middles, low + 8 step, pass fp16's range: they are values like others, to the bits of fp32."""
+    kk = gpu
+    r = rng(abs(step + low) + T)
+    dim, block, n = 64, 16, 300
+    table, pages = pool(r, 1, -(-n // block))
+    parts = filled(r, pages, 2, dim, block)
+    far = r.random(parts[1].shape[:3]) < 0.2
+    parts[1][far] = step, low
+    q = r.normal(size=(1, T, 4, dim)).astype(t)
+    scale = 1e-6
+    out = run(kk, q, parts, table, np.array([n], np.int32), scale=scale)
+    check(out[0], q[0], parts, table[0], n, scale)
