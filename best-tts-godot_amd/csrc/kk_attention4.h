@@ -46,6 +46,13 @@ __device__ __forceinline__ void each(F&& f) {
   }
 }
 
+// What scores are multiplied by, |scale| 2^by: a normal number, since masked ones are
+// -inf and 0 times them NaN.  (Below 2^-126, for queries of zeros or of subnormal values,
+// it says nothing: scores are below 2^36 before it.)
+__device__ __forceinline__ float unscaled4(float scale, int by) {
+  return scale == 0.0f ? 1.0f : fmaxf(ldexpf(__builtin_fabsf(scale), by), 0x1p-126f);
+}
+
 // A key's step, NaN where it or the lowest value is not finite (a key with an
 // infinite one is NaN in its codes of 0).
 __device__ __forceinline__ float key_step(uint32_t scale) {

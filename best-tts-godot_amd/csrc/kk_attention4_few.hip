@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kFew4Threads, NT * W * sizeof(T) <= 28 ? 2 : 1
     all += __shfl_xor(all, 32, 64);
     // scores come out 2^(up - 18) too large
     sum[nt] = all * 0x1p-18f;
-    cq[nt] = a.scale == 0.0f ? 1.0f : ldexpf(__builtin_fabsf(a.scale), 18 - up);
+    cq[nt] = unscaled4(a.scale, 18 - up);
   }
 
   const int shift = __builtin_ctz(p.block);

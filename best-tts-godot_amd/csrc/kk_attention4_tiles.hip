@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
       }
     // scores come out 2^(up - DOWN) too large (codes are 2^-18 as large, steps 2^(18 - DOWN) times)
     all = sum_halves(all) * (CENTRE ? 0x1p-11f : 0x1p-8f);
-    cq = a.scale == 0.0f ? 1.0f : ldexpf(__builtin_fabsf(a.scale), DOWN - up);
+    cq = unscaled4(a.scale, DOWN - up);
 #pragma unroll
     for (int e = 0; e < 3; ++e) {
       const _Float16 part = static_cast<_Float16>(all);

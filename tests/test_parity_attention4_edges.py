@@ -26,3 +26,24 @@ def test_keys_of_fp16s_largest_sizes(gpu, t, T, step, low):
     scale = 1e-6
     out = run(kk, q, parts, table, np.array([n], np.int32), scale=scale)
     check(out[0], q[0], parts, table[0], n, scale)
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("T,group", [(1, 2), (5, 2), (40, 1), (300, 2)])
+@pytest.mark.parametrize("scale", [1e-3, 1e-6, 1e-10, 1e-30, -1e-10])
+def test_queries_of_nothing_under_a_small_scale(gpu, t, T, group, scale):
+    """A query of zeros, or of fp32's smallest values, weighs what it sees alike, whatever the scale is."""
+    kk = gpu
+    r = rng(T)
+    dim, block, n = 64, 32, 437
+    table, pages = pool(r, 1, -(-n // block))
+    parts = filled(r, pages, 2, dim, block)
+    q = r.normal(size=(1, T, 2 * group, dim)).astype(t)
+    q[:, ::2, 0] = 0
+    q[:, -1] = 0
+    if t == np.float32:
+        q[:, T // 2, 1] = 1e-44
+    for window in (0, 130):
+        out = run(kk, q, parts, table, np.array([n], np.int32), scale=scale, window=window)
+        some = np.unique(np.concatenate([[0, T - 1, T // 2], r.integers(0, T, 12)]))
+        check(out[0], q[0], parts, table[0], n, scale, window, queries=some)
