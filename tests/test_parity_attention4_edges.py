@@ -47,3 +47,24 @@ def test_queries_of_nothing_under_a_small_scale(gpu, t, T, group, scale):
         out = run(kk, q, parts, table, np.array([n], np.int32), scale=scale, window=window)
         some = np.unique(np.concatenate([[0, T - 1, T // 2], r.integers(0, T, 12)]))
         check(out[0], q[0], parts, table[0], n, scale, window, queries=some)
+
+
+@pytest.mark.parametrize("t", DTYPES)
+def test_a_batch_past_a_blocks_threads(gpu, t):
+    """600 sequences, some of several parts, where a thread of the block goes through three of them."""
+    kk = gpu
+    r = rng(600)
+    B, block, dim, longest = 600, 64, 64, 6000
+    lengths = np.where(r.random(B) < 0.1, 0, r.integers(1, 90, B)).astype(np.int32)
+    far = [0, 1, 2, 5, 191, 192, 383, 384, 597, 599]
+    lengths[far] = longest - np.arange(len(far)) * 401
+    # pages are shared: what a sequence reads is checked, not who owns it
+    pages = 200
+    table = r.integers(0, pages, (B, -(-longest // block))).astype(np.int32)
+    parts = filled(r, pages, 1, dim, block)
+    q = r.normal(size=(B, 1, 3, dim)).astype(t)
+    out = run(kk, q, parts, table, lengths, scale=0.2)
+    assert not out[lengths == 0].any()
+    for b in sorted({*far, *r.integers(0, B, 20).tolist()}):
+        if lengths[b]:
+            check(out[b], q[b], parts, table[b], int(lengths[b]), 0.2, what=f"sequence {b}")
