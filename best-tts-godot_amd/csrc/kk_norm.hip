@@ -38,10 +38,10 @@ __device__ __forceinline__ void load_weights(const NormArgs& a, int at, float (&
   }
 }
 
-// The sum, or the largest, of the values of a row's LANES threads.
+// The sum, or the largest (NaN where one is), of the values of a row's LANES threads.
 template <int LANES>
 __device__ __forceinline__ double row_all(double v, bool largest, double* part) {
-  auto join = [&](double a, double b) { return largest ? (b > a ? b : a) : a + b; };
+  auto join = [&](double a, double b) { return largest ? (b > a || b != b ? b : a) : a + b; };
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) v = join(v, __shfl_xor(v, off, 64));
   if constexpr (LANES > 64) {
@@ -113,6 +113,13 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rms_norm_kernel(Nor
         load_weights<__half>(a, at, w[c]);
     }
   }
+  float poison = 0.0f;  // NaN where a weight is not finite
+  if (CODES && a.w) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) poison = __builtin_fmaf(w[c][e], 0.0f, poison);
+  }
   H h[NCH][VEC], squares = 0;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
@@ -142,7 +149,6 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rms_norm_kernel(Nor
     squares = row_sum<LANES>(squares, part[0]);
   }
   const H by = H(1) / sqrt(squares / static_cast<H>(a.N) + static_cast<H>(a.eps));
-  H top = 0;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     if (!a.w) continue;
@@ -153,13 +159,22 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rms_norm_kernel(Nor
     }
   }
   if constexpr (CODES) {
+    double top = 0.0;
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) top = fmax(top, fabs(h[c][e]));
+    // (fmax drops NaN, and a weight of 0 an infinity: squares that are not finite hold these)
+    if (!(poison == 0.0f && squares < INFINITY)) top = NAN;
     top = row_all<LANES>(top, true, part[1]);
-    if (lane == 0) a.scale[row] = static_cast<float>(top * by / 127.0);
+    if (lane == 0) a.scale[row] = top == 0.0 ? 0.0f : static_cast<float>(top * by / 127.0);
     const double code = top > 0.0 ? 127.0 / top : 0.0;
+    if (!(top > 0.0)) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[c][e] = 0.0;
+    }
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll

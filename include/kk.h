@@ -580,7 +580,8 @@ int kk_rms_norm(const kk_tensor* out, const kk_tensor* sum, const kk_tensor* x,
 /* The same into 8 bits for kk_matmul_integer_scaled, with a scale for each row:
  * scales f32 [rows], codes int8 like x,
  *   scale = max |y| / 127,   code = rint(y / scale)  (a row of zeros: 0 and 0)
- * of the exact quotient, ties to even.  A row that is not finite has the scale NaN. */
+ * of the exact quotient, ties to even.  A row of which x, residual or the weights are not
+ * finite has the scale NaN and codes of 0. */
 int kk_rms_norm_quant(const kk_tensor* codes, const kk_tensor* scales, const kk_tensor* sum,
                       const kk_tensor* x, const kk_tensor* residual, const kk_tensor* weight,
                       float eps);
