@@ -228,6 +228,22 @@ static int check_ints(const kk_tensor* t, const char* name, int dtype, int64_t n
   return KK_OK;
 }
 
+// Whether a tensor in one piece and one of one axis share memory.
+static bool shared(const kk_tensor* piece, const kk_tensor* axis) {
+  if (numel(piece) == 0 || numel(axis) == 0) return false;
+  const int64_t size = dtype_size(axis->dtype), n = axis->shape[0];
+  int64_t step = n > 1 ? axis->strides[0] * size : 0;
+  int64_t first = reinterpret_cast<int64_t>(axis->data);
+  const int64_t lo = reinterpret_cast<int64_t>(piece->data), hi = lo + numel(piece) * dtype_size(piece->dtype);
+  if (step < 0) {  // from its other end
+    first += (n - 1) * step;
+    step = -step;
+  }
+  // its first value that ends behind the piece's start
+  const int64_t i = first + size > lo ? 0 : step ? (lo - size - first) / step + 1 : n;
+  return i < n && first + i * step < hi;
+}
+
 static int check_table(const kk_tensor* table, int64_t block, int64_t* stride, int* shift, const char* who) {
   KK_TRY(check_tensor(table, "table"));
   if (table->dtype != KK_I32 || table->rank != 2)
@@ -277,10 +293,12 @@ int kk_plan_pages(const kk_tensor* table, const kk_tensor* slots, const kk_tenso
   KK_TRY(check_ints(free, "free", KK_I32, -1, who));
   KK_TRY(check_ints(used, "used", KK_I32, 1, who));
   KK_TRY(check_ints(used_out, "used_out", KK_I32, 1, who));
-  if ((numel(lengths) && lengths->data == starts->data) ||
-      (counts && numel(granted) && (granted->data == counts->data || lengths->data == counts->data)) ||
-      (numel(granted) && granted->data == starts->data))
-    return set_error(KK_E_ARG, "%s: lengths and granted must not be starts or counts", who);
+  // (a block reads the starts and counts of sequences that another may have answered already)
+  const kk_tensor* read[4] = {starts, counts, free, used};
+  for (const kk_tensor* t : read)
+    if (t && (shared(lengths, t) || shared(granted, t)))
+      return set_error(KK_E_ARG, "%s: lengths and granted must not be starts or counts, nor lie in them, free or used", who);
+  if (shared(lengths, granted)) return set_error(KK_E_ARG, "%s: lengths and granted must not share memory", who);
   if (slots->shape[1] > (1 << 30) || free->shape[0] > 0x7fffffff || a.B > (1 << 30))
     return set_error(KK_E_UNSUPPORTED, "%s: too many tokens, sequences or pages", who);
   KK_TRY(require_ready());

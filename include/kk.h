@@ -600,7 +600,8 @@ int kk_rms_norm_quant(const kk_tensor* codes, const kk_tensor* scales, const kk_
  *   positions [B, T]  starts[b] + t, -1 past granted[b]
  *   used_out [1]      *used and the pages taken (may be `used` itself)
  * all int32 but slots (int64).  A start outside the table makes its sequence empty.
- * lengths and granted must not be starts or counts. */
+ * No output may share memory with another tensor of the call, used_out with used
+ * aside (lengths and granted are looked at for it). */
 int kk_plan_pages(const kk_tensor* table, const kk_tensor* slots, const kk_tensor* positions,
                   const kk_tensor* lengths, const kk_tensor* granted, const kk_tensor* used_out,
                   const kk_tensor* starts, const kk_tensor* counts, const kk_tensor* free,

@@ -1,8 +1,10 @@
-"""The serving decoder's norms at the ends of their types."""
+"""The serving decoder's norms at the ends of their types, and its pages in a
+program's own buffers."""
 import numpy as np
 import pytest
 
 from conftest import assert_bitexact, rng
+from oracle import serve_ops as S
 from test_parity_serve import DTYPES
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +50,26 @@ def test_rms_norm_quant_of_a_row_of_zeros_without_eps(gpu, t, N):
     codes, scales = (kk.to_host(v) for v in kk.ops.rms_norm_quant(kk.to_device(x), eps=0.0))
     assert scales[1] == 0 and not codes[1].any()
     assert (scales[[0, 2]] > 0).all() and (np.abs(codes[[0, 2]]).max(-1) == 127).all()
+
+
+def test_plan_pages_between_the_starts_of_a_wider_buffer(gpu):
+    """Outputs that lie between the strided starts and counts share no memory with them."""
+    kk = gpu
+    r = rng(9)
+    B, T, block, columns = 5, 7, 16, 6
+    starts, counts = r.integers(0, 60, B).astype(np.int32), r.integers(0, T + 1, B).astype(np.int32)
+    host = np.full((B, 20), -9, np.int32)
+    host[:, 3], host[:, 18] = starts, counts
+    wide = kk.to_device(host.reshape(-1))
+    table = r.permutation(B * columns).reshape(B, columns).astype(np.int32)
+    free = r.permutation(40).astype(np.int32)
+    of = dict(starts=wide.slice_axis(0, 3, B * 20, 20), counts=wide.slice_axis(0, 18, B * 20, 20),
+              lengths=wide.slice_axis(0, 4, 4 + B), granted=wide.slice_axis(0, 24, 24 + B))
+    t, slots, positions = kk.to_device(table), kk.DeviceTensor.empty((B, T), np.int64), kk.DeviceTensor.empty((B, T), np.int32)
+    used = kk.to_device(np.array([2], np.int32))
+    kk._lib.call("kk_plan_pages", t.desc(), slots.desc(), positions.desc(), of["lengths"].desc(), of["granted"].desc(),
+                 used.desc(), of["starts"].desc(), of["counts"].desc(), kk.to_device(free).desc(), used.desc(), block)
+    want = S.plan(table, starts, counts, free, 2, T, block)
+    for g, w in zip((slots, positions, of["lengths"], of["granted"], used, t), want):
+        assert np.array_equal(kk.to_host(g).reshape(np.shape(w)), w)
+    assert np.array_equal(kk.to_host(of["starts"]), starts) and np.array_equal(kk.to_host(of["counts"]), counts)
