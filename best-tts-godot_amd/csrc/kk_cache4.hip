@@ -28,10 +28,12 @@ constexpr float kMost4 = 65504.0f;
 // What is cached of x: fp16's range, no NaN.
 __device__ __forceinline__ float cached(float x) { return x != x ? 0.0f : __builtin_amdgcn_fmed3f(x, -kMost4, kMost4); }
 
-// clamp(rint((x - low) / step), 0, 15), of the exact quotient: (x - low) / step in
-// fp32 is within 2^-20 of it (it is below 17: three roundings of a half step of
-// 2^-23 of 16), so only where that lies within 2^-12 of a half does the quotient
-// in 64 bits say which side it is on.
+// clamp(rint((x - low) / step), 0, 15), of the exact quotient.  A difference, a
+// reciprocal and a product in fp32 leave three roundings of 2^-24 of it: where it lies
+// between 0 and 15.5, and so says which code, less than 2^-18.  Only within 2^-12 of a half
+// does the quotient in 64 bits say which side it is on.  Others are clamped, however
+// far off: a step that fp16 rounds to its smallest takes them to 22, a lowest value that
+// it rounds up below 0.
 __device__ __forceinline__ uint32_t code4(float x, float low, float step, float by) {
   const float q = (x - low) * by, r = rintf(q);
   float c = r;
