@@ -652,6 +652,7 @@ int kk_cache4_attention(const kk_tensor* out, const kk_tensor* q, const kk_tenso
  *   those before which less than top_p[b] of the weight kept so far comes
  *                                                           (1 and more: all)
  *   those with w >= min_p[b]                                (0 and less: all)
+ * (the first token always: top_p counts as above 0, min_p as at most 1),
  * and tokens[b] (int32) is the first whose running weight passes uniforms[b] times
  * that of all kept; logs[b] (f32, may be NULL) the logarithm of its share of it.
  * A temperature that is not above 0 takes the largest logit (the first of equal
