@@ -1,11 +1,11 @@
-"""The serving decoder's norms at the ends of their types, and its pages in a
-program's own buffers."""
+"""The serving decoder's norms at the ends of their types, its pages in a program's
+own buffers, its draws under masks that are numbers."""
 import numpy as np
 import pytest
 
 from conftest import assert_bitexact, rng
 from oracle import serve_ops as S
-from test_parity_serve import DTYPES
+from test_parity_serve import DTYPES, check_sample
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,22 @@ def test_plan_pages_between_the_starts_of_a_wider_buffer(gpu):
     for g, w in zip((slots, positions, of["lengths"], of["granted"], used, t), want):
         assert np.array_equal(kk.to_host(g).reshape(np.shape(w)), w)
     assert np.array_equal(kk.to_host(of["starts"]), starts) and np.array_equal(kk.to_host(of["counts"]), counts)
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("V", [3000, 50257, 131072])
+@pytest.mark.parametrize("spread", [0.05, 0.5, 2.0])
+def test_sample_under_a_finite_mask(gpu, t, V, spread):
+    """Some logits of the type's lowest value, or of -1e4, as masks put them: the others then lie in few bins, of more
+    tokens than are put in order."""
+    r = rng(V)
+    f = np.float32
+    for low in (np.finfo(t).min, -1e4):
+        x = (spread * r.normal(size=(5, V))).astype(t)
+        x[r.random((5, V)) < 0.1] = low
+        u = r.random(5).astype(f)
+        for limits in (dict(), dict(top_p=np.array([0.9], f)), dict(top_k=np.array([V // 3], np.int32)),
+                       dict(min_p=np.array([0.2], f), temperature=np.array([0.6], f)),
+                       dict(top_k=np.array([V // 2], np.int64), top_p=np.array([0.7], f), min_p=np.array([0.05], f),
+                            temperature=np.array([1.3], f))):
+            check_sample(gpu, x, u, **limits)
