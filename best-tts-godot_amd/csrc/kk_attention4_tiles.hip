@@ -15,12 +15,12 @@ constexpr int kLeastTokens4 = 256;  // of a block that shares them
 // the registers that multiply them (its three neighbours read the same ones):
 // nothing goes through LDS, and no wave waits for another.  Bound by the vector units
 // (codes, exponentials, weights to halves) beside the products: 2 x 1531 queries of 32
-// heads of 128 over up to 4099 tokens in 279 us, 415 TFLOP/s of fp16.
+// heads of 128 over up to 4099 tokens in 291 us, 400 TFLOP/s of fp16.
 //
 // Keys' lowest values (beside fp32 queries: their middles, in two halves and, past
 // 2^15, 16 times a third, since a step times 8 passes fp16's range) times the query's
 // sum, in three halves, are added by a product of their own.  Queries, codes and
-// weights as there: in one half a weight (246 us for the queries above) outputs are up
+// weights as there: in one half a weight (251 us for the queries above) outputs are up
 // to 13 times as far off as their own rounding to fp16.
 //
 // SHARE: cut.row_waves waves (4, 2 or 1: as many as have queries) share the tokens
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(64 * WAVES, W <= 4 ? 2 : 1)
 
   // of two waves that share vector units one comes first, so that they do not come to
   // multiply, and to wait for the vector units, at the same times (a wave's slot:
-  // bits 0 to 3 of HW_ID; 317 against 305 us)
+  // bits 0 to 3 of HW_ID; 310 against 291 us)
   if (__builtin_amdgcn_s_getreg(4 | 3 << 11) & 1) __builtin_amdgcn_s_setprio(1);
   if (begin < end) {
     find_pages(begin);
@@ -487,9 +487,9 @@ static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, const TileC
 // Tokens shared by the waves of a block where it has 64 queries at most (16 sequences of
 // 64 queries a key head over up to 4000 tokens: 115 us where the other waves idle,
 // 65 here), and by eight waves, of which one block fits a CU, where whole rounds of a
-// tile's blocks take five eighths of the CUs or more (heads of 128, 128 blocks: 127 us
-// with four waves, 105 with eight; 176: 67 and 56; heads of 64 in fp32, 144 blocks: 47
-// and 50); else four waves, and as many blocks as fit two a CU.
+// tile's blocks take five eighths of the CUs or more (fp16 heads of 128, 128 blocks: 148 us
+// with four waves, 124 with eight; 176: 83 and 72; heads of 64 in fp32, 144 blocks: 60
+// and 60); else four waves, and as many blocks as fit two a CU.
 template <typename T, int W, bool BIG>
 static int launch_tiles4(const QueryArgs& a, const Paged4Rows& rows, int64_t tokens) {
   const int64_t queries = int64_t{a.T} * a.group, pairs = a.B * rows.a.heads, tiles = ceil_div(queries, kTileRows);

@@ -1,6 +1,7 @@
 // A paged cache of 4-bit keys and values: tokens into their slots, and what the
-// codes stand for.  Bound by memory (long calls) or by their launch (single
-// tokens).
+// codes stand for.  Bound by memory (the codes' values: 44 MB in 7.4 us), by values that
+// leave a byte a lane (3 x 2051 tokens of 12 heads of 64 in fp32, 43 MB: 15 us, where a
+// copy takes 8.7) or by their launch (single tokens).
 #include "kk_decode.h"
 
 namespace kk {

@@ -573,8 +573,9 @@ int kk_process_logits(const kk_tensor* out, const kk_tensor* logits, const kk_te
  * x, residual, out and sum [.., N], f32 or f16 each (sum of residual's dtype), rows
  * evenly spaced, a row's values next to each other, 1 <= N <= 16384; the norm is
  * that of h before it is rounded to sum's dtype.  Squares are summed in fp32 (in 64
- * bits for 8-bit results): values past 2^63 count as infinite.  out and sum may each be
- * x or residual itself, but not both the same. */
+ * bits for 8-bit results): values past 2^63 count as infinite, and squares of values below
+ * 2^-63 lose bits, which shows where eps is as small.  out and sum may each be x or
+ * residual itself, but not both the same. */
 int kk_rms_norm(const kk_tensor* out, const kk_tensor* sum, const kk_tensor* x,
                 const kk_tensor* residual, const kk_tensor* weight, float eps);
 /* The same into 8 bits for kk_matmul_integer_scaled, with a scale for each row:
