@@ -68,3 +68,17 @@ def test_a_batch_past_a_blocks_threads(gpu, t):
     for b in sorted({*far, *r.integers(0, B, 20).tolist()}):
         if lengths[b]:
             check(out[b], q[b], parts, table[b], int(lengths[b]), 0.2, what=f"sequence {b}")
+
+
+@pytest.mark.parametrize("T", [1, 20, 60, 200])
+@pytest.mark.parametrize("step,low", [(9000, 0), (65000, 65504), (65504, -65504), (2.0 ** -24, 60000), (0, -65504)])
+def test_values_of_fp16s_largest_sizes(gpu, T, step, low):
+    kk = gpu
+    r = rng(T)
+    dim, block, n = 96, 32, 333
+    table, pages = pool(r, 1, -(-n // block))
+    parts = filled(r, pages, 2, dim, block)
+    parts[3][r.random(parts[3].shape[:3]) < 0.2] = step, low
+    q = r.normal(size=(1, T, 4, dim)).astype(np.float32)
+    out = run(kk, q, parts, table, np.array([n], np.int32), scale=0.1)
+    check(out[0], q[0], parts, table[0], n, 0.1)
